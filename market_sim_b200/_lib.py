@@ -1,4 +1,5 @@
-"""ctypes binding of ``libmfhead.so`` (the C-ABI in ``include/mf_head.h``).
+"""ctypes binding of ``libmfhead.so`` (the C-ABI in ``include/mf_head.h`` and
+``include/mf_loss.h``).
 
 The library is the product: there is no Python or CPU fallback.  Importing
 this module fails loudly when the shared library is missing; build it with
@@ -70,8 +71,19 @@ _SIGNATURES["mf_pipeline_submit_packed_u16ids"] = _SIGNATURES["mf_pipeline_submi
 _SIGNATURES["mf_pipeline_wait"] = [_P, _U64]
 _SIGNATURES["mf_pipeline_synchronize"] = [_P]
 
+# losses over the tied table (include/mf_loss.h)
+for _t in ("f16", "bf16"):
+    _SIGNATURES["mf_dense_xent_" + _t] = [_P, _U64] * 6 + [_U64] * 3 + [_P]
+    _SIGNATURES["mf_dense_xent_backward_" + _t] = [_P, _U64] * 8 + [_U64] * 3 + [_P]
+    _SIGNATURES["mf_dense_distill_" + _t] = ([_P, _U64] * 5 + [ctypes.c_float] + [_P, _U64] * 3
+                                             + [_U64] * 3 + [_P])
+    _SIGNATURES["mf_dense_distill_backward_" + _t] = ([_P, _U64] * 5 + [ctypes.c_float]
+                                                      + [_P, _U64] * 5 + [_U64] * 3 + [_P])
+
 _U64_FUNCS = {"mf_head_workspace_bytes": [_U64], "mf_dfa_workspace_bytes": [_U64],
-              "mf_dense_workspace_bytes": [_U64], "mf_exchange_bytes": [_U64, ctypes.c_uint32]}
+              "mf_dense_workspace_bytes": [_U64], "mf_exchange_bytes": [_U64, ctypes.c_uint32],
+              "mf_dense_loss_workspace_bytes": [_U64] * 3,
+              "mf_dense_loss_backward_workspace_bytes": [_U64] * 3}
 _U32_FUNCS = {"mf_version": [], "mf_built_arch": [], "mf_pipeline_depth": [_P]}
 _PTR_FUNCS = {"mf_pipeline_stream": [_P, ctypes.c_uint32]}
 _VOID_FUNCS = {"mf_pipeline_destroy": [_P]}
@@ -116,6 +128,6 @@ def _load() -> ctypes.CDLL:
 
 lib = _load()
 
-#: every symbol include/mf_head.h declares (checked by the CPU test suite)
+#: every symbol include/mf_head.h and include/mf_loss.h declare (checked by the CPU test suite)
 EXPORTED = sorted(list(_SIGNATURES) + list(_U64_FUNCS) + list(_U32_FUNCS) + list(_PTR_FUNCS)
                   + list(_VOID_FUNCS))

@@ -526,6 +526,282 @@ class RaggedHead:
         return out_ids, out_scores
 
 
+# ---- losses over the tied table (include/mf_loss.h) ------------------------
+
+def dense_loss_workspace_bytes(rows: int, hidden_size: int, vocab: int) -> int:
+    """Workspace of the forward calls; 0 for sizes outside the limits."""
+    return int(lib.mf_dense_loss_workspace_bytes(rows, hidden_size, vocab))
+
+
+def dense_loss_backward_workspace_bytes(rows: int, hidden_size: int, vocab: int) -> int:
+    """Workspace of the backward calls; 0 for sizes outside the limits."""
+    return int(lib.mf_dense_loss_backward_workspace_bytes(rows, hidden_size, vocab))
+
+
+def _xent(f, hidden, embedding, targets, losses, lse, workspace, rows, hidden_size, vocab, stream):
+    return _status(f(*_pb(hidden), *_pb(embedding), *_pb(targets), *_pb(losses), *_pb(lse),
+                     *_pb(workspace), rows, hidden_size, vocab, _sp(stream)))
+
+
+def dense_xent_f16(hidden: Buffer, embedding: Buffer, targets: Buffer, losses: Buffer, lse: Buffer,
+                   workspace: Buffer, rows: int, hidden_size: int, vocab: int, stream) -> Status:
+    """Softmax cross entropy of each row's target over the whole vocabulary:
+    losses[r] = lse[r] - score(r, targets[r]).  INVALID_TOKEN_ID rows are
+    ignored (loss 0)."""
+    return _xent(lib.mf_dense_xent_f16, hidden, embedding, targets, losses, lse, workspace, rows,
+                 hidden_size, vocab, stream)
+
+
+def dense_xent_bf16(hidden: Buffer, embedding: Buffer, targets: Buffer, losses: Buffer, lse: Buffer,
+                    workspace: Buffer, rows: int, hidden_size: int, vocab: int, stream) -> Status:
+    """``dense_xent_f16`` on bfloat16 hidden rows and table."""
+    return _xent(lib.mf_dense_xent_bf16, hidden, embedding, targets, losses, lse, workspace, rows,
+                 hidden_size, vocab, stream)
+
+
+def _xent_backward(f, hidden, embedding, targets, lse, grad_losses, d_hidden, d_embedding,
+                   workspace, rows, hidden_size, vocab, stream):
+    return _status(f(*_pb(hidden), *_pb(embedding), *_pb(targets), *_pb(lse), *_pb(grad_losses),
+                     *_pb(d_hidden), *_pb(d_embedding), *_pb(workspace), rows, hidden_size, vocab,
+                     _sp(stream)))
+
+
+def dense_xent_backward_f16(hidden: Buffer, embedding: Buffer, targets: Buffer, lse: Buffer,
+                            grad_losses: Buffer, d_hidden: Optional[Buffer],
+                            d_embedding: Optional[Buffer], workspace: Buffer, rows: int,
+                            hidden_size: int, vocab: int, stream) -> Status:
+    """Gradients of sum(grad_losses * losses) of ``dense_xent_f16`` (either
+    output may be None)."""
+    return _xent_backward(lib.mf_dense_xent_backward_f16, hidden, embedding, targets, lse,
+                          grad_losses, d_hidden, d_embedding, workspace, rows, hidden_size, vocab,
+                          stream)
+
+
+def dense_xent_backward_bf16(hidden: Buffer, embedding: Buffer, targets: Buffer, lse: Buffer,
+                             grad_losses: Buffer, d_hidden: Optional[Buffer],
+                             d_embedding: Optional[Buffer], workspace: Buffer, rows: int,
+                             hidden_size: int, vocab: int, stream) -> Status:
+    """``dense_xent_backward_f16`` on bfloat16 hidden rows and table."""
+    return _xent_backward(lib.mf_dense_xent_backward_bf16, hidden, embedding, targets, lse,
+                          grad_losses, d_hidden, d_embedding, workspace, rows, hidden_size, vocab,
+                          stream)
+
+
+def _distill(f, hidden, embedding, offsets, ids, teacher_logits, temperature, losses, lse,
+             workspace, rows, hidden_size, vocab, stream):
+    return _status(f(*_pb(hidden), *_pb(embedding), *_pb(offsets), *_pb(ids), *_pb(teacher_logits),
+                     float(temperature), *_pb(losses), *_pb(lse), *_pb(workspace), rows,
+                     hidden_size, vocab, _sp(stream)))
+
+
+def dense_distill_f16(hidden: Buffer, embedding: Buffer, offsets: Buffer, ids: Optional[Buffer],
+                      teacher_logits: Optional[Buffer], temperature: float, losses: Buffer,
+                      lse: Buffer, workspace: Buffer, rows: int, hidden_size: int, vocab: int,
+                      stream) -> Status:
+    """Distillation from a teacher's top logits: row r's entries are
+    [offsets[r], offsets[r+1]) of ids (ascending) and teacher_logits;
+    losses[r] = T^2 KL(teacher over its set || student over the vocabulary)."""
+    return _distill(lib.mf_dense_distill_f16, hidden, embedding, offsets, ids, teacher_logits,
+                    temperature, losses, lse, workspace, rows, hidden_size, vocab, stream)
+
+
+def dense_distill_bf16(hidden: Buffer, embedding: Buffer, offsets: Buffer, ids: Optional[Buffer],
+                       teacher_logits: Optional[Buffer], temperature: float, losses: Buffer,
+                       lse: Buffer, workspace: Buffer, rows: int, hidden_size: int, vocab: int,
+                       stream) -> Status:
+    """``dense_distill_f16`` on bfloat16 hidden rows and table."""
+    return _distill(lib.mf_dense_distill_bf16, hidden, embedding, offsets, ids, teacher_logits,
+                    temperature, losses, lse, workspace, rows, hidden_size, vocab, stream)
+
+
+def _distill_backward(f, hidden, embedding, offsets, ids, teacher_logits, temperature, lse,
+                      grad_losses, d_hidden, d_embedding, workspace, rows, hidden_size, vocab,
+                      stream):
+    return _status(f(*_pb(hidden), *_pb(embedding), *_pb(offsets), *_pb(ids), *_pb(teacher_logits),
+                     float(temperature), *_pb(lse), *_pb(grad_losses), *_pb(d_hidden),
+                     *_pb(d_embedding), *_pb(workspace), rows, hidden_size, vocab, _sp(stream)))
+
+
+def dense_distill_backward_f16(hidden: Buffer, embedding: Buffer, offsets: Buffer,
+                               ids: Optional[Buffer], teacher_logits: Optional[Buffer],
+                               temperature: float, lse: Buffer, grad_losses: Buffer,
+                               d_hidden: Optional[Buffer], d_embedding: Optional[Buffer],
+                               workspace: Buffer, rows: int, hidden_size: int, vocab: int,
+                               stream) -> Status:
+    """Gradients of sum(grad_losses * losses) of ``dense_distill_f16`` (either
+    output may be None)."""
+    return _distill_backward(lib.mf_dense_distill_backward_f16, hidden, embedding, offsets, ids,
+                             teacher_logits, temperature, lse, grad_losses, d_hidden, d_embedding,
+                             workspace, rows, hidden_size, vocab, stream)
+
+
+def dense_distill_backward_bf16(hidden: Buffer, embedding: Buffer, offsets: Buffer,
+                                ids: Optional[Buffer], teacher_logits: Optional[Buffer],
+                                temperature: float, lse: Buffer, grad_losses: Buffer,
+                                d_hidden: Optional[Buffer], d_embedding: Optional[Buffer],
+                                workspace: Buffer, rows: int, hidden_size: int, vocab: int,
+                                stream) -> Status:
+    """``dense_distill_backward_f16`` on bfloat16 hidden rows and table."""
+    return _distill_backward(lib.mf_dense_distill_backward_bf16, hidden, embedding, offsets, ids,
+                             teacher_logits, temperature, lse, grad_losses, d_hidden, d_embedding,
+                             workspace, rows, hidden_size, vocab, stream)
+
+
+class DenseLoss:
+    """Owns the workspace for repeated loss calls on one stream.
+
+    ``embedding`` (fp16 or bfloat16 [vocab, hidden_size], contiguous) stays
+    resident and is read in place, so an optimizer may update it between
+    calls.  Forward methods return ``(losses, lse)``, backward methods
+    ``(d_hidden, d_embedding)``; outputs are allocated unless given, and a
+    gradient is left out (None) with ``hidden_grad=False`` /
+    ``embedding_grad=False``.  With ``backward=False`` only the forward
+    workspace is kept.  ``stream`` defaults to the current stream, which must
+    not be the legacy default stream; tensors made on another stream have to
+    be ordered before the call (``Stream.wait_stream``).  Calls of one object
+    share its workspace: they must not overlap on the GPU.
+    """
+
+    def __init__(self, embedding, max_rows: int, stream=None, backward: bool = True):
+        import torch
+
+        kinds = {torch.float16: "f16", torch.bfloat16: "bf16"}
+        if embedding.dtype not in kinds or embedding.dim() != 2:
+            raise ValueError("the table is fp16 or bfloat16 [vocab, hidden_size]")
+        self.embedding = embedding
+        self.vocab, self.hidden_size = int(embedding.shape[0]), int(embedding.shape[1])
+        self.max_rows, self.stream = int(max_rows), stream
+        sizes = (self.max_rows, self.hidden_size, self.vocab)
+        nbytes = dense_loss_workspace_bytes(*sizes)
+        if nbytes == 0:
+            raise ValueError(f"rows, hidden_size, vocab = {sizes} are outside the limits")
+        if backward:
+            nbytes = max(nbytes, dense_loss_backward_workspace_bytes(*sizes))
+        self._backward = backward
+        kind = kinds[embedding.dtype]
+        names = globals()
+        self._xent, self._xent_backward, self._distill, self._distill_backward = (
+            names[f"dense_{n}_{kind}"] for n in ("xent", "xent_backward", "distill",
+                                                 "distill_backward"))
+        self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=embedding.device)
+
+    def _tensor(self, name, t, dtype, shape):
+        if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() \
+                or t.device != self.embedding.device:
+            raise ValueError(f"{name}: a contiguous {dtype} tensor of shape {shape} on "
+                             f"{self.embedding.device} is wanted, not {t.dtype} {tuple(t.shape)} "
+                             f"on {t.device}")
+        return t
+
+    def _given(self, name, t, dtype, shape):
+        import torch
+
+        if t is None:  # from the memory of the stream that writes it
+            with torch.cuda.device(self.embedding.device), torch.cuda.stream(self._on()):
+                return torch.empty(shape, dtype=dtype, device=self.embedding.device)
+        return self._tensor(name, t, dtype, shape)
+
+    def _on(self):
+        import torch
+
+        if self.stream is None:
+            return torch.cuda.current_stream(self.embedding.device)
+        return _torch_stream(self.stream)
+
+    def _rows(self, hidden):
+        rows = int(hidden.shape[0])
+        if rows > self.max_rows:
+            raise ValueError(f"batch of {rows} rows exceeds max_rows={self.max_rows}")
+        self._tensor("hidden", hidden, self.embedding.dtype, (rows, self.hidden_size))
+        self._tensor("embedding", self.embedding, self.embedding.dtype,
+                     (self.vocab, self.hidden_size))
+        return rows
+
+    def _sets(self, rows, offsets, ids, teacher_logits):
+        import torch
+
+        self._tensor("offsets", offsets, torch.int32, (rows + 1,))
+        self._tensor("ids", ids, torch.int32, (ids.numel(),))
+        self._tensor("teacher_logits", teacher_logits, torch.float32, (ids.numel(),))
+        return offsets, ids, teacher_logits
+
+    def _call(self, f, *args):
+        import torch
+
+        with torch.cuda.device(self.embedding.device):
+            st = f(*args, self._on())
+        if not st.ok():
+            raise RuntimeError(f"{f.__name__} failed: {st}")
+
+    def cross_entropy(self, hidden, targets, losses=None, lse=None):
+        """targets int32 [rows]; -1 (``INVALID_TOKEN_ID``) ignores a row."""
+        import torch
+
+        rows = self._rows(hidden)
+        self._tensor("targets", targets, torch.int32, (rows,))
+        losses = self._given("losses", losses, torch.float32, (rows,))
+        lse = self._given("lse", lse, torch.float32, (rows,))
+        self._call(self._xent, hidden, self.embedding, targets, losses, lse, self.workspace, rows,
+                   self.hidden_size, self.vocab)
+        return losses, lse
+
+    def distill(self, hidden, offsets, ids, teacher_logits, temperature=1.0, losses=None,
+                lse=None):
+        """The teacher's top logits as CSR: offsets int32 [rows + 1], ids int32
+        (ascending within a row) and teacher_logits float32 [entries]."""
+        import torch
+
+        rows = self._rows(hidden)
+        sets = self._sets(rows, offsets, ids, teacher_logits)
+        losses = self._given("losses", losses, torch.float32, (rows,))
+        lse = self._given("lse", lse, torch.float32, (rows,))
+        self._call(self._distill, hidden, self.embedding, *sets, temperature, losses, lse,
+                   self.workspace, rows, self.hidden_size, self.vocab)
+        return losses, lse
+
+    def _gradients(self, rows, lse, grad_losses, d_hidden, d_embedding, hidden_grad,
+                   embedding_grad):
+        import torch
+
+        if not self._backward:
+            raise RuntimeError("this DenseLoss was made with backward=False")
+        self._tensor("lse", lse, torch.float32, (rows,))
+        self._tensor("grad_losses", grad_losses, torch.float32, (rows,))
+        kind = self.embedding.dtype
+        if hidden_grad:
+            d_hidden = self._given("d_hidden", d_hidden, kind, (rows, self.hidden_size))
+        if embedding_grad:
+            d_embedding = self._given("d_embedding", d_embedding, kind,
+                                      (self.vocab, self.hidden_size))
+        return (d_hidden if hidden_grad else None), (d_embedding if embedding_grad else None)
+
+    def cross_entropy_backward(self, hidden, targets, lse, grad_losses, d_hidden=None,
+                               d_embedding=None, hidden_grad=True, embedding_grad=True):
+        """Gradients of ``(grad_losses * losses).sum()``; ``lse`` as
+        ``cross_entropy`` returned it."""
+        import torch
+
+        rows = self._rows(hidden)
+        self._tensor("targets", targets, torch.int32, (rows,))
+        out = self._gradients(rows, lse, grad_losses, d_hidden, d_embedding, hidden_grad,
+                              embedding_grad)
+        self._call(self._xent_backward, hidden, self.embedding, targets, lse, grad_losses, *out,
+                   self.workspace, rows, self.hidden_size, self.vocab)
+        return out
+
+    def distill_backward(self, hidden, offsets, ids, teacher_logits, temperature, lse, grad_losses,
+                         d_hidden=None, d_embedding=None, hidden_grad=True, embedding_grad=True):
+        """Gradients of ``(grad_losses * losses).sum()``; ``lse`` as ``distill``
+        returned it with the same temperature."""
+        rows = self._rows(hidden)
+        sets = self._sets(rows, offsets, ids, teacher_logits)
+        out = self._gradients(rows, lse, grad_losses, d_hidden, d_embedding, hidden_grad,
+                              embedding_grad)
+        self._call(self._distill_backward, hidden, self.embedding, *sets, temperature, lse,
+                   grad_losses, *out, self.workspace, rows, self.hidden_size, self.vocab)
+        return out
+
+
 class HostPipeline:
     """Restricted head over batches that live in host memory (native
     ``mf_pipeline_*``): each ``submit`` copies one batch (hidden rows, CSR
