@@ -60,13 +60,14 @@
 extern "C" {
 #endif
 
-#define MF_LOSS_MAX_ROWS (1u << 22)
+#define MF_LOSS_MAX_ROWS (1u << 20)
 #define MF_LOSS_MAX_VOCAB (1u << 24)
 #define MF_LOSS_MAX_HIDDEN 8192u
 
 /* Bytes of device memory a forward call and a backward call need; 0 for sizes
- * outside the limits.  A backward call's workspace is at most about 256 MiB (one piece of
- * d) + rows x hidden_size x 6, larger only for more than 512 Ki rows. */
+ * outside the limits.  A backward call's holds two pieces of d of at most 128
+ * MiB (512 bytes a row above 256 Ki rows), a copy of the hidden rows and a few
+ * FP32 sums of d_hidden. */
 MF_API uint64_t mf_dense_loss_workspace_bytes(uint64_t rows, uint64_t hidden_size, uint64_t vocab);
 MF_API uint64_t mf_dense_loss_backward_workspace_bytes(uint64_t rows, uint64_t hidden_size,
                                                        uint64_t vocab);

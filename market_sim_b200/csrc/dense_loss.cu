@@ -2,41 +2,88 @@
 // entropy over the whole vocabulary and distillation from a teacher's top
 // logits, with their gradients.
 //
-// Plain version: 64 x 64 tiles on the FP32 pipes.
+// Forward, one pass: scores S = H E^T tile by tile on the tensor cores; each
+// row keeps a running maximum m and sum l = sum exp(s - m) in registers while
+// its pair of CTAs walks the vocabulary, and picks the wanted columns' scores
+// out of the accumulator; a small kernel joins the walks.
+// Backward: the scores again, a piece of the vocabulary at a time, turned into
+// d = T g (p - q) in the epilogue and stored in 16 bits (a piece, never all of
+// it), then two products on the piece: d E into FP32 sums of d_hidden and
+// d^T H into d_embedding.  One launch makes piece i + 1 of d and the products
+// of piece i, so the many small score tiles fill the SMs that the long product
+// tiles leave idle; a last kernel joins and rounds d_hidden.
+//
+// All three products are one engine: tile = 256 rows (M) x up to 256 columns
+// (N) on a pair of CTAs (tcgen05 cta_group::2), K in chunks of 64 through a
+// ring of shared-memory stages filled by TMA, two accumulators in TMEM so that
+// one drains while the next fills.  A persistent grid of one pair per two SMs;
+// each pair works through fixed ranges of tiles chosen on the host.
+//   S  = H E^T   A = hidden rows (K-major), B = table rows (K-major)
+//   d E          A = d (K-major),           B = table piece (N-major)
+//   d^T H        A = d (M-major),           B = scaled hidden copy (N-major)
+// Every mbarrier wait is bounded; a pair whose wait runs out writes NaN into
+// what is left of its tiles, drains its copies and returns.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <initializer_list>
+#include <mutex>
 
 #include "common.cuh"
 #include "mf_loss.h"
+#include "tcgen05.cuh"
 
 namespace mfb {
 namespace loss {
 
-constexpr int kTile = 64;
-constexpr int kStep = 16;
-constexpr int kThreads = 256;
-constexpr uint32_t kWorkers = 148;                 // forward: walks over the vocabulary
-constexpr uint64_t kPieceBytes = 256ull << 20;     // one piece of d
+constexpr int kBM = 128;       // rows of a tile per CTA (256 per pair)
+constexpr int kBN = 256;       // columns of a score tile
+constexpr int kBK = 64;        // K elements per chunk
+constexpr int kStages = 6;
+constexpr int kAChunk = kBM * kBK * 2;        // 16 KB per CTA
+constexpr int kBChunk = kBN / 2 * kBK * 2;    // at most 16 KB per CTA
+constexpr int kEpiWarps = 8;   // two per TMEM lane quadrant, each on half the columns
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr uint32_t kTmemCols = 512;
+constexpr int kSetupThreads = 256;
+constexpr uint32_t kMaxPairs = 74;             // pairs of the persistent grid
+constexpr uint64_t kPieceBytes = 128ull << 20; // one piece of d
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 
 template <typename T>
 struct Type;
 template <>
 struct Type<__half> {
-  // d / gmax is at most 1: times 2^15 it uses fp16's whole range, and keeps
-  // full precision down to 2^-29 of the largest weight
+  // d / (largest weight) is at most 1: times 2^15 it uses fp16's whole range,
+  // and keeps full precision down to 2^-29 of the largest weight
   static constexpr float kScale = 32768.f;
+  static constexpr uint32_t kFormat = 0;  // of the instruction descriptor
+  static constexpr CUtensorMapDataType kMap = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   static __device__ __forceinline__ float to(__half x) { return __half2float(x); }
   static __device__ __forceinline__ __half from(float x) { return __float2half_rn(x); }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
 };
 template <>
 struct Type<__nv_bfloat16> {
   static constexpr float kScale = 1.f;
+  static constexpr uint32_t kFormat = 1;
+  static constexpr CUtensorMapDataType kMap = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   static __device__ __forceinline__ float to(__nv_bfloat16 x) { return __bfloat162float(x); }
   static __device__ __forceinline__ __nv_bfloat16 from(float x) { return __float2bfloat16_rn(x); }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
 };
 
 // What a row wants: one target, or a teacher's set.
@@ -53,12 +100,16 @@ struct Wanted {
 __device__ __forceinline__ bool stat_empty(float2 s) { return s.x == -INFINITY; }
 __device__ __forceinline__ bool stat_invalid(float2 s) { return s.x != s.x; }
 
-struct Partial {  // of one row over one walk: running max, sum of exp, sum of q s
-  float m, l, dot;
+// Of one row over one walk through the vocabulary, half of every tile's
+// columns: the largest score in units of ln 2, the sum of exp relative to it,
+// the sum of q s / T.
+struct __align__(16) Partial {
+  float m, l, dot, unused;
 };
 
 // One warp per row: the teacher's normaliser and entropy.
 __global__ void teacher_kernel(Wanted w, uint32_t rows, uint32_t entries, uint32_t vocab) {
+  pdl_trigger();
   const uint32_t lane = threadIdx.x & 31;
   for (uint32_t r = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; r < rows;
        r += (gridDim.x * blockDim.x) >> 5) {
@@ -106,116 +157,6 @@ __device__ __forceinline__ int32_t first_entry(const Wanted& w, uint32_t r, uint
   return lo;
 }
 
-// acc[i][j] = sum_k A(m0 + ty + 16 i, k) B(n0 + tx + 16 j, k); A(m, k) is
-// a[m * am + k * ak], zero outside [0, M) x [0, K); B likewise.
-template <typename T>
-__device__ __forceinline__ void tile_product(float (&acc)[4][4], const T* a, uint64_t am,
-                                             uint64_t ak, const T* b, uint64_t bn, uint64_t bk,
-                                             uint32_t m0, uint32_t M, uint32_t n0, uint32_t N,
-                                             uint32_t K, float (*sa)[kTile + 1],
-                                             float (*sb)[kTile + 1]) {
-  const uint32_t tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-  for (uint32_t k0 = 0; k0 < K; k0 += kStep) {
-    for (uint32_t e = threadIdx.x; e < kTile * kStep; e += kThreads) {
-      // neighbouring threads along whichever index is contiguous
-      const uint32_t ia = ak == 1 ? e / kStep : e % kTile, ka = ak == 1 ? e % kStep : e / kTile;
-      const uint32_t ib = bk == 1 ? e / kStep : e % kTile, kb = bk == 1 ? e % kStep : e / kTile;
-      sa[ka][ia] = (m0 + ia < M && k0 + ka < K)
-                       ? Type<T>::to(a[(uint64_t)(m0 + ia) * am + (uint64_t)(k0 + ka) * ak]) : 0.f;
-      sb[kb][ib] = (n0 + ib < N && k0 + kb < K)
-                       ? Type<T>::to(b[(uint64_t)(n0 + ib) * bn + (uint64_t)(k0 + kb) * bk]) : 0.f;
-    }
-    __syncthreads();
-    for (int k = 0; k < kStep; ++k)
-      for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j)
-          acc[i][j] = fmaf(sa[k][ty + 16 * i], sb[k][tx + 16 * j], acc[i][j]);
-    __syncthreads();
-  }
-}
-
-// Forward: block (m, split) walks its share of the vocabulary tiles for 64 rows.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) forward_kernel(const T* hidden, const T* emb, Wanted w,
-                                                           Partial* out, uint32_t rows,
-                                                           uint32_t width, uint32_t vocab,
-                                                           uint32_t splits) {
-  __shared__ float sa[kStep][kTile + 1], sb[kStep][kTile + 1], st[kTile][kTile + 1];
-  const uint32_t m0 = blockIdx.x * kTile, split = blockIdx.y;
-  const uint32_t tiles = (vocab + kTile - 1) / kTile;
-  const uint32_t t0 = (uint32_t)((uint64_t)tiles * split / splits);
-  const uint32_t t1 = (uint32_t)((uint64_t)tiles * (split + 1) / splits);
-  const uint32_t tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const uint32_t r = m0 + threadIdx.x;
-  const bool owner = threadIdx.x < kTile && r < rows;
-  Partial p{-INFINITY, 0.f, 0.f};
-  uint32_t target = kInvalid;
-  int32_t at = 0, end = 0;
-  float tlse = 0.f;
-  if (owner && w.targets) target = w.targets[r];
-  if (owner && w.offsets) {
-    const float2 s = w.stat[r];
-    if (!stat_empty(s) && !stat_invalid(s)) {
-      at = first_entry(w, r, t0 * kTile);
-      end = w.offsets[r + 1];
-      tlse = s.x;
-    }
-  }
-  for (uint32_t t = t0; t < t1; ++t) {
-    float acc[4][4];
-    tile_product(acc, hidden, width, 1, emb, width, 1, m0, rows, t * kTile, vocab, width, sa, sb);
-    for (int i = 0; i < 4; ++i)
-      for (int j = 0; j < 4; ++j) st[ty + 16 * i][tx + 16 * j] = acc[i][j] * w.inv_t;
-    __syncthreads();
-    if (owner) {
-      const uint32_t n = min((uint32_t)kTile, vocab - t * kTile);
-      float m = p.m;
-      for (uint32_t c = 0; c < n; ++c) m = fmaxf(m, st[threadIdx.x][c]);
-      float l = p.l * (p.m == m ? 1.f : expf(p.m - m));
-      for (uint32_t c = 0; c < n; ++c) l += expf(st[threadIdx.x][c] - m);
-      p.m = m;
-      p.l = l;
-      if (w.targets && target - t * kTile < n) p.dot = st[threadIdx.x][target - t * kTile];
-      for (; at < end && (uint32_t)w.ids[at] < t * kTile + n; ++at) {
-        const float q = expf(w.logits[at] * w.inv_t - tlse);
-        if (q > 0.f) p.dot = fmaf(q, st[threadIdx.x][w.ids[at] - t * kTile], p.dot);
-      }
-    }
-    __syncthreads();
-  }
-  if (owner) out[(uint64_t)r * splits + split] = p;
-}
-
-// One thread per row joins the walks' partial sums.
-__global__ void merge_kernel(Wanted w, const Partial* part, uint32_t splits, uint32_t rows,
-                             uint32_t vocab, float* losses, float* lse) {
-  const uint32_t r = blockIdx.x * blockDim.x + threadIdx.x;
-  if (r >= rows) return;
-  float m = -INFINITY, l = 0.f, dot = 0.f;
-  for (uint32_t s = 0; s < splits; ++s) m = fmaxf(m, part[(uint64_t)r * splits + s].m);
-  for (uint32_t s = 0; s < splits; ++s) {
-    const Partial p = part[(uint64_t)r * splits + s];
-    l += p.l * (p.m == m ? 1.f : expf(p.m - m));
-    dot += p.dot;
-  }
-  const float z = m + logf(l);
-  lse[r] = z;
-  float loss;
-  if (w.targets) {
-    const uint32_t t = w.targets[r];
-    loss = t == kInvalid ? 0.f : (t >= vocab ? __uint_as_float(0x7FC00000u) : z - dot);
-  } else {
-    const float2 s = w.stat[r];
-    const float t = 1.f / w.inv_t;
-    loss = stat_empty(s) ? 0.f : (stat_invalid(s) ? s.x : t * t * (s.y + (z - dot)));
-  }
-  losses[r] = loss;
-}
-
-// ---- backward ----------------------------------------------------------
-
 struct RowGrad {  // one row's factors of d
   float coef;     // d16 = (p - q) * coef
   float scale;    // d_hidden = (d16 . E) * scale
@@ -230,20 +171,23 @@ __device__ __forceinline__ float row_weight(const Wanted& w, const float* grad, 
 
 // Row factors and the copy of the hidden rows that d_embedding is made of.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) setup_kernel(Wanted w, const float* grad,
-                                                         const T* hidden, T* scaled, RowGrad* rg,
-                                                         float* gmax_out, uint32_t rows,
-                                                         uint32_t width, uint32_t vocab) {
-  __shared__ float s_max[kThreads / 32];
+__global__ void __launch_bounds__(kSetupThreads) setup_kernel(Wanted w, const float* grad,
+                                                              const T* hidden, T* scaled,
+                                                              RowGrad* rg, float* gmax_out,
+                                                              uint32_t rows, uint32_t width,
+                                                              uint32_t vocab) {
+  __shared__ float s_max[kSetupThreads / 32];
+  pdl_trigger();
+  pdl_wait();
   float g = 0.f;
-  for (uint32_t r = threadIdx.x; r < rows; r += kThreads) {
+  for (uint32_t r = threadIdx.x; r < rows; r += kSetupThreads) {
     const float a = fabsf(row_weight(w, grad, r, vocab));
     if (a < INFINITY) g = fmaxf(g, a);  // an infinite weight spoils its own row only
   }
   for (int o = 16; o; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
   if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = g;
   __syncthreads();
-  for (int i = 0; i < kThreads / 32; ++i) g = fmaxf(g, s_max[i]);
+  for (int i = 0; i < kSetupThreads / 32; ++i) g = fmaxf(g, s_max[i]);
   if (blockIdx.x == 0 && threadIdx.x == 0) *gmax_out = g;
   for (uint32_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const float wr = row_weight(w, grad, r, vocab);
@@ -258,94 +202,637 @@ __global__ void __launch_bounds__(kThreads) setup_kernel(Wanted w, const float* 
     }
     if (threadIdx.x == 0)
       rg[r] = RowGrad{mant * Type<T>::kScale, g * two_e / Type<T>::kScale};
-    for (uint32_t c = threadIdx.x; c < width; c += kThreads)
+    for (uint32_t c = threadIdx.x; c < width; c += kSetupThreads)
       scaled[(uint64_t)r * width + c] =
           wr == 0.f ? Type<T>::from(0.f)
                     : Type<T>::from(Type<T>::to(hidden[(uint64_t)r * width + c]) * two_e);
   }
 }
 
-// One piece of d: columns [v0, v0 + n_cols) for 64 rows x 64 columns a block.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) piece_kernel(const T* hidden, const T* emb, Wanted w,
-                                                         const float* lse, const RowGrad* rg, T* d,
-                                                         uint32_t pitch, uint32_t rows,
-                                                         uint32_t width, uint32_t v0,
-                                                         uint32_t n_cols) {
-  __shared__ float sa[kStep][kTile + 1], sb[kStep][kTile + 1], st[kTile][kTile + 1];
-  const uint32_t m0 = blockIdx.x * kTile, n0 = blockIdx.y * kTile;
-  const uint32_t tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const uint32_t r = m0 + threadIdx.x;
-  float acc[4][4];
-  tile_product(acc, hidden, width, 1, emb + (uint64_t)v0 * width, width, 1, m0, rows, n0, n_cols,
-               width, sa, sb);
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) st[ty + 16 * i][tx + 16 * j] = acc[i][j] * w.inv_t;
+
+// ---- the tile engine ----------------------------------------------------
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 32 TMEM lanes x 32 consecutive f32 columns -> 32 registers per thread.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void store_v8(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// Shared-memory descriptor of an operand whose M or N index is contiguous:
+// atoms of `atom_bytes` (128: SWIZZLE_128B, 64: SWIZZLE_64B) x 8 k, k groups
+// 8 atom_bytes apart (SBO), atoms one 64-k box apart (LBO), version 1 (sm_100).
+__device__ __forceinline__ uint64_t mn_desc(uint32_t addr, uint32_t atom_bytes) {
+  uint64_t d = 0;
+  d |= (uint64_t)((addr >> 4) & 0x3FFFu);
+  d |= (uint64_t)((kBK * atom_bytes) >> 4) << 16;
+  d |= (uint64_t)((8 * atom_bytes) >> 4) << 32;
+  d |= 1ull << 46;
+  d |= (atom_bytes == 128 ? 2ull : 4ull) << 61;
+  return d;
+}
+
+__device__ __forceinline__ void mma_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
+                                         uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+struct Maps {
+  CUtensorMap hidden, table;   // K-major score operands, 64 x 128 boxes
+  CUtensorMap d_k, table_n;    // d E: 64 x 128 and 32 x 64 boxes
+  CUtensorMap d_m, scaled_n;   // d^T H: 64 x 64 and 32 x 64 boxes
+};
+
+enum : uint32_t { kScore = 0, kHidden = 1, kTable = 2 };
+
+struct Params {
+  uint32_t rows, width, vocab;
+  uint32_t m_tiles;             // 256-row tiles of the batch
+  uint32_t w_chunks;            // ceil(width / 64)
+  // score tiles: vocabulary rows [v0, v0 + cols)
+  uint32_t v0, cols, n_tiles;
+  Partial* partial;             // forward: [2 slots][rows]
+  void* d;                      // backward: the piece being made
+  uint32_t pitch;
+  const float* lse;
+  const RowGrad* rg;
+  // product tiles: vocabulary rows [pv0, pv0 + pcols)
+  uint32_t pv0, pcols, bn, bn_tiles;
+  uint32_t p_chunks, per_split;  // d E: K chunks of the piece, and of one split
+  float* planes;                 // [splits][rows][width]
+  uint32_t add;                  // planes hold earlier pieces' sums
+  uint32_t r_chunks;             // d^T H: K chunks of the batch
+  void* table_out;               // d_embedding + pv0 rows
+  const float* gmax;
+  // per pair: tile ranges of the three kinds
+  uint32_t hidden_at[kMaxPairs + 1], table_at[kMaxPairs + 1], score_at[kMaxPairs + 1];
+};
+
+struct Smem {
+  static constexpr int a = 0;
+  static constexpr int b = kStages * kAChunk;
+  static constexpr int bars = b + kStages * kBChunk;
+  // barriers: full[S], empty[S], acc_full[2], acc_empty[2], drain
+  static constexpr int n_bars = 2 * kStages + 5;
+  static constexpr int tmem_slot = bars + n_bars * 8;
+  static constexpr int abort_flag = tmem_slot + 4;
+  static constexpr int issued = abort_flag + 4;  // u32[kStages]: loads issued per stage
+  static constexpr int size = issued + 4 * kStages;
+};
+constexpr size_t kSmemBytes = Smem::size + 1024;  // + alignment slack
+static_assert(kSmemBytes <= 227 * 1024, "shared memory");
+
+struct Tile {
+  uint32_t kind, m, n, k0, chunks, split;
+};
+
+// The tiles of one pair, in order: d E, d^T H, scores.
+struct Walk {
+  uint32_t h0, nh, t0, nt, s0, ns;
+  __device__ __forceinline__ Walk(const Params& p, uint32_t pair) {
+    h0 = p.hidden_at[pair];
+    nh = p.hidden_at[pair + 1] - h0;
+    t0 = p.table_at[pair];
+    nt = p.table_at[pair + 1] - t0;
+    s0 = p.score_at[pair];
+    ns = p.score_at[pair + 1] - s0;
+  }
+  __device__ __forceinline__ uint32_t count() const { return nh + nt + ns; }
+  __device__ __forceinline__ Tile at(const Params& p, uint32_t i) const {
+    Tile t;
+    t.k0 = 0;
+    t.split = 0;
+    if (i < nh) {
+      const uint32_t x = h0 + i, y = x / p.bn_tiles;
+      t.kind = kHidden;
+      t.n = x % p.bn_tiles;
+      t.m = y % p.m_tiles;
+      t.split = y / p.m_tiles;
+      t.k0 = t.split * p.per_split;
+      t.chunks = min(p.per_split, p.p_chunks - t.k0);
+    } else if (i < nh + nt) {
+      const uint32_t x = t0 + i - nh;
+      t.kind = kTable;
+      t.n = x % p.bn_tiles;
+      t.m = x / p.bn_tiles;
+      t.chunks = p.r_chunks;
+    } else {
+      const uint32_t x = s0 + i - nh - nt;
+      t.kind = kScore;
+      t.n = x % p.n_tiles;
+      t.m = x / p.n_tiles;
+      t.chunks = p.w_chunks;
+    }
+    return t;
+  }
+};
+
+// The wanted columns of one row, ascending, through a window of four.
+template <bool kDistill>
+struct Cursor {
+  uint32_t id[kDistill ? 4 : 1];
+  float t[kDistill ? 4 : 1];
+  int32_t at, end;
+
+  __device__ __forceinline__ void none() {
+    id[0] = 0xFFFFFFFFu;
+    at = end = 0;
+    if constexpr (kDistill) id[1] = id[2] = id[3] = 0xFFFFFFFFu;
+  }
+  // Row r from its first entry >= v on.
+  __device__ __forceinline__ void start(const Wanted& w, uint32_t r, uint32_t v, bool live) {
+    none();
+    if (!live) return;
+    if constexpr (kDistill) {
+      at = first_entry(w, r, v);
+      end = w.offsets[r + 1];
+    } else {
+      id[0] = w.targets[r];
+    }
+  }
+  __device__ __forceinline__ void pop() {
+    if constexpr (kDistill) {
+#pragma unroll
+      for (int i = 0; i < 3; ++i) id[i] = id[i + 1], t[i] = t[i + 1];
+      id[3] = 0xFFFFFFFFu;
+    } else {
+      id[0] = 0xFFFFFFFFu;
+    }
+  }
+  __device__ __forceinline__ void fill(const Wanted& w) {
+    if constexpr (kDistill) {
+      int n = 0;  // slots in use
+#pragma unroll
+      for (int i = 0; i < 4; ++i) n += id[i] != 0xFFFFFFFFu;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int32_t k = at + i - n;
+        if (i >= n && k < end) id[i] = (uint32_t)w.ids[k], t[i] = w.logits[k];
+      }
+      at = min(end, at + 4 - n);
+    }
+  }
+  // Drops entries below v and tops the window up.
+  __device__ __forceinline__ void skip_to(const Wanted& w, uint32_t v) {
+    if constexpr (kDistill) {
+      fill(w);
+      while (id[0] < v) next(w);
+    }
+  }
+  __device__ __forceinline__ void next(const Wanted& w) {
+    pop();
+    if constexpr (kDistill)
+      if (id[0] == 0xFFFFFFFFu && at < end) fill(w);
+  }
+  // The weight of the first entry; `tlse2` in units of ln 2.
+  __device__ __forceinline__ float weight(float c2, float tlse2) const {
+    if constexpr (kDistill) return exp2_approx(fmaf(t[0], c2, -tlse2));
+    return 1.f;
+  }
+};
+
+// r[i] for an index that differs from lane to lane (63 selects).
+__device__ __forceinline__ float pick64(const uint32_t (&r)[64], uint32_t i) {
+  uint32_t a[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) a[j] = (i & 32u) ? r[j + 32] : r[j];
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1)
+#pragma unroll
+    for (int j = 0; j < s; ++j) a[j] = (i & (uint32_t)s) ? a[j + s] : a[j];
+  return __uint_as_float(a[0]);
+}
+
+template <typename T, bool kForward, bool kDistill>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p, Wanted w) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* sm = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(sm);
+  const uint32_t bar0 = sbase + Smem::bars;
+  auto full = [&](uint32_t s) { return bar0 + 8 * s; };
+  auto empty = [&](uint32_t s) { return bar0 + 8 * (kStages + s); };
+  auto acc_full = [&](uint32_t b) { return bar0 + 8 * (2 * kStages + b); };
+  auto acc_empty = [&](uint32_t b) { return bar0 + 8 * (2 * kStages + 2 + b); };
+  const uint32_t drain = bar0 + 8 * (2 * kStages + 4);
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(sm + Smem::abort_flag);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + Smem::tmem_slot);
+  volatile uint32_t* issued = reinterpret_cast<volatile uint32_t*>(sm + Smem::issued);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t rank;  // 0 = leader (issues the MMAs), 1 = peer
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const bool leader = rank == 0;
+  const uint32_t pair = blockIdx.x >> 1;
+  pdl_trigger();
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      bar_init(full(s), 1);
+      bar_init(empty(s), 1);
+      issued[s] = 0u;
+    }
+    for (int b = 0; b < 2; ++b) {
+      bar_init(acc_full(b), 1);
+      bar_init(acc_empty(b), 2 * kEpiWarps);  // leader's: one arrival per epilogue warp of the pair
+    }
+    bar_init(drain, 1);
+    *abort_flag = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  cluster_sync();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const Walk walk(p, pair);
+  const uint32_t tiles = walk.count();
+  pdl_wait();  // the previous kernel's results, before any bounded wait begins
+
+  if (warp == 0) {
+    // ---- producer: both CTAs load their halves; the copies complete on the
+    // leader's barriers, whose expected byte counts cover both ----
+    if (lane == 0) {
+      uint32_t it = 0;
+      for (uint32_t i = 0; i < tiles && !*abort_flag; ++i) {
+        const Tile t = walk.at(p, i);
+        const uint32_t b_bytes = t.kind == kScore ? (uint32_t)kBChunk : p.bn * kBK;
+        const int arow = (int)(t.m * 2 * kBM + rank * kBM);
+        const int bcol = t.kind == kScore ? (int)(p.v0 + t.n * kBN + rank * (kBN / 2))
+                                          : (int)(t.n * p.bn + rank * (p.bn / 2));
+        for (uint32_t kc = 0; kc < t.chunks; ++kc, ++it) {
+          const uint32_t s = it % kStages;
+          if (!bar_wait(empty(s), ((it / kStages) & 1u) ^ 1u)) {
+            *abort_flag = 1u;
+            break;
+          }
+          const uint32_t bar = mapa(full(s), 0);
+          const uint32_t a = sbase + Smem::a + s * kAChunk, b = sbase + Smem::b + s * kBChunk;
+          if (leader) bar_expect_tx(full(s), 2 * (kAChunk + b_bytes));
+          const int k = (int)((t.k0 + kc) * kBK);
+          if (t.kind == kScore) {
+            tma_load_2d(a, &maps.hidden, k, arow, bar);
+            tma_load_2d(b, &maps.table, k, bcol, bar);
+          } else if (t.kind == kHidden) {
+            tma_load_2d(a, &maps.d_k, k, arow, bar);
+            for (uint32_t j = 0; j < p.bn / 64; ++j)
+              tma_load_2d(b + j * 4096, &maps.table_n, bcol + (int)(32 * j), (int)p.pv0 + k, bar);
+          } else {
+            tma_load_2d(a, &maps.d_m, arow, k, bar);
+            tma_load_2d(a + 8192, &maps.d_m, arow + 64, k, bar);
+            for (uint32_t j = 0; j < p.bn / 64; ++j)
+              tma_load_2d(b + j * 4096, &maps.scaled_n, bcol + (int)(32 * j), k, bar);
+          }
+          issued[s] = issued[s] + 1u;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---- MMA issuer (leader CTA only) ----
+    if (lane == 0 && leader && tiles > 0) {
+      // F32 accumulator, A and B of type T, M = 256; bit 15 / 16: A / B not K-major
+      constexpr uint32_t kIdesc = (1u << 4) | (Type<T>::kFormat << 7) | (Type<T>::kFormat << 10) |
+                                  ((uint32_t)((2 * kBM) >> 4) << 24);
+      bool ok = true;
+      uint32_t it = 0;
+      for (uint32_t i = 0; ok && i < tiles && !*abort_flag; ++i) {
+        const Tile t = walk.at(p, i);
+        const uint32_t buf = i & 1u;
+        if (!bar_wait(acc_empty(buf), ((i >> 1) & 1u) ^ 1u)) {
+          ok = false;
+          break;
+        }
+        fence_after();
+        const uint32_t acc = tmem + buf * kBN;
+        const uint32_t n = t.kind == kScore ? (uint32_t)kBN : p.bn;
+        const uint32_t idesc = kIdesc | ((n >> 3) << 17) | (t.kind == kTable ? 1u << 15 : 0u) |
+                               (t.kind != kScore ? 1u << 16 : 0u);
+        for (uint32_t kc = 0; kc < t.chunks; ++kc, ++it) {
+          const uint32_t s = it % kStages;
+          if (!bar_wait(full(s), (it / kStages) & 1u)) {
+            ok = false;
+            break;
+          }
+          fence_after();
+          const uint32_t a = sbase + Smem::a + s * kAChunk, b = sbase + Smem::b + s * kBChunk;
+#pragma unroll
+          for (int k4 = 0; k4 < kBK / 16; ++k4) {
+            const uint64_t ad = t.kind == kTable ? mn_desc(a + 2048 * k4, 128)
+                                                 : sw128_desc(a + 32 * k4);
+            const uint64_t bd = t.kind == kScore ? sw128_desc(b + 32 * k4)
+                                                 : mn_desc(b + 1024 * k4, 64);
+            mma_pair(acc, ad, bd, idesc, (kc | (uint32_t)k4) != 0u);
+          }
+          mma_commit_pair(empty(s));  // frees the stage (both CTAs) once read
+        }
+        if (!ok) break;
+        mma_commit_pair(acc_full(buf));
+      }
+      if (!ok) *abort_flag = 1u;
+      mma_commit_local(drain);
+      bar_wait(drain, 0);
+    }
+  } else {
+    // ---- epilogue: warp w serves TMEM lanes 32 (w % 4) .. + 31 (one tile row
+    // per thread) and column half (w - 2) / 4 ----
+    const uint32_t quad = (uint32_t)(warp & 3);
+    const uint32_t half = (uint32_t)(warp - 2) >> 2;
+    const uint32_t tile_row = rank * kBM + quad * 32 + (uint32_t)lane;
+    const uint32_t leader_acc_empty0 = mapa(acc_empty(0), 0);
+    const uint32_t leader_acc_empty1 = mapa(acc_empty(1), 0);
+    const float nan = __uint_as_float(0x7FC00000u);
+    const float c2 = w.inv_t * kLog2e;
+    bool dead = false;
+    // state of the row this thread holds while it walks along score tiles
+    uint32_t cur_m = 0xFFFFFFFFu, row = 0, slot = 0;
+    bool live = false;
+    float tlse2 = 0.f, run_m = -INFINITY, run_l = 0.f, dot = 0.f, z2 = 0.f, coef = 0.f;
+    Cursor<kDistill> cur;
+    cur.none();
+    auto flush = [&]() {
+      if (kForward && cur_m != 0xFFFFFFFFu && row < p.rows)
+        p.partial[(uint64_t)slot * p.rows + row] =
+            Partial{dead ? nan : run_m, dead ? nan : run_l, dot, 0.f};
+    };
+    for (uint32_t i = 0; i < tiles; ++i) {
+      const Tile t = walk.at(p, i);
+      const uint32_t buf = i & 1u;
+      if (t.kind == kScore) {
+        const uint32_t v = p.v0 + t.n * kBN + half * (kBN / 2);
+        if (t.m != cur_m) {
+          flush();
+          cur_m = t.m;
+          row = t.m * 2 * kBM + tile_row;
+          live = row < p.rows;
+          if (kForward) {
+            // slot: this pair's place among the pairs that walk row tile m
+            const uint64_t x = (uint64_t)t.m * p.n_tiles;
+            uint32_t lo = 0, hi = pair;  // first pair whose range reaches x
+            while (lo < hi) {
+              const uint32_t mid = (lo + hi) / 2;
+              if (p.score_at[mid + 1] > x) hi = mid; else lo = mid + 1;
+            }
+            slot = 2 * (pair - lo) + half;
+            run_m = -INFINITY;
+            run_l = dot = 0.f;
+          } else if (live) {
+            coef = p.rg[row].coef;
+            z2 = p.lse[row] * kLog2e;
+            live = coef != 0.f;
+          }
+          if (kDistill && live) {
+            const float2 st = w.stat[row];
+            live = !stat_empty(st) && !stat_invalid(st);
+            tlse2 = st.x * kLog2e;
+          }
+          cur.start(w, row, v, live);
+        }
+        cur.skip_to(w, v);
+      }
+      if (!dead && (*abort_flag || !bar_wait(acc_full(buf), (i >> 1) & 1u))) {
+        *abort_flag = 1u;
+        dead = true;
+      }
+      fence_after();
+      const uint32_t acc = tmem + ((quad * 32u) << 16) + buf * kBN;
+      if (t.kind == kScore) {
+        const uint32_t c_end = p.cols - min(p.cols, t.n * kBN);  // columns of the tile that exist
+#pragma unroll 1
+        for (uint32_t c = half * (kBN / 2); c < (half + 1) * (kBN / 2); c += 64) {
+          if (c >= c_end) break;
+          uint32_t r[64];
+          if (!dead) {
+            tmem_ld64(acc + c, r);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) r[j] = __float_as_uint(nan);
+          }
+          const uint32_t col = p.v0 + t.n * kBN + c;  // vocabulary id of r[0]
+          if constexpr (kForward) {
+            if (c + 64 > c_end) {
+#pragma unroll
+              for (int j = 0; j < 64; ++j)
+                if (c + j >= c_end) r[j] = 0xFF800000u;  // -inf
+            }
+            float mx = __uint_as_float(r[0]);
+#pragma unroll
+            for (int j = 1; j < 64; ++j) mx = fmaxf(mx, __uint_as_float(r[j]));
+            const float m = fmaxf(run_m, mx * c2);
+            float l[4] = {run_l * exp2_approx(run_m - m), 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 64; ++j)
+              l[j & 3] += exp2_approx(fmaf(__uint_as_float(r[j]), c2, -m));
+            run_m = m;
+            run_l = (l[0] + l[1]) + (l[2] + l[3]);
+            while (__any_sync(0xFFFFFFFFu, cur.id[0] - col < 64u)) {
+              const float s = pick64(r, cur.id[0] - col);
+              if (cur.id[0] - col < 64u) {
+                const float q = cur.weight(c2, tlse2);
+                if (q > 0.f) dot = fmaf(q, s * w.inv_t, dot);
+                cur.next(w);
+              }
+            }
+          } else {
+            T* out = static_cast<T*>(p.d) + (uint64_t)row * p.pitch + t.n * kBN + c;
+            const uint32_t keep = coef != 0.f ? 0xFFFFFFFFu : 0u;
+            if (row < p.rows) {
+#pragma unroll
+              for (int j = 0; j < 64; j += 16) {
+                uint32_t v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  const float x = exp2_approx(fmaf(__uint_as_float(r[j + 2 * e]), c2, -z2)) * coef;
+                  const float y =
+                      exp2_approx(fmaf(__uint_as_float(r[j + 2 * e + 1]), c2, -z2)) * coef;
+                  v[e] = Type<T>::pack(x, y) & keep;
+                }
+                store_v8(out + j, v);
+              }
+            }
+            while (__any_sync(0xFFFFFFFFu, cur.id[0] - col < 64u)) {
+              const float s = pick64(r, cur.id[0] - col);
+              if (cur.id[0] - col < 64u) {  // p - q in FP32, over the element just stored
+                const float x = exp2_approx(fmaf(s, c2, -z2)) - cur.weight(c2, tlse2);
+                out[cur.id[0] - col] = Type<T>::from(x * coef);
+                cur.next(w);
+              }
+            }
+          }
+        }
+      } else if constexpr (!kForward) {
+        const uint32_t c_half = p.bn / 2;
+        const uint32_t m_row = t.m * 2 * kBM + tile_row;
+        const bool mine = m_row < (t.kind == kHidden ? p.rows : p.pcols);
+        const float scale = t.kind == kTable ? *p.gmax / Type<T>::kScale : 1.f;
+#pragma unroll 1
+        for (uint32_t c = half * c_half; c < (half + 1) * c_half; c += 32) {
+          const uint32_t col = t.n * p.bn + c;
+          if (col >= p.width) break;
+          uint32_t r[32];
+          if (!dead) {
+            tmem_ld32(acc + c, r);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(nan);
+          }
+          if (!mine) continue;
+          if (t.kind == kHidden) {
+            float* out = p.planes + ((uint64_t)t.split * p.rows + m_row) * p.width + col;
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              if (col + j >= p.width) break;
+              float4 v = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]),
+                                     __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
+              float4* at = reinterpret_cast<float4*>(out + j);
+              if (p.add) {
+                const float4 o = *at;
+                v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+              }
+              *at = v;
+            }
+          } else {
+            T* out = static_cast<T*>(p.table_out) + (uint64_t)m_row * p.width + col;
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+              if (col + j >= p.width) break;
+              uint4 v;
+              v.x = Type<T>::pack(__uint_as_float(r[j]) * scale, __uint_as_float(r[j + 1]) * scale);
+              v.y = Type<T>::pack(__uint_as_float(r[j + 2]) * scale,
+                                  __uint_as_float(r[j + 3]) * scale);
+              v.z = Type<T>::pack(__uint_as_float(r[j + 4]) * scale,
+                                  __uint_as_float(r[j + 5]) * scale);
+              v.w = Type<T>::pack(__uint_as_float(r[j + 6]) * scale,
+                                  __uint_as_float(r[j + 7]) * scale);
+              *reinterpret_cast<uint4*>(out + j) = v;
+            }
+          }
+        }
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive_cluster(buf ? leader_acc_empty1 : leader_acc_empty0);
+    }
+    flush();
+  }
+
+  // ---- teardown: drain the producers' copies, free TMEM ----
   __syncthreads();
-  if (threadIdx.x >= kTile || r >= rows) return;
-  const RowGrad g = rg[r];
-  const uint32_t n = min((uint32_t)kTile, n_cols - n0);
-  const uint32_t first = v0 + n0;
-  int32_t at = 0, end = 0;
-  float tlse = 0.f;
-  if (w.offsets && g.coef != 0.f) {
-    at = first_entry(w, r, first);
-    end = w.offsets[r + 1];
-    tlse = w.stat[r].x;
-  }
-  const float z = lse[r];
-  for (uint32_t c = 0; c < n; ++c) {
-    float p = expf(st[threadIdx.x][c] - z);
-    if (w.targets) {
-      if (w.targets[r] == first + c) p -= 1.f;
-    } else if (at < end && (uint32_t)w.ids[at] == first + c) {
-      p -= expf(w.logits[at] * w.inv_t - tlse);
-      ++at;
+  if (*abort_flag && threadIdx.x == 0) {
+    if (leader) {  // wait (bounded) for the last copy issued into each stage
+      for (int s = 0; s < kStages; ++s)
+        if (issued[s] > 0u) bar_wait(full(s), (issued[s] - 1u) & 1u);
+    } else {
+      // the peer's copies complete on the leader's barriers: give any still
+      // in flight 1 ms (a copy of this GPU's memory takes microseconds)
+      const uint64_t t0 = global_ns();
+      while (global_ns() - t0 < 1000000ull) __nanosleep(10000);
     }
-    d[(uint64_t)r * pitch + n0 + c] = Type<T>::from(g.coef == 0.f ? 0.f : p * g.coef);
   }
+  fence_before();
+  cluster_sync();  // no CTA frees TMEM or exits while its pair may still touch it
+  fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(kTmemCols)
+                 : "memory");
 }
 
-// d_hidden: adds one piece's part; the last piece scales and rounds.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) hidden_kernel(const T* d, uint32_t pitch, const T* emb,
-                                                          float* sum, T* out, const RowGrad* rg,
-                                                          uint32_t rows, uint32_t width,
-                                                          uint32_t n_cols, bool first, bool last) {
-  __shared__ float sa[kStep][kTile + 1], sb[kStep][kTile + 1];
-  const uint32_t m0 = blockIdx.x * kTile, n0 = blockIdx.y * kTile;
-  float acc[4][4];
-  tile_product(acc, d, pitch, 1, emb, 1, width, m0, rows, n0, width, n_cols, sa, sb);
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t r = m0 + (threadIdx.x >> 4) + 16 * i, c = n0 + (threadIdx.x & 15) + 16 * j;
-      if (r >= rows || c >= width) continue;
-      float v = acc[i][j];
-      if (!first) v += sum[(uint64_t)r * width + c];
-      if (last)
-        out[(uint64_t)r * width + c] = Type<T>::from(rg[r].coef == 0.f ? 0.f : v * rg[r].scale);
-      else
-        sum[(uint64_t)r * width + c] = v;
-    }
+// One warp per row joins the walks' partial sums.  Row tile m's n_tiles tiles
+// lie in the ranges of a few consecutive pairs.
+__global__ void merge_kernel(Wanted w, const Partial* part, uint32_t n_tiles, uint32_t total,
+                             uint32_t pairs, uint32_t rows, uint32_t vocab, float* losses,
+                             float* lse) {
+  pdl_trigger();
+  pdl_wait();
+  const uint32_t r = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+  if (r >= rows) return;
+  const uint64_t x0 = (uint64_t)(r / (2 * kBM)) * n_tiles, x1 = x0 + n_tiles - 1;
+  // range of pair i: [total i / pairs, total (i + 1) / pairs)
+  const uint32_t first = (uint32_t)(((x0 + 1) * pairs - 1) / total);
+  const uint32_t last = (uint32_t)(((x1 + 1) * pairs - 1) / total);
+  const uint32_t slots = 2 * (last - first + 1);
+  float m = -INFINITY, l = 0.f, dot = 0.f;
+  for (uint32_t s = lane; s < slots; s += 32) {
+    const Partial q = part[(uint64_t)s * rows + r];
+    const float mn = fmaxf(m, q.m);
+    // a half tile beyond the vocabulary has l = 0 at m = -inf
+    l = l * (m == mn ? 1.f : exp2_approx(m - mn)) +
+        q.l * (q.m == mn ? 1.f : exp2_approx(q.m - mn));
+    m = mn;
+    dot += q.dot;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const float om = __shfl_xor_sync(0xFFFFFFFFu, m, o), ol = __shfl_xor_sync(0xFFFFFFFFu, l, o);
+    const float mn = fmaxf(m, om);
+    l = l * (m == mn ? 1.f : exp2_approx(m - mn)) + ol * (om == mn ? 1.f : exp2_approx(om - mn));
+    m = mn;
+    dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
+  }
+  if (lane) return;
+  const float z = (m + log2f(l)) * kLn2;
+  lse[r] = z;
+  float loss;
+  if (w.targets) {
+    const uint32_t t = w.targets[r];
+    loss = t == kInvalid ? 0.f : (t >= vocab ? __uint_as_float(0x7FC00000u) : z - dot);
+  } else {
+    const float2 s = w.stat[r];
+    const float t = 1.f / w.inv_t;
+    loss = stat_empty(s) ? 0.f : (stat_invalid(s) ? s.x : t * t * (s.y + (z - dot)));
+  }
+  losses[r] = loss;
 }
 
-// d_embedding rows of one piece.
+// d_hidden: the splits' sums in a fixed order, scaled and rounded; eight
+// columns a thread.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) table_kernel(const T* d, uint32_t pitch,
-                                                         const T* scaled, T* out,
-                                                         const float* gmax, uint32_t rows,
-                                                         uint32_t width, uint32_t n_cols) {
-  __shared__ float sa[kStep][kTile + 1], sb[kStep][kTile + 1];
-  const uint32_t m0 = blockIdx.x * kTile, n0 = blockIdx.y * kTile;
-  float acc[4][4];
-  tile_product(acc, d, 1, pitch, scaled, 1, width, m0, n_cols, n0, width, rows, sa, sb);
-  const float scale = *gmax / Type<T>::kScale;
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t v = m0 + (threadIdx.x >> 4) + 16 * i, c = n0 + (threadIdx.x & 15) + 16 * j;
-      if (v < n_cols && c < width)
-        out[(uint64_t)v * width + c] = Type<T>::from(acc[i][j] * scale);
-    }
+__global__ void __launch_bounds__(256) finish_kernel(const float* planes, uint32_t splits,
+                                                     const RowGrad* rg, T* out, uint32_t rows,
+                                                     uint32_t width) {
+  pdl_wait();
+  const uint64_t i = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) * 8;
+  const uint64_t n = (uint64_t)rows * width;
+  if (i >= n) return;
+  float v[8] = {};
+  for (uint32_t s = 0; s < splits; ++s) {
+    const float4 a = *reinterpret_cast<const float4*>(planes + s * n + i);
+    const float4 b = *reinterpret_cast<const float4*>(planes + s * n + i + 4);
+    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+    v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+  }
+  const RowGrad g = rg[i / width];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = g.coef == 0.f ? 0.f : v[j] * g.scale;
+  *reinterpret_cast<uint4*>(out + i) =
+      make_uint4(Type<T>::pack(v[0], v[1]), Type<T>::pack(v[2], v[3]), Type<T>::pack(v[4], v[5]),
+                 Type<T>::pack(v[6], v[7]));
 }
 
 // ---- host --------------------------------------------------------------
@@ -381,38 +868,56 @@ bool sizes_ok(uint64_t rows, uint64_t width, uint64_t vocab) {
          width <= MF_LOSS_MAX_HIDDEN && vocab != 0 && vocab <= MF_LOSS_MAX_VOCAB;
 }
 
-uint32_t forward_splits(uint64_t rows, uint64_t vocab) {
-  const uint64_t m = (rows + kTile - 1) / kTile, n = (vocab + kTile - 1) / kTile;
-  uint64_t s = (kWorkers + m - 1) / m;
-  return (uint32_t)(s < n ? s : n);
-}
-
 struct ForwardPlan {
-  uint64_t stat, partial, bytes;
-  uint32_t splits;
+  uint64_t m_tiles, n_tiles, stat, partial, bytes;
   ForwardPlan(uint64_t rows, uint64_t vocab) {
-    splits = forward_splits(rows, vocab);
+    m_tiles = (rows + 2 * kBM - 1) / (2 * kBM);
+    n_tiles = (vocab + kBN - 1) / kBN;
+    // pairs that share a row tile: its n_tiles tiles lie in ranges of at least
+    // floor(m n / pairs) tiles
+    uint64_t per = m_tiles * n_tiles / kMaxPairs;
+    if (per < 1) per = 1;
+    uint64_t slots = (n_tiles + per - 1) / per + 1;
+    if (slots > n_tiles) slots = n_tiles;
     stat = 0;
     partial = round_up(rows * sizeof(float2), 256);
-    bytes = round_up(partial + rows * splits * sizeof(Partial), 256);
+    bytes = round_up(partial + 2 * slots * rows * sizeof(Partial), 256);
   }
 };
 
 struct BackwardPlan {
-  uint64_t stat, rg, gmax, scaled, sum, piece, bytes;
-  uint32_t cols;  // vocabulary rows of one piece
+  uint64_t m_tiles, stat, rg, gmax, scaled, planes, piece[2], bytes;
+  uint32_t cols, pieces;  // vocabulary rows of one piece
+  uint32_t bn, bn_tiles;  // product tiles along the hidden width
+  uint32_t splits, per_split;
   BackwardPlan(uint64_t rows, uint64_t width, uint64_t vocab) {
-    uint64_t c = kPieceBytes / (2 * rows) / 256 * 256;
-    if (c < 256) c = 256;
-    const uint64_t all = round_up(vocab, 256);
-    cols = (uint32_t)(c < all ? c : all);
+    m_tiles = (rows + 2 * kBM - 1) / (2 * kBM);
+    uint64_t c = kPieceBytes / (2 * rows) / kBN * kBN;
+    if (c < kBN) c = kBN;
+    pieces = (uint32_t)((vocab + c - 1) / c);
+    cols = (uint32_t)round_up((vocab + pieces - 1) / pieces, kBN);
+    pieces = (uint32_t)((vocab + cols - 1) / cols);
+    bn_tiles = (uint32_t)((width + kBN - 1) / kBN);
+    bn = (uint32_t)round_up((width + bn_tiles - 1) / bn_tiles, 64);
+    // d E is split along the piece so that no tile is longer than half a
+    // pair's share of the two products
+    const uint64_t chunks = ((cols < vocab ? cols : vocab) + kBK - 1) / kBK;
+    const uint64_t total = bn_tiles * (m_tiles * chunks + (cols + 2 * kBM - 1) / (2 * kBM) *
+                                                              ((rows + kBK - 1) / kBK));
+    uint64_t most = total / kMaxPairs / 2;
+    if (most < 4) most = 4;
+    splits = (uint32_t)((chunks + most - 1) / most);
+    per_split = (uint32_t)((chunks + splits - 1) / splits);
+    splits = (uint32_t)((chunks + per_split - 1) / per_split);
     stat = 0;
     rg = round_up(stat + rows * sizeof(float2), 256);
     gmax = round_up(rg + rows * sizeof(RowGrad), 256);
     scaled = gmax + 256;
-    sum = round_up(scaled + rows * width * 2, 256);
-    piece = round_up(sum + (cols < vocab ? rows * width * 4 : 0), 256);
-    bytes = round_up(piece + rows * cols * 2, 256);
+    planes = round_up(scaled + rows * width * 2, 256);
+    piece[0] = round_up(planes + (uint64_t)splits * rows * width * 4, 256);
+    const uint64_t one = round_up(rows * cols * 2, 256);
+    piece[1] = piece[0] + (pieces > 1 ? one : 0);
+    bytes = piece[1] + one;
   }
 };
 
@@ -450,58 +955,200 @@ mf_status check(uint64_t rows, uint64_t width, uint64_t vocab, void* stream, Spa
   return ok();
 }
 
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static std::once_flag once;
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  });
+  return fn;
+}
+
+// 2-D tensor map over 16-bit [rows, cols] with `pitch` columns from row to row,
+// boxes of 64 columns (128-byte swizzle) or 32 (64-byte swizzle).
+template <typename T>
+bool make_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch,
+              uint32_t box_cols, uint32_t box_rows) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {cols, rows};
+  const cuuint64_t strides[1] = {pitch * 2};
+  const cuuint32_t box[2] = {box_cols, box_rows};
+  const cuuint32_t elem[2] = {1, 1};
+  return fn(map, Type<T>::kMap, 2, const_cast<void*>(base), dims, strides, box, elem,
+            CU_TENSOR_MAP_INTERLEAVE_NONE,
+            box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Sets the kernel's shared-memory limit (once per device) and returns how
+// many CTA pairs can be resident at once, at most kMaxPairs.
+template <typename T, bool kForward, bool kDistill>
+cudaError_t resident_pairs(uint32_t* pairs) {
+  static std::mutex mu;
+  static uint32_t cached[64] = {};
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  uint32_t& c = cached[dev & 63];
+  if (c == 0) {
+    auto kernel = engine_kernel<T, kForward, kDistill>;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(sms & ~1), 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = kSmemBytes;
+    int clusters = 0;
+    e = cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg);
+    if (e != cudaSuccess) return e;
+    uint32_t n = clusters < 1 ? 1u : (uint32_t)clusters;
+    if (n > (uint32_t)sms / 2) n = (uint32_t)sms / 2;
+    c = n > kMaxPairs ? kMaxPairs : n;
+  }
+  *pairs = c;
+  return cudaSuccess;
+}
+
+// A launch that may begin while the previous kernel of the call drains; every
+// kernel waits for it before it reads or writes.
+template <typename... P, typename... A>
+cudaError_t launch_after(void (*kernel)(P...), uint64_t blocks, unsigned threads, size_t smem,
+                         cudaStream_t s, bool after, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = after ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Deals n tiles of cost c to the pairs, each getting a contiguous range, so
+// that the loads (which include earlier deals) come out level.
+void deal(uint32_t n, double c, uint32_t pairs, double* load, uint32_t* at) {
+  uint32_t count[kMaxPairs] = {}, order[kMaxPairs];
+  double part[kMaxPairs] = {};
+  double sum = n * c;
+  for (uint32_t i = 0; i < pairs; ++i) sum += load[i];
+  // the common level; pairs already above it get nothing
+  bool out[kMaxPairs] = {};
+  uint32_t in = pairs;
+  for (bool again = n > 0; again;) {
+    again = false;
+    for (uint32_t i = 0; i < pairs; ++i)
+      if (!out[i] && load[i] * in > sum && in > 1) {
+        out[i] = again = true;
+        sum -= load[i];
+        --in;
+      }
+  }
+  uint32_t dealt = 0, m = 0;
+  for (uint32_t i = 0; i < pairs && n > 0; ++i) {
+    if (out[i]) continue;
+    part[i] = (sum / in - load[i]) / c;
+    if (part[i] < 0) part[i] = 0;
+    count[i] = (uint32_t)part[i];
+    if (count[i] > n - dealt) count[i] = n - dealt;
+    dealt += count[i];
+    part[i] -= count[i];
+    order[m++] = i;
+  }
+  // what rounding left over, one each
+  std::sort(order, order + m, [&](uint32_t x, uint32_t y) {
+    return part[x] != part[y] ? part[x] > part[y] : x < y;
+  });
+  for (uint32_t i = 0; dealt < n; i = i + 1 < m ? i + 1 : 0, ++dealt) ++count[order[i]];
+  at[0] = 0;
+  for (uint32_t i = 0; i < pairs; ++i) {
+    at[i + 1] = at[i] + count[i];
+    load[i] += count[i] * c;
+  }
+}
+
 mf_status launched(cudaError_t e) {
   return e == cudaSuccess ? ok() : fail(MF_CUDA_BACKEND_FAILURE, (uint32_t)e);
 }
 
-void teacher_launch(const Wanted& w, uint64_t rows, uint64_t entries, uint64_t vocab,
-                    cudaStream_t s) {
+cudaError_t teacher_launch(const Wanted& w, uint64_t rows, uint64_t entries, uint64_t vocab,
+                           cudaStream_t s) {
   const uint64_t blocks = (rows + 7) / 8;
-  teacher_kernel<<<(unsigned)(blocks < 1184 ? blocks : 1184), 256, 0, s>>>(
-      w, (uint32_t)rows, (uint32_t)entries, (uint32_t)vocab);
+  return launch_after(teacher_kernel, blocks < 1184 ? blocks : 1184, 256, 0, s, false, w,
+                      (uint32_t)rows, (uint32_t)entries, (uint32_t)vocab);
 }
 
-template <typename T>
-mf_status forward(Span hidden, Span embedding, Span targets, Span ids, Span logits, bool distill,
+template <typename T, bool kDistill>
+mf_status forward(Span hidden, Span embedding, Span targets, Span ids, Span logits,
                   float temperature, Span losses, Span lse, Span workspace, uint64_t rows,
                   uint64_t width, uint64_t vocab, void* stream) {
   const uint64_t needed = sizes_ok(rows, width, vocab) ? ForwardPlan(rows, vocab).bytes : 0;
   mf_status st = check(rows, width, vocab, stream, hidden, embedding, {losses, lse}, workspace,
-                       needed, distill, targets, ids, logits, temperature);
+                       needed, kDistill, targets, ids, logits, temperature);
   if (st.code != MF_OK) return st;
   if (outputs_overlap({losses, lse, workspace}, {hidden, embedding, targets, ids, logits}))
     return fail(MF_INVALID_ARGUMENT);
   const ForwardPlan plan(rows, vocab);
   char* ws = static_cast<char*>(const_cast<void*>(workspace.p));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint32_t pairs = 0;
+  cudaError_t e = resident_pairs<T, true, kDistill>(&pairs);
+  if (e != cudaSuccess) return fail(MF_CUDA_RUNTIME_FAILURE, (uint32_t)e);
+  Maps maps = {};
+  if (!make_map<T>(&maps.hidden, hidden.p, rows, width, width, kBK, kBM) ||
+      !make_map<T>(&maps.table, embedding.p, vocab, width, width, kBK, kBN / 2))
+    return fail(MF_CUDA_RUNTIME_FAILURE);
   Wanted w{};
-  w.inv_t = distill ? 1.f / temperature : 1.f;
-  if (distill) {
+  w.inv_t = kDistill ? 1.f / temperature : 1.f;
+  if (kDistill) {
     w.offsets = static_cast<const int32_t*>(targets.p);
     w.ids = static_cast<const int32_t*>(ids.p);
     w.logits = static_cast<const float*>(logits.p);
     w.stat = reinterpret_cast<float2*>(ws + plan.stat);
-    teacher_launch(w, rows, ids.bytes / 4, vocab, s);
+    e = teacher_launch(w, rows, ids.bytes / 4, vocab, s);
+    if (e != cudaSuccess) return launched(e);
   } else {
     w.targets = static_cast<const uint32_t*>(targets.p);
   }
-  Partial* part = reinterpret_cast<Partial*>(ws + plan.partial);
-  forward_kernel<T><<<dim3((unsigned)((rows + kTile - 1) / kTile), plan.splits), kThreads, 0, s>>>(
-      static_cast<const T*>(hidden.p), static_cast<const T*>(embedding.p), w, part,
-      (uint32_t)rows, (uint32_t)width, (uint32_t)vocab, plan.splits);
-  merge_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, s>>>(
-      w, part, plan.splits, (uint32_t)rows, (uint32_t)vocab,
-      static_cast<float*>(const_cast<void*>(losses.p)), static_cast<float*>(const_cast<void*>(lse.p)));
-  return launched(cudaGetLastError());
+  const uint64_t total = plan.m_tiles * plan.n_tiles;
+  if (pairs > total) pairs = (uint32_t)total;
+  Params p = {};
+  p.rows = (uint32_t)rows;
+  p.width = (uint32_t)width;
+  p.vocab = (uint32_t)vocab;
+  p.m_tiles = (uint32_t)plan.m_tiles;
+  p.w_chunks = (uint32_t)((width + kBK - 1) / kBK);
+  p.cols = (uint32_t)vocab;
+  p.n_tiles = (uint32_t)plan.n_tiles;
+  p.partial = reinterpret_cast<Partial*>(ws + plan.partial);
+  for (uint32_t i = 0; i <= pairs; ++i) p.score_at[i] = (uint32_t)(total * i / pairs);
+  e = launch_after(engine_kernel<T, true, kDistill>, 2 * pairs, kThreads, kSmemBytes, s, kDistill,
+                   maps, p, w);
+  if (e != cudaSuccess) return launched(e);
+  e = launch_after(merge_kernel, (rows + 7) / 8, 256, 0, s, true, w,
+                   static_cast<const Partial*>(p.partial), p.n_tiles, (uint32_t)total, pairs,
+                   p.rows, p.vocab, static_cast<float*>(const_cast<void*>(losses.p)),
+                   static_cast<float*>(const_cast<void*>(lse.p)));
+  return launched(e);
 }
 
-template <typename T>
-mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span logits, bool distill,
+template <typename T, bool kDistill>
+mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span logits,
                    float temperature, Span lse, Span grad, Span d_hidden, Span d_embedding,
                    Span workspace, uint64_t rows, uint64_t width, uint64_t vocab, void* stream) {
   const uint64_t needed = sizes_ok(rows, width, vocab) ? BackwardPlan(rows, width, vocab).bytes : 0;
   mf_status st = check(rows, width, vocab, stream, hidden, embedding, {lse, grad}, workspace,
-                       needed, distill, targets, ids, logits, temperature);
+                       needed, kDistill, targets, ids, logits, temperature);
   if (st.code != MF_OK) return st;
   if ((d_hidden.p == nullptr && d_embedding.p == nullptr) ||
       d_hidden.bytes != (d_hidden.p ? rows * width * 2 : 0) ||
@@ -513,46 +1160,97 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
   const BackwardPlan plan(rows, width, vocab);
   char* ws = static_cast<char*>(const_cast<void*>(workspace.p));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint32_t pairs = 0;
+  cudaError_t err = resident_pairs<T, false, kDistill>(&pairs);
+  if (err != cudaSuccess) return fail(MF_CUDA_RUNTIME_FAILURE, (uint32_t)err);
+  RowGrad* rg = reinterpret_cast<RowGrad*>(ws + plan.rg);
+  float* gmax = reinterpret_cast<float*>(ws + plan.gmax);
+  T* scaled = reinterpret_cast<T*>(ws + plan.scaled);
+  float* planes = reinterpret_cast<float*>(ws + plan.planes);
+  T* dh = static_cast<T*>(const_cast<void*>(d_hidden.p));
+  T* de = static_cast<T*>(const_cast<void*>(d_embedding.p));
+  Maps maps = {};
+  if (!make_map<T>(&maps.hidden, hidden.p, rows, width, width, kBK, kBM) ||
+      !make_map<T>(&maps.table, embedding.p, vocab, width, width, kBK, kBN / 2) ||
+      !make_map<T>(&maps.table_n, embedding.p, vocab, width, width, 32, kBK) ||
+      !make_map<T>(&maps.scaled_n, scaled, rows, width, width, 32, kBK))
+    return fail(MF_CUDA_RUNTIME_FAILURE);
   Wanted w{};
-  w.inv_t = distill ? 1.f / temperature : 1.f;
-  if (distill) {
+  w.inv_t = kDistill ? 1.f / temperature : 1.f;
+  if (kDistill) {
     w.offsets = static_cast<const int32_t*>(targets.p);
     w.ids = static_cast<const int32_t*>(ids.p);
     w.logits = static_cast<const float*>(logits.p);
     w.stat = reinterpret_cast<float2*>(ws + plan.stat);
-    teacher_launch(w, rows, ids.bytes / 4, vocab, s);
+    err = teacher_launch(w, rows, ids.bytes / 4, vocab, s);
+    if (err != cudaSuccess) return launched(err);
   } else {
     w.targets = static_cast<const uint32_t*>(targets.p);
   }
-  RowGrad* rg = reinterpret_cast<RowGrad*>(ws + plan.rg);
-  float* gmax = reinterpret_cast<float*>(ws + plan.gmax);
-  T* scaled = reinterpret_cast<T*>(ws + plan.scaled);
-  float* sum = reinterpret_cast<float*>(ws + plan.sum);
-  T* d = reinterpret_cast<T*>(ws + plan.piece);
-  const T* h = static_cast<const T*>(hidden.p);
-  const T* e = static_cast<const T*>(embedding.p);
-  T* dh = static_cast<T*>(const_cast<void*>(d_hidden.p));
-  T* de = static_cast<T*>(const_cast<void*>(d_embedding.p));
-  const float* z = static_cast<const float*>(lse.p);
-  setup_kernel<T><<<(unsigned)(rows < 592 ? rows : 592), kThreads, 0, s>>>(
-      w, static_cast<const float*>(grad.p), h, scaled, rg, gmax, (uint32_t)rows, (uint32_t)width,
-      (uint32_t)vocab);
-  const unsigned mt = (unsigned)((rows + kTile - 1) / kTile);
-  const unsigned ht = (unsigned)((width + kTile - 1) / kTile);
-  for (uint64_t v0 = 0; v0 < vocab; v0 += plan.cols) {
-    const uint32_t n = (uint32_t)(vocab - v0 < plan.cols ? vocab - v0 : plan.cols);
-    const unsigned nt = (n + kTile - 1) / kTile;
-    piece_kernel<T><<<dim3(mt, nt), kThreads, 0, s>>>(h, e, w, z, rg, d, plan.cols, (uint32_t)rows,
-                                                      (uint32_t)width, (uint32_t)v0, n);
-    if (dh)
-      hidden_kernel<T><<<dim3(mt, ht), kThreads, 0, s>>>(d, plan.cols, e + v0 * width, sum, dh, rg,
-                                                         (uint32_t)rows, (uint32_t)width, n,
-                                                         v0 == 0, v0 + n == vocab);
-    if (de)
-      table_kernel<T><<<dim3(nt, ht), kThreads, 0, s>>>(d, plan.cols, scaled, de + v0 * width, gmax,
-                                                        (uint32_t)rows, (uint32_t)width, n);
+  err = launch_after(setup_kernel<T>, rows < 592 ? rows : 592, kSetupThreads, 0, s, kDistill, w,
+                     static_cast<const float*>(grad.p), static_cast<const T*>(hidden.p), scaled,
+                     rg, gmax, (uint32_t)rows, (uint32_t)width, (uint32_t)vocab);
+  if (err != cudaSuccess) return launched(err);
+
+  Params p = {};
+  p.rows = (uint32_t)rows;
+  p.width = (uint32_t)width;
+  p.vocab = (uint32_t)vocab;
+  p.m_tiles = (uint32_t)plan.m_tiles;
+  p.w_chunks = (uint32_t)((width + kBK - 1) / kBK);
+  p.pitch = plan.cols;
+  p.lse = static_cast<const float*>(lse.p);
+  p.rg = rg;
+  p.bn = plan.bn;
+  p.bn_tiles = plan.bn_tiles;
+  p.per_split = plan.per_split;
+  p.planes = planes;
+  p.r_chunks = (uint32_t)((rows + kBK - 1) / kBK);
+  p.gmax = gmax;
+  auto piece_cols = [&](uint32_t i) {
+    const uint64_t left = vocab - (uint64_t)i * plan.cols;
+    return (uint32_t)(left < plan.cols ? left : plan.cols);
+  };
+  // launch i makes piece i of d and the products of piece i - 1
+  for (uint32_t i = 0; i <= plan.pieces; ++i) {
+    double load[kMaxPairs] = {};
+    uint32_t n_hidden = 0, n_table = 0, n_score = 0;
+    if (i > 0) {
+      p.pv0 = (i - 1) * plan.cols;
+      p.pcols = piece_cols(i - 1);
+      p.p_chunks = (p.pcols + kBK - 1) / kBK;
+      p.add = i > 1;
+      p.table_out = de ? de + (uint64_t)p.pv0 * width : nullptr;
+      const void* d = ws + plan.piece[(i - 1) & 1];
+      if (!make_map<T>(&maps.d_k, d, rows, p.pcols, plan.cols, kBK, kBM) ||
+          !make_map<T>(&maps.d_m, d, rows, p.pcols, plan.cols, kBK, kBK))
+        return fail(MF_CUDA_RUNTIME_FAILURE);
+      // a short last piece fills only the first splits
+      const uint32_t splits = (p.p_chunks + p.per_split - 1) / p.per_split;
+      if (dh) n_hidden = splits * p.m_tiles * p.bn_tiles;
+      if (de) n_table = (p.pcols + 2 * kBM - 1) / (2 * kBM) * p.bn_tiles;
+    }
+    if (i < plan.pieces) {
+      p.v0 = i * plan.cols;
+      p.cols = piece_cols(i);
+      p.n_tiles = (p.cols + kBN - 1) / kBN;
+      p.d = ws + plan.piece[i & 1];
+      n_score = p.m_tiles * p.n_tiles;
+    }
+    // costs in columns x chunks, an epilogue taken as at least four chunks
+    auto cost = [](uint32_t n, uint32_t chunks) { return (double)n * (chunks < 4 ? 4 : chunks) + 64; };
+    deal(n_hidden, cost(p.bn, p.per_split), pairs, load, p.hidden_at);
+    deal(n_table, cost(p.bn, p.r_chunks), pairs, load, p.table_at);
+    deal(n_score, cost(kBN, p.w_chunks), pairs, load, p.score_at);
+    err = launch_after(engine_kernel<T, false, kDistill>, 2 * pairs, kThreads, kSmemBytes, s, true,
+                       maps, p, w);
+    if (err != cudaSuccess) return launched(err);
   }
-  return launched(cudaGetLastError());
+  if (dh)
+    err = launch_after(finish_kernel<T>, (rows * width / 8 + 255) / 256, 256, 0, s, true,
+                       static_cast<const float*>(planes), plan.splits,
+                       static_cast<const RowGrad*>(rg), dh, p.rows, p.width);
+  return launched(err);
 }
 
 }  // namespace loss
@@ -578,8 +1276,8 @@ extern "C" uint64_t mf_dense_loss_backward_workspace_bytes(uint64_t rows, uint64
       const void* targets, uint64_t targets_bytes, void* losses, uint64_t losses_bytes, void* lse, \
       uint64_t lse_bytes, void* workspace, uint64_t workspace_bytes, uint64_t rows,                \
       uint64_t hidden_size, uint64_t vocab, void* stream) {                                        \
-    return loss::forward<TYPE>({hidden, hidden_bytes}, {embedding, embedding_bytes},               \
-                               {targets, targets_bytes}, {}, {}, false, 1.f,                       \
+    return loss::forward<TYPE, false>({hidden, hidden_bytes}, {embedding, embedding_bytes},        \
+                               {targets, targets_bytes}, {}, {}, 1.f,                              \
                                {losses, losses_bytes}, {lse, lse_bytes},                           \
                                {workspace, workspace_bytes}, rows, hidden_size, vocab, stream);    \
   }                                                                                                \
@@ -590,8 +1288,8 @@ extern "C" uint64_t mf_dense_loss_backward_workspace_bytes(uint64_t rows, uint64
       uint64_t d_hidden_bytes, void* d_embedding, uint64_t d_embedding_bytes, void* workspace,     \
       uint64_t workspace_bytes, uint64_t rows, uint64_t hidden_size, uint64_t vocab,               \
       void* stream) {                                                                              \
-    return loss::backward<TYPE>({hidden, hidden_bytes}, {embedding, embedding_bytes},              \
-                                {targets, targets_bytes}, {}, {}, false, 1.f, {lse, lse_bytes},    \
+    return loss::backward<TYPE, false>({hidden, hidden_bytes}, {embedding, embedding_bytes},       \
+                                {targets, targets_bytes}, {}, {}, 1.f, {lse, lse_bytes},           \
                                 {grad_losses, grad_losses_bytes}, {d_hidden, d_hidden_bytes},      \
                                 {d_embedding, d_embedding_bytes}, {workspace, workspace_bytes},    \
                                 rows, hidden_size, vocab, stream);                                 \
@@ -603,9 +1301,9 @@ extern "C" uint64_t mf_dense_loss_backward_workspace_bytes(uint64_t rows, uint64
       uint64_t losses_bytes, void* lse, uint64_t lse_bytes, void* workspace,                       \
       uint64_t workspace_bytes, uint64_t rows, uint64_t hidden_size, uint64_t vocab,               \
       void* stream) {                                                                              \
-    return loss::forward<TYPE>({hidden, hidden_bytes}, {embedding, embedding_bytes},               \
+    return loss::forward<TYPE, true>({hidden, hidden_bytes}, {embedding, embedding_bytes},         \
                                {offsets, offsets_bytes}, {ids, ids_bytes},                         \
-                               {teacher_logits, teacher_logits_bytes}, true, temperature,          \
+                               {teacher_logits, teacher_logits_bytes}, temperature,                \
                                {losses, losses_bytes}, {lse, lse_bytes},                           \
                                {workspace, workspace_bytes}, rows, hidden_size, vocab, stream);    \
   }                                                                                                \
@@ -617,9 +1315,9 @@ extern "C" uint64_t mf_dense_loss_backward_workspace_bytes(uint64_t rows, uint64
       void* d_hidden, uint64_t d_hidden_bytes, void* d_embedding, uint64_t d_embedding_bytes,      \
       void* workspace, uint64_t workspace_bytes, uint64_t rows, uint64_t hidden_size,              \
       uint64_t vocab, void* stream) {                                                              \
-    return loss::backward<TYPE>({hidden, hidden_bytes}, {embedding, embedding_bytes},              \
+    return loss::backward<TYPE, true>({hidden, hidden_bytes}, {embedding, embedding_bytes},        \
                                 {offsets, offsets_bytes}, {ids, ids_bytes},                        \
-                                {teacher_logits, teacher_logits_bytes}, true, temperature,         \
+                                {teacher_logits, teacher_logits_bytes}, temperature,               \
                                 {lse, lse_bytes}, {grad_losses, grad_losses_bytes},                \
                                 {d_hidden, d_hidden_bytes}, {d_embedding, d_embedding_bytes},      \
                                 {workspace, workspace_bytes}, rows, hidden_size, vocab, stream);   \
