@@ -45,17 +45,25 @@ namespace loss {
 constexpr int kBM = 128;       // rows of a tile per CTA (256 per pair)
 constexpr int kBN = 256;       // columns of a score tile
 constexpr int kBK = 64;        // K elements per chunk
-constexpr int kStages = 6;
-constexpr int kAChunk = kBM * kBK * 2;        // 16 KB per CTA
-constexpr int kBChunk = kBN / 2 * kBK * 2;    // at most 16 KB per CTA
+constexpr int kMaxStages = 6;
+constexpr int kChunkBytes = kBM * kBK * 2;    // 128 rows x 64 K: 16 KB
+constexpr int kScoreStage = 2 * kChunkBytes;
+constexpr int kRingBytes = 14 * kChunkBytes;  // tiles in shared memory, per CTA
 constexpr int kEpiWarps = 8;   // two per TMEM lane quadrant, each on half the columns
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr uint32_t kTmemCols = 512;
-constexpr int kSetupThreads = 256;
+constexpr int kSetupThreads = 1024;
 constexpr uint32_t kMaxPairs = 74;             // pairs of the persistent grid
 constexpr uint64_t kPieceBytes = 128ull << 20; // one piece of d
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+// The tensor core's additions drop the bits that fall below the sum's last
+// place, always towards zero, so a score comes out too small by a part that
+// grows with the width: measured 3.6e-9 to 4.5e-9 a product for scores that
+// grow steadily (64 to 1,024 products, standard deviation 0.2e-9), less where
+// the products cancel and the score is small.  Scores are scaled by 1 + width
+// 2^-28.
+constexpr float kLostPerProduct = 3.725290298461914e-9f;
 
 template <typename T>
 struct Type;
@@ -170,26 +178,32 @@ __device__ __forceinline__ float row_weight(const Wanted& w, const float* grad, 
 }
 
 // Row factors and the copy of the hidden rows that d_embedding is made of.
+// Every block finds the largest weight by itself (8 bytes a row from L2, many
+// in flight); then a warp per row.
 template <typename T>
-__global__ void __launch_bounds__(kSetupThreads) setup_kernel(Wanted w, const float* grad,
-                                                              const T* hidden, T* scaled,
-                                                              RowGrad* rg, float* gmax_out,
-                                                              uint32_t rows, uint32_t width,
-                                                              uint32_t vocab) {
+__global__ void __launch_bounds__(kSetupThreads)
+setup_kernel(Wanted w, const float* grad, const T* hidden, T* scaled, RowGrad* rg, float* gmax_out,
+             uint32_t rows, uint32_t width, uint32_t vocab) {
   __shared__ float s_max[kSetupThreads / 32];
   pdl_trigger();
   pdl_wait();
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float g = 0.f;
+#pragma unroll 8
   for (uint32_t r = threadIdx.x; r < rows; r += kSetupThreads) {
     const float a = fabsf(row_weight(w, grad, r, vocab));
-    if (a < INFINITY) g = fmaxf(g, a);  // an infinite weight spoils its own row only
+    g = fmaxf(g, a < INFINITY ? a : 0.f);  // an infinite weight spoils its own row only
   }
+#pragma unroll
   for (int o = 16; o; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
-  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = g;
+  if (lane == 0) s_max[warp] = g;
   __syncthreads();
-  for (int i = 0; i < kSetupThreads / 32; ++i) g = fmaxf(g, s_max[i]);
+  g = s_max[lane % (kSetupThreads / 32)];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
   if (blockIdx.x == 0 && threadIdx.x == 0) *gmax_out = g;
-  for (uint32_t r = blockIdx.x; r < rows; r += gridDim.x) {
+  for (uint32_t r = blockIdx.x * (kSetupThreads / 32) + warp; r < rows;
+       r += gridDim.x * (kSetupThreads / 32)) {
     const float wr = row_weight(w, grad, r, vocab);
     // |wr| / gmax = mant 2^e with mant in (1/2, 1]: d16 carries mant, the
     // hidden row 2^e, which is exact
@@ -200,15 +214,19 @@ __global__ void __launch_bounds__(kSetupThreads) setup_kernel(Wanted w, const fl
       if (fabsf(mant) == 0.5f) mant *= 2.f, e -= 1;
       two_e = ldexpf(1.f, e);
     }
-    if (threadIdx.x == 0)
-      rg[r] = RowGrad{mant * Type<T>::kScale, g * two_e / Type<T>::kScale};
-    for (uint32_t c = threadIdx.x; c < width; c += kSetupThreads)
-      scaled[(uint64_t)r * width + c] =
-          wr == 0.f ? Type<T>::from(0.f)
-                    : Type<T>::from(Type<T>::to(hidden[(uint64_t)r * width + c]) * two_e);
+    if (lane == 0) rg[r] = RowGrad{mant * Type<T>::kScale, g * two_e / Type<T>::kScale};
+    for (uint32_t c = lane * 8; c < width; c += 256) {
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (wr != 0.f) {
+        x = ld_v4(hidden + (uint64_t)r * width + c);
+        T* v = reinterpret_cast<T*>(&x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = Type<T>::from(Type<T>::to(v[j]) * two_e);
+      }
+      *reinterpret_cast<uint4*>(scaled + (uint64_t)r * width + c) = x;
+    }
   }
 }
-
 
 // ---- the tile engine ----------------------------------------------------
 
@@ -218,15 +236,24 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-// 32 TMEM lanes x 32 consecutive f32 columns -> 32 registers per thread.
+// 32 TMEM lanes x 32 consecutive f32 columns -> 32 registers per thread, valid
+// after tmem_wait_ld.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+__device__ __forceinline__ void add_v4(float* p, const uint32_t* v) {
+  asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1,%2,%3,%4};" ::"l"(p),
+               "f"(__uint_as_float(v[0])), "f"(__uint_as_float(v[1])), "f"(__uint_as_float(v[2])),
+               "f"(__uint_as_float(v[3]))
+               : "memory");
+}
 __device__ __forceinline__ void store_v8(void* p, const uint32_t* v) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]),
                "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
@@ -270,39 +297,54 @@ struct Params {
   uint32_t w_chunks;            // ceil(width / 64)
   // score tiles: vocabulary rows [v0, v0 + cols)
   uint32_t v0, cols, n_tiles;
-  Partial* partial;             // forward: [2 slots][rows]
+  float score_scale;            // 1 + what the tensor core's additions lose
+  Partial* partial;             // forward: [slots][rows]
   void* d;                      // backward: the piece being made
   uint32_t pitch;
   const float* lse;
   const RowGrad* rg;
   // product tiles: vocabulary rows [pv0, pv0 + pcols)
   uint32_t pv0, pcols, bn, bn_tiles;
+  uint32_t blocks;               // 256-row blocks that share a tile's B
+  uint32_t h_groups;             // m_tiles / blocks
+  uint32_t t_tiles;              // 256-row tiles of the piece
+  uint32_t p_stages, p_stage_bytes;
   uint32_t p_chunks, per_split;  // d E: K chunks of the piece, and of one split
   float* planes;                 // [splits][rows][width]
   uint32_t add;                  // planes hold earlier pieces' sums
   uint32_t r_chunks;             // d^T H: K chunks of the batch
   void* table_out;               // d_embedding + pv0 rows
+  uint32_t wide_rows;            // its rows start on 32 bytes
   const float* gmax;
   // per pair: tile ranges of the three kinds
   uint32_t hidden_at[kMaxPairs + 1], table_at[kMaxPairs + 1], score_at[kMaxPairs + 1];
 };
 
+// Shared memory: one region that score tiles and product tiles lay out
+// differently, each kind with barriers of its own (a pair does all its products
+// before its scores, and drains between).
+//   products  p_stages x (up to 16 KB of B, blocks x 16 KB of A)
+//   scores    6 x (16 KB of table, 16 KB of hidden rows)
+// (Keeping the hidden tile in shared memory, 9 chunks of 16 KB at width 576,
+// and streaming the table alone through 5 stages: 352 against 356 us for 8,192
+// x 49,152 forward, where the tensor cores' power is the limit, but 81 against
+// 79 us for 4,096 x 16,384 and 37 against 34 us for 256 x 49,152.)
 struct Smem {
-  static constexpr int a = 0;
-  static constexpr int b = kStages * kAChunk;
-  static constexpr int bars = b + kStages * kBChunk;
-  // barriers: full[S], empty[S], acc_full[2], acc_empty[2], drain
-  static constexpr int n_bars = 2 * kStages + 5;
+  static constexpr int bars = kRingBytes;
+  // barriers: product full, empty, score full, empty [6 each],
+  // acc_full[2], acc_empty[2], drain
+  static constexpr int n_bars = 4 * kMaxStages + 5;
   static constexpr int tmem_slot = bars + n_bars * 8;
   static constexpr int abort_flag = tmem_slot + 4;
-  static constexpr int issued = abort_flag + 4;  // u32[kStages]: loads issued per stage
-  static constexpr int size = issued + 4 * kStages;
+  // u32: product stages and score stages filled
+  static constexpr int issued = abort_flag + 4;
+  static constexpr int size = issued + 4 * 2;
 };
 constexpr size_t kSmemBytes = Smem::size + 1024;  // + alignment slack
 static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 
 struct Tile {
-  uint32_t kind, m, n, k0, chunks, split;
+  uint32_t kind, m, blocks, n, k0, chunks, split;
 };
 
 // The tiles of one pair, in order: d E, d^T H, scores.
@@ -325,24 +367,36 @@ struct Walk {
       const uint32_t x = h0 + i, y = x / p.bn_tiles;
       t.kind = kHidden;
       t.n = x % p.bn_tiles;
-      t.m = y % p.m_tiles;
-      t.split = y / p.m_tiles;
+      t.m = y % p.h_groups * p.blocks;
+      t.blocks = min(p.blocks, p.m_tiles - t.m);
+      t.split = y / p.h_groups;
       t.k0 = t.split * p.per_split;
       t.chunks = min(p.per_split, p.p_chunks - t.k0);
     } else if (i < nh + nt) {
       const uint32_t x = t0 + i - nh;
       t.kind = kTable;
       t.n = x % p.bn_tiles;
-      t.m = x / p.bn_tiles;
+      t.m = x / p.bn_tiles * p.blocks;
+      t.blocks = min(p.blocks, p.t_tiles - t.m);
       t.chunks = p.r_chunks;
     } else {
       const uint32_t x = s0 + i - nh - nt;
       t.kind = kScore;
       t.n = x % p.n_tiles;
       t.m = x / p.n_tiles;
+      t.blocks = 1;
       t.chunks = p.w_chunks;
     }
     return t;
+  }
+};
+
+// A ring of stages: which one is next, and the parity of its barriers.
+struct Ring {
+  uint32_t n, at = 0, fills = 0;  // `fills`: earlier fills of stage `at`
+  __device__ __forceinline__ explicit Ring(uint32_t stages) : n(stages) {}
+  __device__ __forceinline__ void next() {
+    if (++at == n) at = 0, ++fills;
   }
 };
 
@@ -404,8 +458,8 @@ struct Cursor {
       if (id[0] == 0xFFFFFFFFu && at < end) fill(w);
   }
   // The weight of the first entry; `tlse2` in units of ln 2.
-  __device__ __forceinline__ float weight(float c2, float tlse2) const {
-    if constexpr (kDistill) return exp2_approx(fmaf(t[0], c2, -tlse2));
+  __device__ __forceinline__ float weight(float t2, float tlse2) const {
+    if constexpr (kDistill) return exp2_approx(fmaf(t[0], t2, -tlse2));
     return 1.f;
   }
 };
@@ -430,11 +484,13 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(sm);
   const uint32_t bar0 = sbase + Smem::bars;
-  auto full = [&](uint32_t s) { return bar0 + 8 * s; };
-  auto empty = [&](uint32_t s) { return bar0 + 8 * (kStages + s); };
-  auto acc_full = [&](uint32_t b) { return bar0 + 8 * (2 * kStages + b); };
-  auto acc_empty = [&](uint32_t b) { return bar0 + 8 * (2 * kStages + 2 + b); };
-  const uint32_t drain = bar0 + 8 * (2 * kStages + 4);
+  auto p_full = [&](uint32_t st) { return bar0 + 8 * st; };
+  auto p_empty = [&](uint32_t st) { return bar0 + 8 * (kMaxStages + st); };
+  auto s_full = [&](uint32_t st) { return bar0 + 8 * (2 * kMaxStages + st); };
+  auto s_empty = [&](uint32_t st) { return bar0 + 8 * (3 * kMaxStages + st); };
+  auto acc_full = [&](uint32_t b) { return bar0 + 8 * (4 * kMaxStages + b); };
+  auto acc_empty = [&](uint32_t b) { return bar0 + 8 * (4 * kMaxStages + 2 + b); };
+  const uint32_t drain = bar0 + 8 * (4 * kMaxStages + 4);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(sm + Smem::abort_flag);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + Smem::tmem_slot);
   volatile uint32_t* issued = reinterpret_cast<volatile uint32_t*>(sm + Smem::issued);
@@ -447,11 +503,8 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
   pdl_trigger();
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      bar_init(full(s), 1);
-      bar_init(empty(s), 1);
-      issued[s] = 0u;
-    }
+    for (uint32_t st = 0; st < 4 * kMaxStages; ++st) bar_init(bar0 + 8 * st, 1);
+    issued[0] = issued[1] = 0u;
     for (int b = 0; b < 2; ++b) {
       bar_init(acc_full(b), 1);
       bar_init(acc_empty(b), 2 * kEpiWarps);  // leader's: one arrival per epilogue warp of the pair
@@ -479,39 +532,71 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
     // ---- producer: both CTAs load their halves; the copies complete on the
     // leader's barriers, whose expected byte counts cover both ----
     if (lane == 0) {
-      uint32_t it = 0;
-      for (uint32_t i = 0; i < tiles && !*abort_flag; ++i) {
+      Ring pr(p.p_stages), sr(kMaxStages);
+      const uint32_t leader_p_full = mapa(p_full(0), 0), leader_s_full = mapa(s_full(0), 0);
+      bool ok = true;
+      for (uint32_t i = 0; ok && i < tiles && !*abort_flag; ++i) {
         const Tile t = walk.at(p, i);
-        const uint32_t b_bytes = t.kind == kScore ? (uint32_t)kBChunk : p.bn * kBK;
         const int arow = (int)(t.m * 2 * kBM + rank * kBM);
-        const int bcol = t.kind == kScore ? (int)(p.v0 + t.n * kBN + rank * (kBN / 2))
-                                          : (int)(t.n * p.bn + rank * (p.bn / 2));
-        for (uint32_t kc = 0; kc < t.chunks; ++kc, ++it) {
-          const uint32_t s = it % kStages;
-          if (!bar_wait(empty(s), ((it / kStages) & 1u) ^ 1u)) {
-            *abort_flag = 1u;
-            break;
+        if (t.kind == kScore) {
+          if (i == walk.nh + walk.nt) {  // every product stage read by its MMAs
+            for (uint32_t st = 0; ok && st < pr.n; ++st) {
+              const uint32_t fills = pr.fills + (st < pr.at ? 1u : 0u);
+              ok = bar_wait(p_empty(st), (fills & 1u) ^ 1u);
+            }
+            if (!ok) break;
           }
-          const uint32_t bar = mapa(full(s), 0);
-          const uint32_t a = sbase + Smem::a + s * kAChunk, b = sbase + Smem::b + s * kBChunk;
-          if (leader) bar_expect_tx(full(s), 2 * (kAChunk + b_bytes));
-          const int k = (int)((t.k0 + kc) * kBK);
-          if (t.kind == kScore) {
-            tma_load_2d(a, &maps.hidden, k, arow, bar);
-            tma_load_2d(b, &maps.table, k, bcol, bar);
-          } else if (t.kind == kHidden) {
-            tma_load_2d(a, &maps.d_k, k, arow, bar);
-            for (uint32_t j = 0; j < p.bn / 64; ++j)
-              tma_load_2d(b + j * 4096, &maps.table_n, bcol + (int)(32 * j), (int)p.pv0 + k, bar);
-          } else {
-            tma_load_2d(a, &maps.d_m, arow, k, bar);
-            tma_load_2d(a + 8192, &maps.d_m, arow + 64, k, bar);
-            for (uint32_t j = 0; j < p.bn / 64; ++j)
-              tma_load_2d(b + j * 4096, &maps.scaled_n, bcol + (int)(32 * j), k, bar);
+          const int brow = (int)(p.v0 + t.n * kBN + rank * (kBN / 2));
+          const int k_end = (int)(t.chunks * kBK);
+          for (int k = 0; k < k_end; k += kBK) {
+            if (!bar_wait(s_empty(sr.at), (sr.fills & 1u) ^ 1u)) {
+              ok = false;
+              break;
+            }
+            const uint32_t bar = leader_s_full + 8 * sr.at;
+            const uint32_t at = sbase + sr.at * kScoreStage;
+            if (leader) bar_expect_tx(s_full(sr.at), 2 * kScoreStage);
+            tma_load_2d(at, &maps.table, k, brow, bar);
+            tma_load_2d(at + kChunkBytes, &maps.hidden, k, arow, bar);
+            sr.next();
           }
-          issued[s] = issued[s] + 1u;
+        } else if constexpr (!kForward) {
+          const int bcol = (int)(t.n * p.bn + rank * (p.bn / 2));
+          const uint32_t bytes = 2 * (t.blocks * kChunkBytes + p.bn * kBK);
+          const uint32_t b_boxes = p.bn / 64;
+          int k = (int)(t.k0 * kBK);
+          const int k_end = k + (int)(t.chunks * kBK);
+          for (; k < k_end; k += kBK) {
+            if (!bar_wait(p_empty(pr.at), (pr.fills & 1u) ^ 1u)) {
+              ok = false;
+              break;
+            }
+            const uint32_t bar = leader_p_full + 8 * pr.at;
+            uint32_t at = sbase + pr.at * p.p_stage_bytes;
+            if (leader) bar_expect_tx(p_full(pr.at), bytes);
+            if (t.kind == kHidden) {
+              for (uint32_t j = 0; j < b_boxes; ++j, at += 4096)
+                tma_load_2d(at, &maps.table_n, bcol + (int)(32 * j), (int)p.pv0 + k, bar);
+              tma_load_2d(at, &maps.d_k, k, arow, bar);
+              if (t.blocks > 1) tma_load_2d(at + kChunkBytes, &maps.d_k, k, arow + 2 * kBM, bar);
+            } else {
+              for (uint32_t j = 0; j < b_boxes; ++j, at += 4096)
+                tma_load_2d(at, &maps.scaled_n, bcol + (int)(32 * j), k, bar);
+              tma_load_2d(at, &maps.d_m, arow, k, bar);
+              tma_load_2d(at + 8192, &maps.d_m, arow + 64, k, bar);
+              if (t.blocks > 1) {
+                tma_load_2d(at + kChunkBytes, &maps.d_m, arow + 2 * kBM, k, bar);
+                tma_load_2d(at + kChunkBytes + 8192, &maps.d_m, arow + 2 * kBM + 64, k, bar);
+              }
+            }
+            pr.next();
+          }
         }
       }
+      if (!ok) *abort_flag = 1u;
+      // what is in flight, for the teardown after an abort
+      issued[0] = pr.fills * pr.n + pr.at;
+      issued[1] = sr.fills * sr.n + sr.at;
     }
   } else if (warp == 1) {
     // ---- MMA issuer (leader CTA only) ----
@@ -520,39 +605,62 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
       constexpr uint32_t kIdesc = (1u << 4) | (Type<T>::kFormat << 7) | (Type<T>::kFormat << 10) |
                                   ((uint32_t)((2 * kBM) >> 4) << 24);
       bool ok = true;
-      uint32_t it = 0;
+      Ring pr(p.p_stages), sr(kMaxStages);
+      uint32_t sub = 0;  // accumulators used so far: buffer sub & 1
+      const uint64_t k_major = sw128_desc(sbase);  // + offset / 16: any place of the region
+      const uint64_t m_major = mn_desc(sbase, 128), n_major = mn_desc(sbase, 64);
       for (uint32_t i = 0; ok && i < tiles && !*abort_flag; ++i) {
         const Tile t = walk.at(p, i);
-        const uint32_t buf = i & 1u;
-        if (!bar_wait(acc_empty(buf), ((i >> 1) & 1u) ^ 1u)) {
-          ok = false;
-          break;
-        }
+        for (uint32_t j = 0; ok && j < t.blocks; ++j)
+          ok = bar_wait(acc_empty((sub + j) & 1u), (((sub + j) >> 1) & 1u) ^ 1u);
+        if (!ok) break;
         fence_after();
-        const uint32_t acc = tmem + buf * kBN;
-        const uint32_t n = t.kind == kScore ? (uint32_t)kBN : p.bn;
-        const uint32_t idesc = kIdesc | ((n >> 3) << 17) | (t.kind == kTable ? 1u << 15 : 0u) |
-                               (t.kind != kScore ? 1u << 16 : 0u);
-        for (uint32_t kc = 0; kc < t.chunks; ++kc, ++it) {
-          const uint32_t s = it % kStages;
-          if (!bar_wait(full(s), (it / kStages) & 1u)) {
-            ok = false;
-            break;
-          }
-          fence_after();
-          const uint32_t a = sbase + Smem::a + s * kAChunk, b = sbase + Smem::b + s * kBChunk;
+        const uint32_t acc = tmem + (sub & 1u) * kBN;
+        if (t.kind == kScore) {
+          constexpr uint32_t idesc = kIdesc | ((uint32_t)(kBN >> 3) << 17);
+          for (uint32_t kc = 0; kc < t.chunks; ++kc) {
+            if (!bar_wait(s_full(sr.at), sr.fills & 1u)) {
+              ok = false;
+              break;
+            }
+            fence_after();
+            const uint64_t b = k_major + sr.at * (kScoreStage / 16), a = b + kChunkBytes / 16;
 #pragma unroll
-          for (int k4 = 0; k4 < kBK / 16; ++k4) {
-            const uint64_t ad = t.kind == kTable ? mn_desc(a + 2048 * k4, 128)
-                                                 : sw128_desc(a + 32 * k4);
-            const uint64_t bd = t.kind == kScore ? sw128_desc(b + 32 * k4)
-                                                 : mn_desc(b + 1024 * k4, 64);
-            mma_pair(acc, ad, bd, idesc, (kc | (uint32_t)k4) != 0u);
+            for (int k4 = 0; k4 < kBK / 16; ++k4)
+              mma_pair(acc, a + 2 * k4, b + 2 * k4, idesc, (kc | (uint32_t)k4) != 0u);
+            mma_commit_pair(s_empty(sr.at));  // frees the stage (both CTAs) once read
+            sr.next();
           }
-          mma_commit_pair(empty(s));  // frees the stage (both CTAs) once read
+        } else if constexpr (!kForward) {
+          const uint32_t idesc = kIdesc | ((p.bn >> 3) << 17) |
+                                 (t.kind == kTable ? 1u << 15 : 0u) | (1u << 16);
+          const uint64_t a0 = (t.kind == kTable ? m_major : k_major) + p.bn * kBK / 16;
+          const uint32_t a_step = t.kind == kTable ? 2048 / 16 : 2;
+          const uint32_t stage = p.p_stage_bytes / 16;
+          const uint32_t acc1 = tmem + ((sub + 1) & 1u) * kBN;
+          for (uint32_t kc = 0; kc < t.chunks; ++kc) {
+            if (!bar_wait(p_full(pr.at), pr.fills & 1u)) {
+              ok = false;
+              break;
+            }
+            fence_after();
+            const uint64_t b = n_major + pr.at * stage, a = a0 + pr.at * stage;
+#pragma unroll
+            for (int k4 = 0; k4 < kBK / 16; ++k4)
+              mma_pair(acc, a + a_step * k4, b + 64 * k4, idesc, (kc | (uint32_t)k4) != 0u);
+            if (t.blocks > 1) {
+#pragma unroll
+              for (int k4 = 0; k4 < kBK / 16; ++k4)
+                mma_pair(acc1, a + kChunkBytes / 16 + a_step * k4, b + 64 * k4, idesc,
+                         (kc | (uint32_t)k4) != 0u);
+            }
+            mma_commit_pair(p_empty(pr.at));
+            pr.next();
+          }
         }
         if (!ok) break;
-        mma_commit_pair(acc_full(buf));
+        for (uint32_t j = 0; j < t.blocks; ++j) mma_commit_pair(acc_full((sub + j) & 1u));
+        sub += t.blocks;
       }
       if (!ok) *abort_flag = 1u;
       mma_commit_local(drain);
@@ -567,7 +675,9 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
     const uint32_t leader_acc_empty0 = mapa(acc_empty(0), 0);
     const uint32_t leader_acc_empty1 = mapa(acc_empty(1), 0);
     const float nan = __uint_as_float(0x7FC00000u);
-    const float c2 = w.inv_t * kLog2e;
+    const float t2 = w.inv_t * kLog2e;  // of the teacher's logits
+    const float inv_t = w.inv_t * p.score_scale;
+    const float c2 = inv_t * kLog2e;
     bool dead = false;
     // state of the row this thread holds while it walks along score tiles
     uint32_t cur_m = 0xFFFFFFFFu, row = 0, slot = 0;
@@ -575,14 +685,22 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
     float tlse2 = 0.f, run_m = -INFINITY, run_l = 0.f, dot = 0.f, z2 = 0.f, coef = 0.f;
     Cursor<kDistill> cur;
     cur.none();
+    auto release = [&](uint32_t buf) {  // the accumulator has been read
+      fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive_cluster(buf ? leader_acc_empty1 : leader_acc_empty0);
+    };
     auto flush = [&]() {
       if (kForward && cur_m != 0xFFFFFFFFu && row < p.rows)
         p.partial[(uint64_t)slot * p.rows + row] =
             Partial{dead ? nan : run_m, dead ? nan : run_l, dot, 0.f};
     };
-    for (uint32_t i = 0; i < tiles; ++i) {
-      const Tile t = walk.at(p, i);
-      const uint32_t buf = i & 1u;
+    uint32_t sub = 0;
+    for (uint32_t i = 0, block = 0; i < tiles; ++sub) {
+      Tile t = walk.at(p, i);
+      t.m += block;
+      if (++block == t.blocks) block = 0, ++i;
+      const uint32_t buf = sub & 1u;
       if (t.kind == kScore) {
         const uint32_t v = p.v0 + t.n * kBN + half * (kBN / 2);
         if (t.m != cur_m) {
@@ -615,7 +733,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
         }
         cur.skip_to(w, v);
       }
-      if (!dead && (*abort_flag || !bar_wait(acc_full(buf), (i >> 1) & 1u))) {
+      if (!dead && (*abort_flag || !bar_wait(acc_full(buf), (sub >> 1) & 1u))) {
         *abort_flag = 1u;
         dead = true;
       }
@@ -653,8 +771,8 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
             while (__any_sync(0xFFFFFFFFu, cur.id[0] - col < 64u)) {
               const float s = pick64(r, cur.id[0] - col);
               if (cur.id[0] - col < 64u) {
-                const float q = cur.weight(c2, tlse2);
-                if (q > 0.f) dot = fmaf(q, s * w.inv_t, dot);
+                const float q = cur.weight(t2, tlse2);
+                if (q > 0.f) dot = fmaf(q, s * inv_t, dot);
                 cur.next(w);
               }
             }
@@ -678,7 +796,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
             while (__any_sync(0xFFFFFFFFu, cur.id[0] - col < 64u)) {
               const float s = pick64(r, cur.id[0] - col);
               if (cur.id[0] - col < 64u) {  // p - q in FP32, over the element just stored
-                const float x = exp2_approx(fmaf(s, c2, -z2)) - cur.weight(c2, tlse2);
+                const float x = exp2_approx(fmaf(s, c2, -z2)) - cur.weight(t2, tlse2);
                 out[cur.id[0] - col] = Type<T>::from(x * coef);
                 cur.next(w);
               }
@@ -689,54 +807,61 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
         const uint32_t c_half = p.bn / 2;
         const uint32_t m_row = t.m * 2 * kBM + tile_row;
         const bool mine = m_row < (t.kind == kHidden ? p.rows : p.pcols);
+        const uint64_t at = ((uint64_t)(t.kind == kHidden ? t.split : 0u) * p.rows + m_row) * p.width;
         const float scale = t.kind == kTable ? *p.gmax / Type<T>::kScale : 1.f;
 #pragma unroll 1
-        for (uint32_t c = half * c_half; c < (half + 1) * c_half; c += 32) {
-          const uint32_t col = t.n * p.bn + c;
-          if (col >= p.width) break;
-          uint32_t r[32];
+        for (uint32_t c = 0; c < c_half; c += 64) {
+          uint32_t r[2][32];
+          const bool two = c + 32 < c_half;
           if (!dead) {
-            tmem_ld32(acc + c, r);
+            tmem_ld32(acc + half * c_half + c, r[0]);
+            if (two) tmem_ld32(acc + half * c_half + c + 32, r[1]);
+            tmem_wait_ld();
           } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(nan);
+            for (int j = 0; j < 32; ++j) r[0][j] = r[1][j] = __float_as_uint(nan);
           }
-          if (!mine) continue;
-          if (t.kind == kHidden) {
-            float* out = p.planes + ((uint64_t)t.split * p.rows + m_row) * p.width + col;
+          if (c + 64 >= c_half) release(buf);  // before the last stores
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              if (col + j >= p.width) break;
-              float4 v = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]),
-                                     __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
-              float4* at = reinterpret_cast<float4*>(out + j);
-              if (p.add) {
-                const float4 o = *at;
-                v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+          for (uint32_t q = 0; q < 2; ++q) {
+            const uint32_t col = t.n * p.bn + half * c_half + c + 32 * q;
+            if ((q && !two) || !mine || col >= p.width) continue;
+            const uint32_t n = min(4u, (p.width - col) / 8);  // groups of 8 that exist
+            if (t.kind == kHidden) {
+              float* out = p.planes + at + col;
+              if (p.add) {  // one addition to each element a launch: the order is fixed
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j)
+                  if (j < 2 * n) add_v4(out + 4 * j, r[q] + 4 * j);
+              } else {
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j)
+                  if (j < n) store_v8(out + 8 * j, r[q] + 8 * j);
               }
-              *at = v;
-            }
-          } else {
-            T* out = static_cast<T*>(p.table_out) + (uint64_t)m_row * p.width + col;
+            } else {
+              T* out = static_cast<T*>(p.table_out) + at + col;
+              uint32_t v[16];
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-              if (col + j >= p.width) break;
-              uint4 v;
-              v.x = Type<T>::pack(__uint_as_float(r[j]) * scale, __uint_as_float(r[j + 1]) * scale);
-              v.y = Type<T>::pack(__uint_as_float(r[j + 2]) * scale,
-                                  __uint_as_float(r[j + 3]) * scale);
-              v.z = Type<T>::pack(__uint_as_float(r[j + 4]) * scale,
-                                  __uint_as_float(r[j + 5]) * scale);
-              v.w = Type<T>::pack(__uint_as_float(r[j + 6]) * scale,
-                                  __uint_as_float(r[j + 7]) * scale);
-              *reinterpret_cast<uint4*>(out + j) = v;
+              for (int j = 0; j < 16; ++j)
+                v[j] = Type<T>::pack(__uint_as_float(r[q][2 * j]) * scale,
+                                     __uint_as_float(r[q][2 * j + 1]) * scale);
+              if (p.wide_rows) {  // rows start on 32 bytes, and hold a multiple of that
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j += 2)
+                  if (j < n) store_v8(out + 8 * j, v + 4 * j);
+              } else {
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j)
+                  if (j < n)
+                    *reinterpret_cast<uint4*>(out + 8 * j) =
+                        make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+              }
             }
           }
         }
+        continue;
       }
-      fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive_cluster(buf ? leader_acc_empty1 : leader_acc_empty0);
+      release(buf);
     }
     flush();
   }
@@ -745,8 +870,11 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
   __syncthreads();
   if (*abort_flag && threadIdx.x == 0) {
     if (leader) {  // wait (bounded) for the last copy issued into each stage
-      for (int s = 0; s < kStages; ++s)
-        if (issued[s] > 0u) bar_wait(full(s), (issued[s] - 1u) & 1u);
+      for (uint32_t st = 0; st < kMaxStages; ++st) {
+        if (issued[0] > st && st < p.p_stages)
+          bar_wait(p_full(st), ((issued[0] - st - 1u) / p.p_stages) & 1u);
+        if (issued[1] > st) bar_wait(s_full(st), ((issued[1] - st - 1u) / kMaxStages) & 1u);
+      }
     } else {
       // the peer's copies complete on the leader's barriers: give any still
       // in flight 1 ms (a copy of this GPU's memory takes microseconds)
@@ -764,10 +892,14 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
 }
 
 // One warp per row joins the walks' partial sums.  Row tile m's n_tiles tiles
-// lie in the ranges of a few consecutive pairs.
-__global__ void merge_kernel(Wanted w, const Partial* part, uint32_t n_tiles, uint32_t total,
-                             uint32_t pairs, uint32_t rows, uint32_t vocab, float* losses,
-                             float* lse) {
+// lie in the ranges of a few consecutive pairs.  A target's score is computed
+// again on the FP32 pipes, with rounding to nearest, and takes the place of the
+// tensor core's in the sum: a loss is a difference of two numbers that a sure
+// row has nearly equal.
+template <typename T>
+__global__ void merge_kernel(Wanted w, const T* hidden, const T* table, uint32_t width,
+                             const Partial* part, uint32_t n_tiles, uint32_t total, uint32_t pairs,
+                             uint32_t rows, uint32_t vocab, float* losses, float* lse) {
   pdl_trigger();
   pdl_wait();
   const uint32_t r = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
@@ -795,13 +927,31 @@ __global__ void merge_kernel(Wanted w, const Partial* part, uint32_t n_tiles, ui
     m = mn;
     dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
   }
+  const uint32_t target = w.targets ? w.targets[r] : kInvalid;
+  if (target < vocab) {
+    const T *a = hidden + (uint64_t)r * width, *b = table + (uint64_t)target * width;
+    float s0 = 0.f, s1 = 0.f;
+    for (uint32_t c = lane * 8; c < width; c += 256) {
+      const uint4 x = ld_v4(a + c), y = ld_v4(b + c);
+      const T *xs = reinterpret_cast<const T*>(&x), *ys = reinterpret_cast<const T*>(&y);
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        s0 = fmaf(Type<T>::to(xs[j]), Type<T>::to(ys[j]), s0);
+        s1 = fmaf(Type<T>::to(xs[j + 1]), Type<T>::to(ys[j + 1]), s1);
+      }
+    }
+    float s = s0 + s1;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+    l += exp2_approx(fmaf(s, kLog2e, -m)) - exp2_approx(fmaf(dot, kLog2e, -m));
+    dot = s;
+  }
   if (lane) return;
   const float z = (m + log2f(l)) * kLn2;
   lse[r] = z;
   float loss;
   if (w.targets) {
-    const uint32_t t = w.targets[r];
-    loss = t == kInvalid ? 0.f : (t >= vocab ? __uint_as_float(0x7FC00000u) : z - dot);
+    loss = target == kInvalid ? 0.f : (target >= vocab ? __uint_as_float(0x7FC00000u) : z - dot);
   } else {
     const float2 s = w.stat[r];
     const float t = 1.f / w.inv_t;
@@ -810,29 +960,27 @@ __global__ void merge_kernel(Wanted w, const Partial* part, uint32_t n_tiles, ui
   losses[r] = loss;
 }
 
-// d_hidden: the splits' sums in a fixed order, scaled and rounded; eight
-// columns a thread.
+// d_hidden: the splits' sums in a fixed order, scaled and rounded; four columns
+// a thread.
 template <typename T>
-__global__ void __launch_bounds__(256) finish_kernel(const float* planes, uint32_t splits,
+__global__ void __launch_bounds__(128) finish_kernel(const float* planes, uint32_t splits,
                                                      const RowGrad* rg, T* out, uint32_t rows,
                                                      uint32_t width) {
   pdl_wait();
-  const uint64_t i = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) * 8;
+  const uint64_t i = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) * 4;
   const uint64_t n = (uint64_t)rows * width;
   if (i >= n) return;
-  float v[8] = {};
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
   for (uint32_t s = 0; s < splits; ++s) {
     const float4 a = *reinterpret_cast<const float4*>(planes + s * n + i);
-    const float4 b = *reinterpret_cast<const float4*>(planes + s * n + i + 4);
-    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-    v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+    v = make_float4(v.x + a.x, v.y + a.y, v.z + a.z, v.w + a.w);
   }
   const RowGrad g = rg[i / width];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = g.coef == 0.f ? 0.f : v[j] * g.scale;
-  *reinterpret_cast<uint4*>(out + i) =
-      make_uint4(Type<T>::pack(v[0], v[1]), Type<T>::pack(v[2], v[3]), Type<T>::pack(v[4], v[5]),
-                 Type<T>::pack(v[6], v[7]));
+  const bool in = g.coef != 0.f;
+  *reinterpret_cast<uint2*>(out + i) =
+      make_uint2(Type<T>::pack(in ? v.x * g.scale : 0.f, in ? v.y * g.scale : 0.f),
+                 Type<T>::pack(in ? v.z * g.scale : 0.f, in ? v.w * g.scale : 0.f));
 }
 
 // ---- host --------------------------------------------------------------
@@ -889,6 +1037,7 @@ struct BackwardPlan {
   uint64_t m_tiles, stat, rg, gmax, scaled, planes, piece[2], bytes;
   uint32_t cols, pieces;  // vocabulary rows of one piece
   uint32_t bn, bn_tiles;  // product tiles along the hidden width
+  uint32_t blocks;        // row blocks that share a product tile's B
   uint32_t splits, per_split;
   BackwardPlan(uint64_t rows, uint64_t width, uint64_t vocab) {
     m_tiles = (rows + 2 * kBM - 1) / (2 * kBM);
@@ -906,6 +1055,9 @@ struct BackwardPlan {
                                                               ((rows + kBK - 1) / kBK));
     uint64_t most = total / kMaxPairs / 2;
     if (most < 4) most = 4;
+    // two 256-row blocks a tile cost no accumulator to drain into: for long K
+    blocks = rows >= 32 * kBK && most >= 64 ? 2 : 1;
+    if (blocks == 2) most /= 2;
     splits = (uint32_t)((chunks + most - 1) / most);
     per_split = (uint32_t)((chunks + splits - 1) / splits);
     splits = (uint32_t)((chunks + per_split - 1) / per_split);
@@ -1035,6 +1187,19 @@ cudaError_t launch_after(void (*kernel)(P...), uint64_t blocks, unsigned threads
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// What both directions' engine launches share.
+Params base_params(uint64_t rows, uint64_t width, uint64_t vocab) {
+  Params p = {};
+  p.rows = (uint32_t)rows;
+  p.width = (uint32_t)width;
+  p.vocab = (uint32_t)vocab;
+  p.m_tiles = (uint32_t)((rows + 2 * kBM - 1) / (2 * kBM));
+  p.w_chunks = (uint32_t)((width + kBK - 1) / kBK);
+  p.p_stages = 1;
+  p.score_scale = 1.f + (float)width * kLostPerProduct;
+  return p;
+}
+
 // Deals n tiles of cost c to the pairs, each getting a contiguous range, so
 // that the loads (which include earlier deals) come out level.
 void deal(uint32_t n, double c, uint32_t pairs, double* load, uint32_t* at) {
@@ -1122,12 +1287,7 @@ mf_status forward(Span hidden, Span embedding, Span targets, Span ids, Span logi
   }
   const uint64_t total = plan.m_tiles * plan.n_tiles;
   if (pairs > total) pairs = (uint32_t)total;
-  Params p = {};
-  p.rows = (uint32_t)rows;
-  p.width = (uint32_t)width;
-  p.vocab = (uint32_t)vocab;
-  p.m_tiles = (uint32_t)plan.m_tiles;
-  p.w_chunks = (uint32_t)((width + kBK - 1) / kBK);
+  Params p = base_params(rows, width, vocab);
   p.cols = (uint32_t)vocab;
   p.n_tiles = (uint32_t)plan.n_tiles;
   p.partial = reinterpret_cast<Partial*>(ws + plan.partial);
@@ -1135,7 +1295,8 @@ mf_status forward(Span hidden, Span embedding, Span targets, Span ids, Span logi
   e = launch_after(engine_kernel<T, true, kDistill>, 2 * pairs, kThreads, kSmemBytes, s, kDistill,
                    maps, p, w);
   if (e != cudaSuccess) return launched(e);
-  e = launch_after(merge_kernel, (rows + 7) / 8, 256, 0, s, true, w,
+  e = launch_after(merge_kernel<T>, (rows + 7) / 8, 256, 0, s, true, w,
+                   static_cast<const T*>(hidden.p), static_cast<const T*>(embedding.p), p.width,
                    static_cast<const Partial*>(p.partial), p.n_tiles, (uint32_t)total, pairs,
                    p.rows, p.vocab, static_cast<float*>(const_cast<void*>(losses.p)),
                    static_cast<float*>(const_cast<void*>(lse.p)));
@@ -1187,26 +1348,26 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
   } else {
     w.targets = static_cast<const uint32_t*>(targets.p);
   }
-  err = launch_after(setup_kernel<T>, rows < 592 ? rows : 592, kSetupThreads, 0, s, kDistill, w,
+  err = launch_after(setup_kernel<T>, rows < 32 * 148 ? (rows + 31) / 32 : 148, kSetupThreads, 0, s, kDistill, w,
                      static_cast<const float*>(grad.p), static_cast<const T*>(hidden.p), scaled,
                      rg, gmax, (uint32_t)rows, (uint32_t)width, (uint32_t)vocab);
   if (err != cudaSuccess) return launched(err);
 
-  Params p = {};
-  p.rows = (uint32_t)rows;
-  p.width = (uint32_t)width;
-  p.vocab = (uint32_t)vocab;
-  p.m_tiles = (uint32_t)plan.m_tiles;
-  p.w_chunks = (uint32_t)((width + kBK - 1) / kBK);
+  Params p = base_params(rows, width, vocab);
   p.pitch = plan.cols;
   p.lse = static_cast<const float*>(lse.p);
   p.rg = rg;
   p.bn = plan.bn;
   p.bn_tiles = plan.bn_tiles;
+  p.blocks = plan.blocks;
+  p.h_groups = (p.m_tiles + p.blocks - 1) / p.blocks;
+  p.p_stage_bytes = p.blocks * kChunkBytes + p.bn * kBK;
+  p.p_stages = kRingBytes / p.p_stage_bytes < kMaxStages ? kRingBytes / p.p_stage_bytes : kMaxStages;
   p.per_split = plan.per_split;
   p.planes = planes;
   p.r_chunks = (uint32_t)((rows + kBK - 1) / kBK);
   p.gmax = gmax;
+  p.wide_rows = width % 16 == 0 && (uintptr_t)de % 32 == 0;
   auto piece_cols = [&](uint32_t i) {
     const uint64_t left = vocab - (uint64_t)i * plan.cols;
     return (uint32_t)(left < plan.cols ? left : plan.cols);
@@ -1227,8 +1388,9 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
         return fail(MF_CUDA_RUNTIME_FAILURE);
       // a short last piece fills only the first splits
       const uint32_t splits = (p.p_chunks + p.per_split - 1) / p.per_split;
-      if (dh) n_hidden = splits * p.m_tiles * p.bn_tiles;
-      if (de) n_table = (p.pcols + 2 * kBM - 1) / (2 * kBM) * p.bn_tiles;
+      p.t_tiles = (p.pcols + 2 * kBM - 1) / (2 * kBM);
+      if (dh) n_hidden = splits * p.h_groups * p.bn_tiles;
+      if (de) n_table = (p.t_tiles + p.blocks - 1) / p.blocks * p.bn_tiles;
     }
     if (i < plan.pieces) {
       p.v0 = i * plan.cols;
@@ -1239,15 +1401,15 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
     }
     // costs in columns x chunks, an epilogue taken as at least four chunks
     auto cost = [](uint32_t n, uint32_t chunks) { return (double)n * (chunks < 4 ? 4 : chunks) + 64; };
-    deal(n_hidden, cost(p.bn, p.per_split), pairs, load, p.hidden_at);
-    deal(n_table, cost(p.bn, p.r_chunks), pairs, load, p.table_at);
+    deal(n_hidden, cost(p.blocks * p.bn, p.per_split), pairs, load, p.hidden_at);
+    deal(n_table, cost(p.blocks * p.bn, p.r_chunks), pairs, load, p.table_at);
     deal(n_score, cost(kBN, p.w_chunks), pairs, load, p.score_at);
     err = launch_after(engine_kernel<T, false, kDistill>, 2 * pairs, kThreads, kSmemBytes, s, true,
                        maps, p, w);
     if (err != cudaSuccess) return launched(err);
   }
   if (dh)
-    err = launch_after(finish_kernel<T>, (rows * width / 8 + 255) / 256, 256, 0, s, true,
+    err = launch_after(finish_kernel<T>, (rows * width / 4 + 127) / 128, 128, 0, s, true,
                        static_cast<const float*>(planes), plan.splits,
                        static_cast<const RowGrad*>(rg), dh, p.rows, p.width);
   return launched(err);

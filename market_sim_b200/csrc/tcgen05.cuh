@@ -50,19 +50,26 @@ __device__ __forceinline__ uint64_t global_ns() {
   return t;
 }
 
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0u;
+}
+
 // Wait for the phase of parity `parity` of `bar`, for at most kWaitLimitNs.
+// The clock is read only once a wait turns out to be a long one.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+  for (uint32_t i = 0; i < 64; ++i)
+    if (bar_try(bar, parity)) return true;
   const uint64_t start = global_ns();
   for (uint32_t i = 0;; ++i) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred q;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (done) return true;
+    if (bar_try(bar, parity)) return true;
     if ((i & 255u) == 255u && global_ns() - start > kWaitLimitNs) return false;
   }
 }
