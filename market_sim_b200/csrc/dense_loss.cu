@@ -115,43 +115,49 @@ struct __align__(16) Partial {
   float m, l, dot, unused;
 };
 
-// One warp per row: the teacher's normaliser and entropy.
+// The teacher's normaliser and entropy of row r, by one warp.
+__device__ __forceinline__ float2 teacher_stat(const Wanted& w, uint32_t r, uint32_t entries,
+                                               uint32_t vocab) {
+  const uint32_t lane = threadIdx.x & 31;
+  const int32_t a = w.offsets[r], b = w.offsets[r + 1];
+  bool bad = a < 0 || b < a || (uint32_t)b > entries;
+  float m = -INFINITY;
+  if (!bad) {
+    for (int32_t k = a + (int32_t)lane; k < b; k += 32) {
+      const int32_t id = w.ids[k];
+      const float t = w.logits[k];
+      bad |= id < 0 || (uint32_t)id >= vocab || (k > a && w.ids[k - 1] >= id) || t != t ||
+             t == INFINITY;
+      m = fmaxf(m, t * w.inv_t);
+    }
+  }
+  bad = __any_sync(0xFFFFFFFFu, bad);
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  float2 st = make_float2(-INFINITY, 0.f);
+  if (bad) {
+    st.x = __uint_as_float(0x7FC00000u);
+  } else if (m > -INFINITY) {
+    float l = 0.f;
+    for (int32_t k = a + (int32_t)lane; k < b; k += 32) l += expf(w.logits[k] * w.inv_t - m);
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
+    st.x = m + logf(l);
+    float ent = 0.f;
+    for (int32_t k = a + (int32_t)lane; k < b; k += 32) {
+      const float lq = w.logits[k] * w.inv_t - st.x, q = expf(lq);
+      if (q > 0.f) ent += q * lq;
+    }
+    for (int o = 16; o; o >>= 1) ent += __shfl_xor_sync(0xFFFFFFFFu, ent, o);
+    st.y = ent;
+  }
+  return st;
+}
+
 __global__ void teacher_kernel(Wanted w, uint32_t rows, uint32_t entries, uint32_t vocab) {
   pdl_trigger();
-  const uint32_t lane = threadIdx.x & 31;
   for (uint32_t r = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; r < rows;
        r += (gridDim.x * blockDim.x) >> 5) {
-    const int32_t a = w.offsets[r], b = w.offsets[r + 1];
-    bool bad = a < 0 || b < a || (uint32_t)b > entries;
-    float m = -INFINITY;
-    if (!bad) {
-      for (int32_t k = a + (int32_t)lane; k < b; k += 32) {
-        const int32_t id = w.ids[k];
-        const float t = w.logits[k];
-        bad |= id < 0 || (uint32_t)id >= vocab || (k > a && w.ids[k - 1] >= id) || t != t ||
-               t == INFINITY;
-        m = fmaxf(m, t * w.inv_t);
-      }
-    }
-    bad = __any_sync(0xFFFFFFFFu, bad);
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    float2 st = make_float2(-INFINITY, 0.f);
-    if (bad) {
-      st.x = __uint_as_float(0x7FC00000u);
-    } else if (m > -INFINITY) {
-      float l = 0.f;
-      for (int32_t k = a + (int32_t)lane; k < b; k += 32) l += expf(w.logits[k] * w.inv_t - m);
-      for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
-      st.x = m + logf(l);
-      float ent = 0.f;
-      for (int32_t k = a + (int32_t)lane; k < b; k += 32) {
-        const float lq = w.logits[k] * w.inv_t - st.x, q = expf(lq);
-        if (q > 0.f) ent += q * lq;
-      }
-      for (int o = 16; o; o >>= 1) ent += __shfl_xor_sync(0xFFFFFFFFu, ent, o);
-      st.y = ent;
-    }
-    if (lane == 0) w.stat[r] = st;
+    const float2 st = teacher_stat(w, r, entries, vocab);
+    if ((threadIdx.x & 31) == 0) w.stat[r] = st;
   }
 }
 
@@ -280,6 +286,30 @@ __device__ __forceinline__ void mma_pair(uint32_t tmem_d, uint64_t adesc, uint64
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// One CTA on its own: MMA, commit, load.
+__device__ __forceinline__ void mma_one(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
+                                        uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit_one(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                   bar)
+               : "memory");
+}
+__device__ __forceinline__ void tma_load_local(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                               uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
 
@@ -891,19 +921,66 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
                  : "memory");
 }
 
+// hidden row . table row by one warp on the FP32 pipes, rounding to nearest.
+template <typename T>
+__device__ __forceinline__ float warp_score(const T* a, const T* b, uint32_t width) {
+  float s0 = 0.f, s1 = 0.f;
+  for (uint32_t c = (threadIdx.x & 31) * 8; c < width; c += 256) {
+    const uint4 x = ld_v4(a + c), y = ld_v4(b + c);
+    const T *xs = reinterpret_cast<const T*>(&x), *ys = reinterpret_cast<const T*>(&y);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      s0 = fmaf(Type<T>::to(xs[j]), Type<T>::to(ys[j]), s0);
+      s1 = fmaf(Type<T>::to(xs[j + 1]), Type<T>::to(ys[j + 1]), s1);
+    }
+  }
+  float s = s0 + s1;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+  return s;
+}
+
+// Joins the (m, l) of the lanes of a warp.
+__device__ __forceinline__ void warp_join(float& m, float& l) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const float om = __shfl_xor_sync(0xFFFFFFFFu, m, o), ol = __shfl_xor_sync(0xFFFFFFFFu, l, o);
+    const float mn = fmaxf(m, om);
+    l = l * (m == mn ? 1.f : exp2_approx(m - mn)) + ol * (om == mn ? 1.f : exp2_approx(om - mn));
+    m = mn;
+  }
+}
+__device__ __forceinline__ void join(float& m, float& l, const Partial& q) {
+  const float mn = fmaxf(m, q.m);
+  // a walk without a column has l = 0 at m = -inf
+  l = l * (m == mn ? 1.f : exp2_approx(m - mn)) + q.l * (q.m == mn ? 1.f : exp2_approx(q.m - mn));
+  m = mn;
+}
+
+__device__ __forceinline__ float set_loss(const Wanted& w, float2 s, float z, float dot) {
+  const float t = 1.f / w.inv_t;
+  return stat_empty(s) ? 0.f : (stat_invalid(s) ? s.x : t * t * (s.y + (z - dot)));
+}
+__device__ __forceinline__ float target_loss(uint32_t target, uint32_t vocab, float z, float dot) {
+  return target == kInvalid ? 0.f : (target >= vocab ? __uint_as_float(0x7FC00000u) : z - dot);
+}
+
 // One warp per row joins the walks' partial sums.  Row tile m's n_tiles tiles
 // lie in the ranges of a few consecutive pairs.  A target's score is computed
-// again on the FP32 pipes, with rounding to nearest, and takes the place of the
-// tensor core's in the sum: a loss is a difference of two numbers that a sure
-// row has nearly equal.
+// again on the FP32 pipes and takes the place of the tensor core's in the sum:
+// a loss is a difference of two numbers that a sure row has nearly equal.
 template <typename T>
 __global__ void merge_kernel(Wanted w, const T* hidden, const T* table, uint32_t width,
                              const Partial* part, uint32_t n_tiles, uint32_t total, uint32_t pairs,
                              uint32_t rows, uint32_t vocab, float* losses, float* lse) {
   pdl_trigger();
-  pdl_wait();
   const uint32_t r = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
   if (r >= rows) return;
+  const uint32_t target = w.targets ? w.targets[r] : kInvalid;
+  float score = 0.f;
+  if (target < vocab)
+    score = warp_score(hidden + (uint64_t)r * width, table + (uint64_t)target * width, width);
+  pdl_wait();  // what came before was not written by the previous kernel
   const uint64_t x0 = (uint64_t)(r / (2 * kBM)) * n_tiles, x1 = x0 + n_tiles - 1;
   // range of pair i: [total i / pairs, total (i + 1) / pairs)
   const uint32_t first = (uint32_t)(((x0 + 1) * pairs - 1) / total);
@@ -912,52 +989,263 @@ __global__ void merge_kernel(Wanted w, const T* hidden, const T* table, uint32_t
   float m = -INFINITY, l = 0.f, dot = 0.f;
   for (uint32_t s = lane; s < slots; s += 32) {
     const Partial q = part[(uint64_t)s * rows + r];
-    const float mn = fmaxf(m, q.m);
-    // a half tile beyond the vocabulary has l = 0 at m = -inf
-    l = l * (m == mn ? 1.f : exp2_approx(m - mn)) +
-        q.l * (q.m == mn ? 1.f : exp2_approx(q.m - mn));
-    m = mn;
+    join(m, l, q);
     dot += q.dot;
   }
+  warp_join(m, l);
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const float om = __shfl_xor_sync(0xFFFFFFFFu, m, o), ol = __shfl_xor_sync(0xFFFFFFFFu, l, o);
-    const float mn = fmaxf(m, om);
-    l = l * (m == mn ? 1.f : exp2_approx(m - mn)) + ol * (om == mn ? 1.f : exp2_approx(om - mn));
-    m = mn;
-    dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
-  }
-  const uint32_t target = w.targets ? w.targets[r] : kInvalid;
+  for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
   if (target < vocab) {
-    const T *a = hidden + (uint64_t)r * width, *b = table + (uint64_t)target * width;
-    float s0 = 0.f, s1 = 0.f;
-    for (uint32_t c = lane * 8; c < width; c += 256) {
-      const uint4 x = ld_v4(a + c), y = ld_v4(b + c);
-      const T *xs = reinterpret_cast<const T*>(&x), *ys = reinterpret_cast<const T*>(&y);
-#pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        s0 = fmaf(Type<T>::to(xs[j]), Type<T>::to(ys[j]), s0);
-        s1 = fmaf(Type<T>::to(xs[j + 1]), Type<T>::to(ys[j + 1]), s1);
-      }
-    }
-    float s = s0 + s1;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-    l += exp2_approx(fmaf(s, kLog2e, -m)) - exp2_approx(fmaf(dot, kLog2e, -m));
-    dot = s;
+    l += exp2_approx(fmaf(score, kLog2e, -m)) - exp2_approx(fmaf(dot, kLog2e, -m));
+    dot = score;
   }
   if (lane) return;
   const float z = (m + log2f(l)) * kLn2;
   lse[r] = z;
-  float loss;
-  if (w.targets) {
-    loss = target == kInvalid ? 0.f : (target >= vocab ? __uint_as_float(0x7FC00000u) : z - dot);
-  } else {
-    const float2 s = w.stat[r];
-    const float t = 1.f / w.inv_t;
-    loss = stat_empty(s) ? 0.f : (stat_invalid(s) ? s.x : t * t * (s.y + (z - dot)));
+  losses[r] = w.targets ? target_loss(target, vocab, z, dot) : set_loss(w, w.stat[r], z, dot);
+}
+
+// ---- few rows ------------------------------------------------------------
+//
+// Up to 64 rows: reading the table bounds the call.  The table takes the M side:
+// each CTA (one per SM) streams its own range of table rows once through a deep
+// ring (128 rows x 64 K a stage, fetched 32 rows at a time so that ranges are
+// even to 32 rows), against the hidden rows, which stay in shared memory (N =
+// rows rounded up to 16).  All its scores fit in TMEM, so the softmax needs no
+// running maximum: one pass for each row's maximum over the CTA's range, one
+// for the sum.  The wanted scores come from the FP32 pipes in the join.
+constexpr uint32_t kFewRows = 64;
+constexpr uint32_t kFewMaxStages = 12;
+constexpr uint32_t kFewThreads = 192;  // producer, MMA issuer, 4 epilogue warps
+constexpr uint32_t kFewSmem = 222 * 1024;
+
+struct FewParams {
+  uint32_t rows, n;         // n: rows rounded up to 16
+  uint32_t vocab, range;    // table rows per CTA, a multiple of 32
+  uint32_t w_chunks, stages;
+  float c2;                 // score scale / T in units of ln 2
+  Partial* partial;         // [CTA][rows]
+};
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  tmem_wait_ld();
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+  float m;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kFewThreads, 1)
+few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
+                const __grid_constant__ CUtensorMap tm_table, const FewParams p) {
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ uint64_t bars[2 * kFewMaxStages + 2];
+  __shared__ uint32_t tmem_at, abort_word, filled;
+  __shared__ float2 part[4][kFewRows];
+  const uint32_t hid = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t hid_chunk = p.n * 128;
+  const uint32_t ring = hid + ((p.w_chunks * hid_chunk + 1023u) & ~1023u);
+  const uint32_t bar0 = smem_u32(bars);
+  auto full = [&](uint32_t st) { return bar0 + 8 * st; };
+  auto empty = [&](uint32_t st) { return bar0 + 8 * (kFewMaxStages + st); };
+  const uint32_t h_full = bar0 + 8 * (2 * kFewMaxStages), done = h_full + 8;
+  volatile uint32_t* abort_flag = &abort_word;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t v0 = blockIdx.x * p.range;
+  const uint32_t count = min(p.range, p.vocab - v0);  // table rows of this CTA
+  const uint32_t tiles = (count + 127) / 128;
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    for (uint32_t i = 0; i < 2 * kFewMaxStages + 2; ++i) bar_init(bar0 + 8 * i, 1);
+    abort_word = 0u;
+    filled = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  losses[r] = loss;
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&tmem_at)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_at;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      Ring rg(p.stages);
+      bool ok = true;
+      bar_expect_tx(h_full, p.w_chunks * hid_chunk);
+      for (uint32_t kc = 0; kc < p.w_chunks; ++kc)
+        tma_load_local(hid + kc * hid_chunk, &tm_hidden, (int)(kc * kBK), 0, h_full);
+      for (uint32_t t = 0; ok && t < tiles; ++t) {
+        const uint32_t boxes = min(4u, (count - t * 128 + 31) / 32);
+        for (uint32_t kc = 0; kc < p.w_chunks; ++kc) {
+          if (!bar_wait(empty(rg.at), (rg.fills & 1u) ^ 1u)) {
+            ok = false;
+            break;
+          }
+          bar_expect_tx(full(rg.at), boxes * 4096);
+          for (uint32_t j = 0; j < boxes; ++j)
+            tma_load_local(ring + rg.at * kChunkBytes + j * 4096, &tm_table, (int)(kc * kBK),
+                           (int)(v0 + t * 128 + 32 * j), full(rg.at));
+          rg.next();
+        }
+      }
+      if (!ok) *abort_flag = 1u;
+      filled = rg.fills * rg.n + rg.at;
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // F32 accumulator, A and B of type T, K-major, M = 128
+      const uint32_t idesc = (1u << 4) | (Type<T>::kFormat << 7) | (Type<T>::kFormat << 10) |
+                             ((p.n >> 3) << 17) | (8u << 24);
+      Ring rg(p.stages);
+      bool ok = bar_wait(h_full, 0);
+      for (uint32_t t = 0; ok && t < tiles; ++t) {
+        for (uint32_t kc = 0; kc < p.w_chunks; ++kc) {
+          if (!bar_wait(full(rg.at), rg.fills & 1u)) {
+            ok = false;
+            break;
+          }
+          fence_after();
+          const uint64_t a = sw128_desc(ring + rg.at * kChunkBytes);
+          const uint64_t b = sw128_desc(hid + kc * hid_chunk);
+#pragma unroll
+          for (int k4 = 0; k4 < kBK / 16; ++k4)
+            mma_one(tmem + t * p.n, a + 2 * k4, b + 2 * k4, idesc, (kc | (uint32_t)k4) != 0u);
+          mma_commit_one(empty(rg.at));
+          rg.next();
+        }
+      }
+      if (!ok) *abort_flag = 1u;
+      mma_commit_one(done);  // everything issued, whether or not all of it was
+      bar_wait(done, 0);
+    }
+  } else {
+    const uint32_t quad = warp & 3;
+    const bool ok = bar_wait(done, 0) && !*abort_flag;
+    fence_after();
+    const uint32_t acc = tmem + ((quad * 32u) << 16);
+    for (uint32_t c = 0; c < p.n; c += 16) {
+      float mx[16], l[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) mx[j] = -INFINITY, l[j] = 0.f;
+      for (uint32_t t = 0; t < tiles; ++t) {
+        uint32_t r[16];
+        tmem_ld16(acc + t * p.n + c, r);
+        const bool in = t * 128 + quad * 32 + lane < count;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) mx[j] = fmaxf(mx[j], in ? __uint_as_float(r[j]) : -INFINITY);
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        mx[j] = warp_max(mx[j]) * p.c2;
+        l[j] = mx[j] > -INFINITY ? mx[j] : 0.f;  // a warp without a table row sums zeros
+      }
+      float sum[16] = {};
+      for (uint32_t t = 0; t < tiles; ++t) {
+        uint32_t r[16];
+        tmem_ld16(acc + t * p.n + c, r);
+        const bool in = t * 128 + quad * 32 + lane < count;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          sum[j] += in ? exp2_approx(fmaf(__uint_as_float(r[j]), p.c2, -l[j])) : 0.f;
+      }
+      // add over the lanes, halving the columns a lane keeps: lane x ends with
+      // column x / 2
+#pragma unroll
+      for (int h = 8, o = 16; h > 0; h >>= 1, o >>= 1) {
+        const bool up = lane & (uint32_t)o;
+#pragma unroll
+        for (int j = 0; j < h; ++j) {
+          const float give = up ? sum[j] : sum[j + h];
+          const float keep = up ? sum[j + h] : sum[j];
+          sum[j] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, o);
+          mx[j] = up ? mx[j + h] : mx[j];
+        }
+      }
+      sum[0] += __shfl_xor_sync(0xFFFFFFFFu, sum[0], 1);
+      if ((lane & 1u) == 0)
+        part[quad][c + lane / 2] = make_float2(mx[0], ok ? sum[0] : __uint_as_float(0x7FC00000u));
+    }
+    fence_before();
+    asm volatile("bar.sync 1, 128;" ::: "memory");  // the epilogue warps
+    const uint32_t r = threadIdx.x - 64;
+    if (r < p.rows) {
+      float m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) join(m, l, Partial{part[q][r].x, part[q][r].y, 0.f, 0.f});
+      pdl_wait();
+      p.partial[(uint64_t)blockIdx.x * p.rows + r] = Partial{m, l, 0.f, 0.f};
+    }
+  }
+  pdl_wait();
+  __syncthreads();
+  if (abort_word != 0u && threadIdx.x == 0) {  // copies in flight, bounded
+    bar_wait(h_full, 0);
+    for (uint32_t st = 0; st < p.stages; ++st)
+      if (filled > st) bar_wait(full(st), ((filled - st - 1u) / p.stages) & 1u);
+  }
+  __syncthreads();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(kTmemCols)
+                 : "memory");
+}
+
+// One block per row: the CTAs' sums, the wanted scores, the teacher's
+// distribution.
+constexpr uint32_t kJoinThreads = 256;
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads)
+few_rows_join_kernel(Wanted w, const T* hidden, const T* table, uint32_t width, const Partial* part,
+                     uint32_t slots, uint32_t rows, uint32_t entries, uint32_t vocab,
+                     float* losses, float* lse) {
+  __shared__ float dots[kJoinThreads / 32];
+  pdl_trigger();
+  const uint32_t r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const T* row = hidden + (uint64_t)r * width;
+  const uint32_t target = w.targets ? w.targets[r] : kInvalid;
+  float2 st = make_float2(-INFINITY, 0.f);
+  float dot = 0.f;  // of the row's wanted scores, as weighted
+  if (target < vocab) {
+    if (warp == 0) dot = warp_score(row, table + (uint64_t)target * width, width);
+  } else if (w.offsets) {
+    st = teacher_stat(w, r, entries, vocab);
+    if (!stat_empty(st) && !stat_invalid(st)) {
+      const int32_t end = w.offsets[r + 1];
+      for (int32_t k = w.offsets[r] + (int32_t)warp; k < end; k += kJoinThreads / 32) {
+        const float q = expf(w.logits[k] * w.inv_t - st.x);
+        const float s = warp_score(row, table + (uint64_t)w.ids[k] * width, width);
+        if (q > 0.f) dot = fmaf(q, s * w.inv_t, dot);
+      }
+    }
+  }
+  if (lane == 0) dots[warp] = dot;
+  __syncthreads();
+  if (warp) return;
+  dot = lane < kJoinThreads / 32 ? dots[lane] : 0.f;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
+  pdl_wait();  // what came before was not written by the previous kernel
+  float m = -INFINITY, l = 0.f;
+#pragma unroll 5
+  for (uint32_t s = lane; s < slots; s += 32) join(m, l, part[(uint64_t)s * rows + r]);
+  warp_join(m, l);
+  if (lane) return;
+  const float z = (m + log2f(l)) * kLn2;
+  lse[r] = z;
+  losses[r] = w.targets ? target_loss(target, vocab, z, dot) : set_loss(w, st, z, dot);
 }
 
 // d_hidden: the splits' sums in a fixed order, scaled and rounded; four columns
@@ -1027,6 +1315,8 @@ struct ForwardPlan {
     if (per < 1) per = 1;
     uint64_t slots = (n_tiles + per - 1) / per + 1;
     if (slots > n_tiles) slots = n_tiles;
+    // the few-rows kernel: one slot per CTA
+    if (rows <= kFewRows && slots < kMaxPairs) slots = kMaxPairs;
     stat = 0;
     partial = round_up(rows * sizeof(float2), 256);
     bytes = round_up(partial + 2 * slots * rows * sizeof(Partial), 256);
@@ -1253,6 +1543,72 @@ cudaError_t teacher_launch(const Wanted& w, uint64_t rows, uint64_t entries, uin
                       (uint32_t)rows, (uint32_t)entries, (uint32_t)vocab);
 }
 
+// How the few-rows kernel takes a call; stages 0: it does not.
+struct FewPlan {
+  uint32_t n, range, ctas, stages = 0;
+  uint64_t smem;
+  FewPlan(uint64_t rows, uint64_t width, uint64_t vocab, uint64_t sms) {
+    if (rows > kFewRows) return;
+    n = (uint32_t)round_up(rows, 16);
+    range = (uint32_t)round_up((vocab + sms - 1) / sms, 32);
+    ctas = (uint32_t)((vocab + range - 1) / range);
+    if ((uint64_t)(range + 127) / 128 * n > kTmemCols) return;  // scores beyond TMEM
+    const uint64_t hid = round_up((width + kBK - 1) / kBK * n * 128, 1024);
+    if (hid + 4 * kChunkBytes + 1024 > kFewSmem) return;  // no room for a ring
+    const uint64_t room = (kFewSmem - 1024 - hid) / kChunkBytes;
+    stages = (uint32_t)(room < kFewMaxStages ? room : kFewMaxStages);
+    smem = hid + stages * kChunkBytes + 1024;
+  }
+};
+
+// SMs of the current device, at most twice kMaxPairs (the workspace's slots).
+cudaError_t device_sms(uint32_t* sms) {
+  static std::mutex mu;
+  static uint32_t cached[64] = {};
+  int dev = 0, n = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  uint32_t& c = cached[dev & 63];
+  if (c == 0) {
+    e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    for (const void* k : {(const void*)few_rows_kernel<__half>,
+                          (const void*)few_rows_kernel<__nv_bfloat16>})
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFewSmem);
+    if (e != cudaSuccess) return e;
+    c = (uint32_t)n < 2 * kMaxPairs ? (uint32_t)n : 2 * kMaxPairs;
+  }
+  *sms = c;
+  return cudaSuccess;
+}
+
+template <typename T>
+mf_status forward_few(const FewPlan& few, Wanted w, const T* hidden, const T* table, uint64_t entries,
+                      void* partial, float* losses, float* lse, uint64_t rows, uint64_t width,
+                      uint64_t vocab, cudaStream_t s) {
+  CUtensorMap tm_h, tm_t;
+  if (!make_map<T>(&tm_h, hidden, rows, width, width, kBK, few.n) ||
+      !make_map<T>(&tm_t, table, vocab, width, width, kBK, 32))
+    return fail(MF_CUDA_RUNTIME_FAILURE);
+  FewParams p = {};
+  p.rows = (uint32_t)rows;
+  p.n = few.n;
+  p.vocab = (uint32_t)vocab;
+  p.range = few.range;
+  p.w_chunks = (uint32_t)((width + kBK - 1) / kBK);
+  p.stages = few.stages;
+  p.c2 = w.inv_t * (1.f + (float)width * kLostPerProduct) * kLog2e;
+  p.partial = static_cast<Partial*>(partial);
+  cudaError_t e = launch_after(few_rows_kernel<T>, few.ctas, kFewThreads, few.smem, s, false, tm_h,
+                               tm_t, p);
+  if (e == cudaSuccess)
+    e = launch_after(few_rows_join_kernel<T>, rows, kJoinThreads, 0, s, true, w, hidden, table,
+                     (uint32_t)width, static_cast<const Partial*>(p.partial), few.ctas, p.rows,
+                     (uint32_t)entries, p.vocab, losses, lse);
+  return launched(e);
+}
+
 template <typename T, bool kDistill>
 mf_status forward(Span hidden, Span embedding, Span targets, Span ids, Span logits,
                   float temperature, Span losses, Span lse, Span workspace, uint64_t rows,
@@ -1266,13 +1622,6 @@ mf_status forward(Span hidden, Span embedding, Span targets, Span ids, Span logi
   const ForwardPlan plan(rows, vocab);
   char* ws = static_cast<char*>(const_cast<void*>(workspace.p));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  uint32_t pairs = 0;
-  cudaError_t e = resident_pairs<T, true, kDistill>(&pairs);
-  if (e != cudaSuccess) return fail(MF_CUDA_RUNTIME_FAILURE, (uint32_t)e);
-  Maps maps = {};
-  if (!make_map<T>(&maps.hidden, hidden.p, rows, width, width, kBK, kBM) ||
-      !make_map<T>(&maps.table, embedding.p, vocab, width, width, kBK, kBN / 2))
-    return fail(MF_CUDA_RUNTIME_FAILURE);
   Wanted w{};
   w.inv_t = kDistill ? 1.f / temperature : 1.f;
   if (kDistill) {
@@ -1280,10 +1629,28 @@ mf_status forward(Span hidden, Span embedding, Span targets, Span ids, Span logi
     w.ids = static_cast<const int32_t*>(ids.p);
     w.logits = static_cast<const float*>(logits.p);
     w.stat = reinterpret_cast<float2*>(ws + plan.stat);
-    e = teacher_launch(w, rows, ids.bytes / 4, vocab, s);
-    if (e != cudaSuccess) return launched(e);
   } else {
     w.targets = static_cast<const uint32_t*>(targets.p);
+  }
+  uint32_t sms = 0;
+  cudaError_t e = device_sms(&sms);
+  if (e != cudaSuccess) return fail(MF_CUDA_RUNTIME_FAILURE, (uint32_t)e);
+  const FewPlan few(rows, width, vocab, sms);
+  if (few.stages > 0)
+    return forward_few<T>(few, w, static_cast<const T*>(hidden.p),
+                          static_cast<const T*>(embedding.p), ids.bytes / 4, ws + plan.partial,
+                          static_cast<float*>(const_cast<void*>(losses.p)),
+                          static_cast<float*>(const_cast<void*>(lse.p)), rows, width, vocab, s);
+  uint32_t pairs = 0;
+  e = resident_pairs<T, true, kDistill>(&pairs);
+  if (e != cudaSuccess) return fail(MF_CUDA_RUNTIME_FAILURE, (uint32_t)e);
+  Maps maps = {};
+  if (!make_map<T>(&maps.hidden, hidden.p, rows, width, width, kBK, kBM) ||
+      !make_map<T>(&maps.table, embedding.p, vocab, width, width, kBK, kBN / 2))
+    return fail(MF_CUDA_RUNTIME_FAILURE);
+  if (kDistill) {
+    e = teacher_launch(w, rows, ids.bytes / 4, vocab, s);
+    if (e != cudaSuccess) return launched(e);
   }
   const uint64_t total = plan.m_tiles * plan.n_tiles;
   if (pairs > total) pairs = (uint32_t)total;

@@ -666,8 +666,8 @@ class DenseLoss:
         import torch
 
         kinds = {torch.float16: "f16", torch.bfloat16: "bf16"}
-        if embedding.dtype not in kinds or embedding.dim() != 2:
-            raise ValueError("the table is fp16 or bfloat16 [vocab, hidden_size]")
+        if embedding.dtype not in kinds or embedding.dim() != 2 or not embedding.is_contiguous():
+            raise ValueError("the table is a contiguous fp16 or bfloat16 [vocab, hidden_size]")
         self.embedding = embedding
         self.vocab, self.hidden_size = int(embedding.shape[0]), int(embedding.shape[1])
         self.max_rows, self.stream = int(max_rows), stream
@@ -677,128 +677,137 @@ class DenseLoss:
             raise ValueError(f"rows, hidden_size, vocab = {sizes} are outside the limits")
         if backward:
             nbytes = max(nbytes, dense_loss_backward_workspace_bytes(*sizes))
-        self._backward = backward
+        self._backward, self._torch = backward, torch
+        self._device = embedding.device
         kind = kinds[embedding.dtype]
-        names = globals()
-        self._xent, self._xent_backward, self._distill, self._distill_backward = (
-            names[f"dense_{n}_{kind}"] for n in ("xent", "xent_backward", "distill",
-                                                 "distill_backward"))
-        self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=embedding.device)
-
-    def _tensor(self, name, t, dtype, shape):
-        if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() \
-                or t.device != self.embedding.device:
-            raise ValueError(f"{name}: a contiguous {dtype} tensor of shape {shape} on "
-                             f"{self.embedding.device} is wanted, not {t.dtype} {tuple(t.shape)} "
-                             f"on {t.device}")
-        return t
-
-    def _given(self, name, t, dtype, shape):
-        import torch
-
-        if t is None:  # from the memory of the stream that writes it
-            with torch.cuda.device(self.embedding.device), torch.cuda.stream(self._on()):
-                return torch.empty(shape, dtype=dtype, device=self.embedding.device)
-        return self._tensor(name, t, dtype, shape)
+        self._functions = {n: getattr(lib, f"mf_dense_{n}_{kind}")
+                           for n in ("xent", "xent_backward", "distill", "distill_backward")}
+        self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=self._device)
 
     def _on(self):
-        import torch
-
+        """The stream of the call, as torch knows it."""
         if self.stream is None:
-            return torch.cuda.current_stream(self.embedding.device)
+            return self._torch.cuda.current_stream(self._device)
         return _torch_stream(self.stream)
 
-    def _rows(self, hidden):
-        rows = int(hidden.shape[0])
+    def _wrong(self, name, t, dtype, shape):
+        return ValueError(f"{name}: a contiguous {dtype} tensor of shape {shape} on {self._device} "
+                          f"is wanted, not {t.dtype} {tuple(t.shape)} on {t.device}")
+
+    def _in(self, args, name, t, dtype, shape):
+        """Checks an input and appends its address and bytes."""
+        if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() \
+                or t.device != self._device:
+            raise self._wrong(name, t, dtype, shape)
+        args += (t.data_ptr(), t.numel() * t.element_size())
+
+    def _out(self, args, name, t, dtype, shape):
+        """The same for an output, which is made if it is not given: from the
+        memory of the stream that writes it."""
+        torch = self._torch
+        if t is None:
+            with torch.cuda.device(self._device), torch.cuda.stream(self._on()):
+                t = torch.empty(shape, dtype=dtype, device=self._device)
+        self._in(args, name, t, dtype, shape)
+        return t
+
+    def _begin(self, hidden):
+        rows = hidden.shape[0]
         if rows > self.max_rows:
             raise ValueError(f"batch of {rows} rows exceeds max_rows={self.max_rows}")
-        self._tensor("hidden", hidden, self.embedding.dtype, (rows, self.hidden_size))
-        self._tensor("embedding", self.embedding, self.embedding.dtype,
-                     (self.vocab, self.hidden_size))
-        return rows
+        args, table = [], self.embedding
+        self._in(args, "hidden", hidden, table.dtype, (rows, self.hidden_size))
+        self._in(args, "embedding", table, table.dtype, (self.vocab, self.hidden_size))
+        return rows, args
 
-    def _sets(self, rows, offsets, ids, teacher_logits):
-        import torch
+    def _sets(self, args, rows, offsets, ids, teacher_logits, temperature):
+        torch, entries = self._torch, (ids.numel(),)
+        self._in(args, "offsets", offsets, torch.int32, (rows + 1,))
+        self._in(args, "ids", ids, torch.int32, entries)
+        self._in(args, "teacher_logits", teacher_logits, torch.float32, entries)
+        args.append(float(temperature))
 
-        self._tensor("offsets", offsets, torch.int32, (rows + 1,))
-        self._tensor("ids", ids, torch.int32, (ids.numel(),))
-        self._tensor("teacher_logits", teacher_logits, torch.float32, (ids.numel(),))
-        return offsets, ids, teacher_logits
+    def _call(self, name, args, rows):
+        torch = self._torch
+        if self._device.type == "cuda" and torch.cuda.current_device() != self._device.index:
+            with torch.cuda.device(self._device):
+                st = self._launch(name, args, rows)
+        else:
+            st = self._launch(name, args, rows)
+        if st.code:
+            raise RuntimeError(f"mf_dense_{name} failed: {_status(st)}")
 
-    def _call(self, f, *args):
-        import torch
+    def _launch(self, name, args, rows):
+        ws = self.workspace
+        stream = self.stream
+        if stream is None:
+            stream = self._torch.cuda.current_stream(self._device)
+        return self._functions[name](*args, ws.data_ptr(), ws.numel(), rows, self.hidden_size,
+                                     self.vocab, _stream_handle(stream))
 
-        with torch.cuda.device(self.embedding.device):
-            st = f(*args, self._on())
-        if not st.ok():
-            raise RuntimeError(f"{f.__name__} failed: {st}")
+    def _losses(self, args, rows, losses, lse):
+        f32 = self._torch.float32
+        losses = self._out(args, "losses", losses, f32, (rows,))
+        return losses, self._out(args, "lse", lse, f32, (rows,))
 
     def cross_entropy(self, hidden, targets, losses=None, lse=None):
         """targets int32 [rows]; -1 (``INVALID_TOKEN_ID``) ignores a row."""
-        import torch
-
-        rows = self._rows(hidden)
-        self._tensor("targets", targets, torch.int32, (rows,))
-        losses = self._given("losses", losses, torch.float32, (rows,))
-        lse = self._given("lse", lse, torch.float32, (rows,))
-        self._call(self._xent, hidden, self.embedding, targets, losses, lse, self.workspace, rows,
-                   self.hidden_size, self.vocab)
-        return losses, lse
+        rows, args = self._begin(hidden)
+        self._in(args, "targets", targets, self._torch.int32, (rows,))
+        out = self._losses(args, rows, losses, lse)
+        self._call("xent", args, rows)
+        return out
 
     def distill(self, hidden, offsets, ids, teacher_logits, temperature=1.0, losses=None,
                 lse=None):
         """The teacher's top logits as CSR: offsets int32 [rows + 1], ids int32
         (ascending within a row) and teacher_logits float32 [entries]."""
-        import torch
+        rows, args = self._begin(hidden)
+        self._sets(args, rows, offsets, ids, teacher_logits, temperature)
+        out = self._losses(args, rows, losses, lse)
+        self._call("distill", args, rows)
+        return out
 
-        rows = self._rows(hidden)
-        sets = self._sets(rows, offsets, ids, teacher_logits)
-        losses = self._given("losses", losses, torch.float32, (rows,))
-        lse = self._given("lse", lse, torch.float32, (rows,))
-        self._call(self._distill, hidden, self.embedding, *sets, temperature, losses, lse,
-                   self.workspace, rows, self.hidden_size, self.vocab)
-        return losses, lse
-
-    def _gradients(self, rows, lse, grad_losses, d_hidden, d_embedding, hidden_grad,
+    def _gradients(self, args, rows, lse, grad_losses, d_hidden, d_embedding, hidden_grad,
                    embedding_grad):
-        import torch
-
         if not self._backward:
             raise RuntimeError("this DenseLoss was made with backward=False")
-        self._tensor("lse", lse, torch.float32, (rows,))
-        self._tensor("grad_losses", grad_losses, torch.float32, (rows,))
-        kind = self.embedding.dtype
+        f32, kind = self._torch.float32, self.embedding.dtype
+        self._in(args, "lse", lse, f32, (rows,))
+        self._in(args, "grad_losses", grad_losses, f32, (rows,))
         if hidden_grad:
-            d_hidden = self._given("d_hidden", d_hidden, kind, (rows, self.hidden_size))
+            d_hidden = self._out(args, "d_hidden", d_hidden, kind, (rows, self.hidden_size))
+        else:
+            d_hidden = None
+            args += (0, 0)
         if embedding_grad:
-            d_embedding = self._given("d_embedding", d_embedding, kind,
-                                      (self.vocab, self.hidden_size))
-        return (d_hidden if hidden_grad else None), (d_embedding if embedding_grad else None)
+            d_embedding = self._out(args, "d_embedding", d_embedding, kind,
+                                    (self.vocab, self.hidden_size))
+        else:
+            d_embedding = None
+            args += (0, 0)
+        return d_hidden, d_embedding
 
     def cross_entropy_backward(self, hidden, targets, lse, grad_losses, d_hidden=None,
                                d_embedding=None, hidden_grad=True, embedding_grad=True):
         """Gradients of ``(grad_losses * losses).sum()``; ``lse`` as
         ``cross_entropy`` returned it."""
-        import torch
-
-        rows = self._rows(hidden)
-        self._tensor("targets", targets, torch.int32, (rows,))
-        out = self._gradients(rows, lse, grad_losses, d_hidden, d_embedding, hidden_grad,
+        rows, args = self._begin(hidden)
+        self._in(args, "targets", targets, self._torch.int32, (rows,))
+        out = self._gradients(args, rows, lse, grad_losses, d_hidden, d_embedding, hidden_grad,
                               embedding_grad)
-        self._call(self._xent_backward, hidden, self.embedding, targets, lse, grad_losses, *out,
-                   self.workspace, rows, self.hidden_size, self.vocab)
+        self._call("xent_backward", args, rows)
         return out
 
     def distill_backward(self, hidden, offsets, ids, teacher_logits, temperature, lse, grad_losses,
                          d_hidden=None, d_embedding=None, hidden_grad=True, embedding_grad=True):
         """Gradients of ``(grad_losses * losses).sum()``; ``lse`` as ``distill``
         returned it with the same temperature."""
-        rows = self._rows(hidden)
-        sets = self._sets(rows, offsets, ids, teacher_logits)
-        out = self._gradients(rows, lse, grad_losses, d_hidden, d_embedding, hidden_grad,
+        rows, args = self._begin(hidden)
+        self._sets(args, rows, offsets, ids, teacher_logits, temperature)
+        out = self._gradients(args, rows, lse, grad_losses, d_hidden, d_embedding, hidden_grad,
                               embedding_grad)
-        self._call(self._distill_backward, hidden, self.embedding, *sets, temperature, lse,
-                   grad_losses, *out, self.workspace, rows, self.hidden_size, self.vocab)
+        self._call("distill_backward", args, rows)
         return out
 
 
