@@ -66,8 +66,8 @@ extern "C" {
 
 /* Bytes of device memory a forward call and a backward call need; 0 for sizes
  * outside the limits.  A backward call's holds two pieces of d of at most 128
- * MiB (512 bytes a row above 256 Ki rows), a copy of the hidden rows and a few
- * FP32 sums of d_hidden. */
+ * MiB (512 bytes a row above 256 Ki rows), a copy of the hidden rows and FP32
+ * sums of d_hidden of at most 128 MiB (4 bytes an element above 32 Mi elements). */
 MF_API uint64_t mf_dense_loss_workspace_bytes(uint64_t rows, uint64_t hidden_size, uint64_t vocab);
 MF_API uint64_t mf_dense_loss_backward_workspace_bytes(uint64_t rows, uint64_t hidden_size,
                                                        uint64_t vocab);

@@ -47,7 +47,6 @@ constexpr int kBN = 256;       // columns of a score tile
 constexpr int kBK = 64;        // K elements per chunk
 constexpr int kMaxStages = 6;
 constexpr int kChunkBytes = kBM * kBK * 2;    // 128 rows x 64 K: 16 KB
-constexpr int kScoreStage = 2 * kChunkBytes;
 constexpr int kRingBytes = 14 * kChunkBytes;  // tiles in shared memory, per CTA
 constexpr int kEpiWarps = 8;   // two per TMEM lane quadrant, each on half the columns
 constexpr int kThreads = 64 + 32 * kEpiWarps;
@@ -153,6 +152,7 @@ __device__ __forceinline__ float2 teacher_stat(const Wanted& w, uint32_t r, uint
 }
 
 __global__ void teacher_kernel(Wanted w, uint32_t rows, uint32_t entries, uint32_t vocab) {
+  pdl_wait();
   pdl_trigger();
   for (uint32_t r = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; r < rows;
        r += (gridDim.x * blockDim.x) >> 5) {
@@ -191,8 +191,8 @@ __global__ void __launch_bounds__(kSetupThreads)
 setup_kernel(Wanted w, const float* grad, const T* hidden, T* scaled, RowGrad* rg, float* gmax_out,
              uint32_t rows, uint32_t width, uint32_t vocab) {
   __shared__ float s_max[kSetupThreads / 32];
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float g = 0.f;
 #pragma unroll 8
@@ -252,6 +252,26 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
 }
 __device__ __forceinline__ void tmem_wait_ld() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// Two FP32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 
 __device__ __forceinline__ void add_v4(float* p, const uint32_t* v) {
@@ -319,7 +339,7 @@ struct Maps {
   CUtensorMap d_m, scaled_n;   // d^T H: 64 x 64 and 32 x 64 boxes
 };
 
-enum : uint32_t { kScore = 0, kHidden = 1, kTable = 2 };
+enum : uint32_t { kHidden = 0, kTable = 1, kScore = 2 };  // in the order of a walk
 
 struct Params {
   uint32_t rows, width, vocab;
@@ -327,6 +347,8 @@ struct Params {
   uint32_t w_chunks;            // ceil(width / 64)
   // score tiles: vocabulary rows [v0, v0 + cols)
   uint32_t v0, cols, n_tiles;
+  uint32_t keep_hidden;         // the hidden tile stays in shared memory
+  uint32_t s_ring, s_stages, s_stage_bytes;
   float score_scale;            // 1 + what the tensor core's additions lose
   Partial* partial;             // forward: [slots][rows]
   void* d;                      // backward: the piece being made
@@ -336,12 +358,11 @@ struct Params {
   // product tiles: vocabulary rows [pv0, pv0 + pcols)
   uint32_t pv0, pcols, bn, bn_tiles;
   uint32_t blocks;               // 256-row blocks that share a tile's B
-  uint32_t h_groups;             // m_tiles / blocks
   uint32_t t_tiles;              // 256-row tiles of the piece
   uint32_t p_stages, p_stage_bytes;
   uint32_t p_chunks, per_split;  // d E: K chunks of the piece, and of one split
-  float* planes;                 // [splits][rows][width]
-  uint32_t add;                  // planes hold earlier pieces' sums
+  float* planes;                 // this piece's: [splits][rows][width]
+  uint32_t add;                  // they hold an earlier piece's sums
   uint32_t r_chunks;             // d^T H: K chunks of the batch
   void* table_out;               // d_embedding + pv0 rows
   uint32_t wide_rows;            // its rows start on 32 bytes
@@ -354,11 +375,11 @@ struct Params {
 // differently, each kind with barriers of its own (a pair does all its products
 // before its scores, and drains between).
 //   products  p_stages x (up to 16 KB of B, blocks x 16 KB of A)
-//   scores    6 x (16 KB of table, 16 KB of hidden rows)
-// (Keeping the hidden tile in shared memory, 9 chunks of 16 KB at width 576,
-// and streaming the table alone through 5 stages: 352 against 356 us for 8,192
-// x 49,152 forward, where the tensor cores' power is the limit, but 81 against
-// 79 us for 4,096 x 16,384 and 37 against 34 us for 256 x 49,152.)
+//   scores    the hidden tile of 5 to 9 chunks of 16 KB and up to 6 x 16 KB of
+//             table; for other widths 6 x (16 KB of table, 16 KB of hidden rows)
+// What bounds the engine is shared memory's 128 bytes a clock: at the full rate of
+// the MMAs a score tile reads 64 and refills 64, or 32 with the hidden tile kept;
+// a product tile reads 73 and refills 73, or 57 with two blocks.
 struct Smem {
   static constexpr int bars = kRingBytes;
   // barriers: product full, empty, score full, empty [6 each],
@@ -373,51 +394,65 @@ struct Smem {
 constexpr size_t kSmemBytes = Smem::size + 1024;  // + alignment slack
 static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 
-struct Tile {
-  uint32_t kind, m, blocks, n, k0, chunks, split;
-};
-
-// The tiles of one pair, in order: d E, d^T H, scores.
+// Walks over the tiles of one pair, in order: d E, d^T H, scores.  Within a
+// kind n runs fastest, then m, then (d E) the split.  Steps are additions: the
+// MMA issuer has a few hundred clocks between tiles, and shares its scheduler
+// with two busy warps.
 struct Walk {
-  uint32_t h0, nh, t0, nt, s0, ns;
-  __device__ __forceinline__ Walk(const Params& p, uint32_t pair) {
-    h0 = p.hidden_at[pair];
-    nh = p.hidden_at[pair + 1] - h0;
-    t0 = p.table_at[pair];
-    nt = p.table_at[pair + 1] - t0;
-    s0 = p.score_at[pair];
-    ns = p.score_at[pair + 1] - s0;
+  uint32_t kind, left;             // tiles left of this kind, the current one among them
+  uint32_t n, m, split;            // the current tile
+  uint32_t blocks, k0, chunks;     // its row blocks of 256, first K chunk, chunks
+  uint32_t n_end, m_end, m_step, pair;
+
+  __device__ __forceinline__ Walk(const Params& p, uint32_t of_pair) : pair(of_pair) {
+    kind = kHidden;
+    start(p);
   }
-  __device__ __forceinline__ uint32_t count() const { return nh + nt + ns; }
-  __device__ __forceinline__ Tile at(const Params& p, uint32_t i) const {
-    Tile t;
-    t.k0 = 0;
-    t.split = 0;
-    if (i < nh) {
-      const uint32_t x = h0 + i, y = x / p.bn_tiles;
-      t.kind = kHidden;
-      t.n = x % p.bn_tiles;
-      t.m = y % p.h_groups * p.blocks;
-      t.blocks = min(p.blocks, p.m_tiles - t.m);
-      t.split = y / p.h_groups;
-      t.k0 = t.split * p.per_split;
-      t.chunks = min(p.per_split, p.p_chunks - t.k0);
-    } else if (i < nh + nt) {
-      const uint32_t x = t0 + i - nh;
-      t.kind = kTable;
-      t.n = x % p.bn_tiles;
-      t.m = x / p.bn_tiles * p.blocks;
-      t.blocks = min(p.blocks, p.t_tiles - t.m);
-      t.chunks = p.r_chunks;
-    } else {
-      const uint32_t x = s0 + i - nh - nt;
-      t.kind = kScore;
-      t.n = x % p.n_tiles;
-      t.m = x / p.n_tiles;
-      t.blocks = 1;
-      t.chunks = p.w_chunks;
+  __device__ __forceinline__ bool done() const { return left == 0; }
+  // The current kind's range, or the next one's that is not empty.
+  __device__ __forceinline__ void start(const Params& p) {
+    for (;;) {
+      const uint32_t* at = kind == kHidden ? p.hidden_at : (kind == kTable ? p.table_at : p.score_at);
+      uint32_t x = at[pair];
+      left = at[pair + 1] - x;
+      if (left > 0) {
+        n_end = kind == kScore ? p.n_tiles : p.bn_tiles;
+        m_end = kind == kTable ? p.t_tiles : p.m_tiles;
+        m_step = kind == kScore ? 1u : p.blocks;
+        n = x % n_end;
+        x /= n_end;
+        const uint32_t groups = (m_end + m_step - 1) / m_step;
+        m = x % groups * m_step;
+        split = x / groups;
+        set(p);
+        return;
+      }
+      if (kind == kScore) return;
+      ++kind;
     }
-    return t;
+  }
+  __device__ __forceinline__ void set(const Params& p) {
+    blocks = min(m_step, m_end - m);
+    k0 = split * p.per_split;  // 0 but for d E
+    chunks = kind == kHidden ? min(p.per_split, p.p_chunks - k0)
+                             : (kind == kTable ? p.r_chunks : p.w_chunks);
+  }
+  __device__ __forceinline__ void next(const Params& p) {
+    if (--left == 0) {
+      if (kind == kScore) return;
+      ++kind;
+      start(p);
+      return;
+    }
+    if (++n == n_end) {
+      n = 0;
+      m += m_step;
+      if (m >= m_end) {
+        m = 0;
+        ++split;
+      }
+      set(p);
+    }
   }
 };
 
@@ -530,7 +565,6 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   const bool leader = rank == 0;
   const uint32_t pair = blockIdx.x >> 1;
-  pdl_trigger();
 
   if (threadIdx.x == 0) {
     for (uint32_t st = 0; st < 4 * kMaxStages; ++st) bar_init(bar0 + 8 * st, 1);
@@ -554,22 +588,23 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
   cluster_sync();
   fence_after();
   const uint32_t tmem = *tmem_slot;
-  const Walk walk(p, pair);
-  const uint32_t tiles = walk.count();
+  Walk t(p, pair);
   pdl_wait();  // the previous kernel's results, before any bounded wait begins
+  pdl_trigger();
 
   if (warp == 0) {
     // ---- producer: both CTAs load their halves; the copies complete on the
     // leader's barriers, whose expected byte counts cover both ----
     if (lane == 0) {
-      Ring pr(p.p_stages), sr(kMaxStages);
+      Ring pr(p.p_stages), sr(p.s_stages);
+      uint32_t held = 0xFFFFFFFFu;  // row tile of the kept hidden tile
       const uint32_t leader_p_full = mapa(p_full(0), 0), leader_s_full = mapa(s_full(0), 0);
       bool ok = true;
-      for (uint32_t i = 0; ok && i < tiles && !*abort_flag; ++i) {
-        const Tile t = walk.at(p, i);
+      for (bool scores = false; ok && !t.done() && !*abort_flag; t.next(p)) {
         const int arow = (int)(t.m * 2 * kBM + rank * kBM);
         if (t.kind == kScore) {
-          if (i == walk.nh + walk.nt) {  // every product stage read by its MMAs
+          if (!scores) {  // every product stage read by its MMAs
+            scores = true;
             for (uint32_t st = 0; ok && st < pr.n; ++st) {
               const uint32_t fills = pr.fills + (st < pr.at ? 1u : 0u);
               ok = bar_wait(p_empty(st), (fills & 1u) ^ 1u);
@@ -578,16 +613,23 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
           }
           const int brow = (int)(p.v0 + t.n * kBN + rank * (kBN / 2));
           const int k_end = (int)(t.chunks * kBK);
-          for (int k = 0; k < k_end; k += kBK) {
+          // A kept hidden chunk may be replaced once the MMAs of the tile before
+          // have read it: `chunks` fills ago, while the stage's own wait covers
+          // all but the last s_stages <= chunks fills.
+          const bool load_a = !p.keep_hidden || t.m != held;
+          held = t.m;
+          const uint32_t bytes = 2 * (load_a ? 2 * kChunkBytes : kChunkBytes);
+          uint32_t a_at = sbase;
+          for (int k = 0; k < k_end; k += kBK, a_at += kChunkBytes) {
             if (!bar_wait(s_empty(sr.at), (sr.fills & 1u) ^ 1u)) {
               ok = false;
               break;
             }
             const uint32_t bar = leader_s_full + 8 * sr.at;
-            const uint32_t at = sbase + sr.at * kScoreStage;
-            if (leader) bar_expect_tx(s_full(sr.at), 2 * kScoreStage);
+            const uint32_t at = sbase + p.s_ring + sr.at * p.s_stage_bytes;
+            if (leader) bar_expect_tx(s_full(sr.at), bytes);
             tma_load_2d(at, &maps.table, k, brow, bar);
-            tma_load_2d(at + kChunkBytes, &maps.hidden, k, arow, bar);
+            if (load_a) tma_load_2d(p.keep_hidden ? a_at : at + kChunkBytes, &maps.hidden, k, arow, bar);
             sr.next();
           }
         } else if constexpr (!kForward) {
@@ -630,17 +672,16 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
     }
   } else if (warp == 1) {
     // ---- MMA issuer (leader CTA only) ----
-    if (lane == 0 && leader && tiles > 0) {
+    if (lane == 0 && leader && !t.done()) {
       // F32 accumulator, A and B of type T, M = 256; bit 15 / 16: A / B not K-major
       constexpr uint32_t kIdesc = (1u << 4) | (Type<T>::kFormat << 7) | (Type<T>::kFormat << 10) |
                                   ((uint32_t)((2 * kBM) >> 4) << 24);
       bool ok = true;
-      Ring pr(p.p_stages), sr(kMaxStages);
+      Ring pr(p.p_stages), sr(p.s_stages);
       uint32_t sub = 0;  // accumulators used so far: buffer sub & 1
       const uint64_t k_major = sw128_desc(sbase);  // + offset / 16: any place of the region
       const uint64_t m_major = mn_desc(sbase, 128), n_major = mn_desc(sbase, 64);
-      for (uint32_t i = 0; ok && i < tiles && !*abort_flag; ++i) {
-        const Tile t = walk.at(p, i);
+      for (; ok && !t.done() && !*abort_flag; t.next(p)) {
         for (uint32_t j = 0; ok && j < t.blocks; ++j)
           ok = bar_wait(acc_empty((sub + j) & 1u), (((sub + j) >> 1) & 1u) ^ 1u);
         if (!ok) break;
@@ -648,18 +689,23 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
         const uint32_t acc = tmem + (sub & 1u) * kBN;
         if (t.kind == kScore) {
           constexpr uint32_t idesc = kIdesc | ((uint32_t)(kBN >> 3) << 17);
+          bool ready = bar_try(s_full(sr.at), sr.fills & 1u);
           for (uint32_t kc = 0; kc < t.chunks; ++kc) {
-            if (!bar_wait(s_full(sr.at), sr.fills & 1u)) {
+            if (!ready && !bar_wait(s_full(sr.at), sr.fills & 1u)) {
               ok = false;
               break;
             }
-            fence_after();
-            const uint64_t b = k_major + sr.at * (kScoreStage / 16), a = b + kChunkBytes / 16;
+            const uint32_t at = sr.at;
+            const uint64_t b = k_major + (p.s_ring + at * p.s_stage_bytes) / 16;
+            const uint64_t a = p.keep_hidden ? k_major + kc * (kChunkBytes / 16)
+                                             : b + kChunkBytes / 16;
+            sr.next();
+            // asked before the MMAs, whose issue takes as long as they do
+            ready = bar_try(s_full(sr.at), sr.fills & 1u);
 #pragma unroll
             for (int k4 = 0; k4 < kBK / 16; ++k4)
               mma_pair(acc, a + 2 * k4, b + 2 * k4, idesc, (kc | (uint32_t)k4) != 0u);
-            mma_commit_pair(s_empty(sr.at));  // frees the stage (both CTAs) once read
-            sr.next();
+            mma_commit_pair(s_empty(at));  // frees the stage (both CTAs) once read
           }
         } else if constexpr (!kForward) {
           const uint32_t idesc = kIdesc | ((p.bn >> 3) << 17) |
@@ -668,13 +714,16 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
           const uint32_t a_step = t.kind == kTable ? 2048 / 16 : 2;
           const uint32_t stage = p.p_stage_bytes / 16;
           const uint32_t acc1 = tmem + ((sub + 1) & 1u) * kBN;
+          bool ready = bar_try(p_full(pr.at), pr.fills & 1u);
           for (uint32_t kc = 0; kc < t.chunks; ++kc) {
-            if (!bar_wait(p_full(pr.at), pr.fills & 1u)) {
+            if (!ready && !bar_wait(p_full(pr.at), pr.fills & 1u)) {
               ok = false;
               break;
             }
-            fence_after();
-            const uint64_t b = n_major + pr.at * stage, a = a0 + pr.at * stage;
+            const uint32_t at = pr.at;
+            const uint64_t b = n_major + at * stage, a = a0 + at * stage;
+            pr.next();
+            ready = bar_try(p_full(pr.at), pr.fills & 1u);
 #pragma unroll
             for (int k4 = 0; k4 < kBK / 16; ++k4)
               mma_pair(acc, a + a_step * k4, b + 64 * k4, idesc, (kc | (uint32_t)k4) != 0u);
@@ -684,8 +733,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
                 mma_pair(acc1, a + kChunkBytes / 16 + a_step * k4, b + 64 * k4, idesc,
                          (kc | (uint32_t)k4) != 0u);
             }
-            mma_commit_pair(p_empty(pr.at));
-            pr.next();
+            mma_commit_pair(p_empty(at));
           }
         }
         if (!ok) break;
@@ -708,11 +756,14 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
     const float t2 = w.inv_t * kLog2e;  // of the teacher's logits
     const float inv_t = w.inv_t * p.score_scale;
     const float c2 = inv_t * kLog2e;
+    const float scale = kForward || p.gmax == nullptr ? 1.f : *p.gmax / Type<T>::kScale;  // of d^T H
     bool dead = false;
     // state of the row this thread holds while it walks along score tiles
     uint32_t cur_m = 0xFFFFFFFFu, row = 0, slot = 0;
     bool live = false;
     float tlse2 = 0.f, run_m = -INFINITY, run_l = 0.f, dot = 0.f, z2 = 0.f, coef = 0.f;
+    float e2 = 0.f;                // log2 |coef| - z2
+    uint32_t keep = 0, sign = 0;   // of the packed pairs of d
     Cursor<kDistill> cur;
     cur.none();
     auto release = [&](uint32_t buf) {  // the accumulator has been read
@@ -726,14 +777,11 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
             Partial{dead ? nan : run_m, dead ? nan : run_l, dot, 0.f};
     };
     uint32_t sub = 0;
-    for (uint32_t i = 0, block = 0; i < tiles; ++sub) {
-      Tile t = walk.at(p, i);
-      t.m += block;
-      if (++block == t.blocks) block = 0, ++i;
+    for (uint32_t block = 0; !t.done(); ++sub) {
       const uint32_t buf = sub & 1u;
       if (t.kind == kScore) {
         const uint32_t v = p.v0 + t.n * kBN + half * (kBN / 2);
-        if (t.m != cur_m) {
+        if (t.m != cur_m) {  // (a score tile has one block)
           flush();
           cur_m = t.m;
           row = t.m * 2 * kBM + tile_row;
@@ -752,6 +800,9 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
           } else if (live) {
             coef = p.rg[row].coef;
             z2 = p.lse[row] * kLog2e;
+            e2 = log2f(fabsf(coef)) - z2;
+            keep = coef != 0.f ? 0xFFFFFFFFu : 0u;
+            sign = coef < 0.f ? 0x80008000u : 0u;
             live = coef != 0.f;
           }
           if (kDistill && live) {
@@ -788,16 +839,31 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
               for (int j = 0; j < 64; ++j)
                 if (c + j >= c_end) r[j] = 0xFF800000u;  // -inf
             }
-            float mx = __uint_as_float(r[0]);
+            float mx[4];
 #pragma unroll
-            for (int j = 1; j < 64; ++j) mx = fmaxf(mx, __uint_as_float(r[j]));
-            const float m = fmaxf(run_m, mx * c2);
-            float l[4] = {run_l * exp2_approx(run_m - m), 0.f, 0.f, 0.f};
+            for (int j = 0; j < 4; ++j) mx[j] = __uint_as_float(r[j]);
 #pragma unroll
-            for (int j = 0; j < 64; ++j)
-              l[j & 3] += exp2_approx(fmaf(__uint_as_float(r[j]), c2, -m));
+            for (int j = 4; j < 64; j += 8)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (j + 4 + e < 64)
+                  mx[e] = fmaxf(fmaxf(mx[e], __uint_as_float(r[j + e])),
+                                __uint_as_float(r[j + 4 + e]));
+                else
+                  mx[e] = fmaxf(mx[e], __uint_as_float(r[j + e]));
+            const float m =
+                fmaxf(run_m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c2);
+            float2 l[2] = {make_float2(run_l * exp2_approx(run_m - m), 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+            for (int j = 0; j < 64; j += 2) {
+              const float2 x = fma2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])),
+                                    make_float2(c2, c2), make_float2(-m, -m));
+              l[(j >> 1) & 1] =
+                  add2(l[(j >> 1) & 1], make_float2(exp2_approx(x.x), exp2_approx(x.y)));
+            }
             run_m = m;
-            run_l = (l[0] + l[1]) + (l[2] + l[3]);
+            l[0] = add2(l[0], l[1]);
+            run_l = l[0].x + l[0].y;
             while (__any_sync(0xFFFFFFFFu, cur.id[0] - col < 64u)) {
               const float s = pick64(r, cur.id[0] - col);
               if (cur.id[0] - col < 64u) {
@@ -807,18 +873,18 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
               }
             }
           } else {
+            // |coef| goes into the exponent
             T* out = static_cast<T*>(p.d) + (uint64_t)row * p.pitch + t.n * kBN + c;
-            const uint32_t keep = coef != 0.f ? 0xFFFFFFFFu : 0u;
+            const float2 cc = make_float2(c2, c2), ee = make_float2(e2, e2);
             if (row < p.rows) {
 #pragma unroll
               for (int j = 0; j < 64; j += 16) {
                 uint32_t v[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                  const float x = exp2_approx(fmaf(__uint_as_float(r[j + 2 * e]), c2, -z2)) * coef;
-                  const float y =
-                      exp2_approx(fmaf(__uint_as_float(r[j + 2 * e + 1]), c2, -z2)) * coef;
-                  v[e] = Type<T>::pack(x, y) & keep;
+                  const float2 x = fma2(make_float2(__uint_as_float(r[j + 2 * e]),
+                                                    __uint_as_float(r[j + 2 * e + 1])), cc, ee);
+                  v[e] = (Type<T>::pack(exp2_approx(x.x), exp2_approx(x.y)) & keep) ^ sign;
                 }
                 store_v8(out + j, v);
               }
@@ -835,10 +901,9 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
         }
       } else if constexpr (!kForward) {
         const uint32_t c_half = p.bn / 2;
-        const uint32_t m_row = t.m * 2 * kBM + tile_row;
+        const uint32_t m_row = (t.m + block) * 2 * kBM + tile_row;
         const bool mine = m_row < (t.kind == kHidden ? p.rows : p.pcols);
         const uint64_t at = ((uint64_t)(t.kind == kHidden ? t.split : 0u) * p.rows + m_row) * p.width;
-        const float scale = t.kind == kTable ? *p.gmax / Type<T>::kScale : 1.f;
 #pragma unroll 1
         for (uint32_t c = 0; c < c_half; c += 64) {
           uint32_t r[2][32];
@@ -889,9 +954,14 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
             }
           }
         }
+        if (++block == t.blocks) {
+          block = 0;
+          t.next(p);
+        }
         continue;
       }
       release(buf);
+      t.next(p);
     }
     flush();
   }
@@ -903,7 +973,8 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
       for (uint32_t st = 0; st < kMaxStages; ++st) {
         if (issued[0] > st && st < p.p_stages)
           bar_wait(p_full(st), ((issued[0] - st - 1u) / p.p_stages) & 1u);
-        if (issued[1] > st) bar_wait(s_full(st), ((issued[1] - st - 1u) / kMaxStages) & 1u);
+        if (issued[1] > st && st < p.s_stages)
+          bar_wait(s_full(st), ((issued[1] - st - 1u) / p.s_stages) & 1u);
       }
     } else {
       // the peer's copies complete on the leader's barriers: give any still
@@ -973,7 +1044,6 @@ template <typename T>
 __global__ void merge_kernel(Wanted w, const T* hidden, const T* table, uint32_t width,
                              const Partial* part, uint32_t n_tiles, uint32_t total, uint32_t pairs,
                              uint32_t rows, uint32_t vocab, float* losses, float* lse) {
-  pdl_trigger();
   const uint32_t r = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
   if (r >= rows) return;
   const uint32_t target = w.targets ? w.targets[r] : kInvalid;
@@ -981,12 +1051,14 @@ __global__ void merge_kernel(Wanted w, const T* hidden, const T* table, uint32_t
   if (target < vocab)
     score = warp_score(hidden + (uint64_t)r * width, table + (uint64_t)target * width, width);
   pdl_wait();  // what came before was not written by the previous kernel
+  pdl_trigger();
   const uint64_t x0 = (uint64_t)(r / (2 * kBM)) * n_tiles, x1 = x0 + n_tiles - 1;
   // range of pair i: [total i / pairs, total (i + 1) / pairs)
   const uint32_t first = (uint32_t)(((x0 + 1) * pairs - 1) / total);
   const uint32_t last = (uint32_t)(((x1 + 1) * pairs - 1) / total);
   const uint32_t slots = 2 * (last - first + 1);
   float m = -INFINITY, l = 0.f, dot = 0.f;
+#pragma unroll 5
   for (uint32_t s = lane; s < slots; s += 32) {
     const Partial q = part[(uint64_t)s * rows + r];
     join(m, l, q);
@@ -1061,7 +1133,6 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
   const uint32_t v0 = blockIdx.x * p.range;
   const uint32_t count = min(p.range, p.vocab - v0);  // table rows of this CTA
   const uint32_t tiles = (count + 127) / 128;
-  pdl_trigger();
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < 2 * kFewMaxStages + 2; ++i) bar_init(bar0 + 8 * i, 1);
     abort_word = 0u;
@@ -1079,6 +1150,8 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
   __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_at;
+  pdl_wait();  // what the previous kernel wrote, before any bounded wait begins
+  pdl_trigger();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -1185,11 +1258,9 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
       float m = -INFINITY, l = 0.f;
 #pragma unroll
       for (int q = 0; q < 4; ++q) join(m, l, Partial{part[q][r].x, part[q][r].y, 0.f, 0.f});
-      pdl_wait();
       p.partial[(uint64_t)blockIdx.x * p.rows + r] = Partial{m, l, 0.f, 0.f};
     }
   }
-  pdl_wait();
   __syncthreads();
   if (abort_word != 0u && threadIdx.x == 0) {  // copies in flight, bounded
     bar_wait(h_full, 0);
@@ -1212,7 +1283,6 @@ few_rows_join_kernel(Wanted w, const T* hidden, const T* table, uint32_t width, 
                      uint32_t slots, uint32_t rows, uint32_t entries, uint32_t vocab,
                      float* losses, float* lse) {
   __shared__ float dots[kJoinThreads / 32];
-  pdl_trigger();
   const uint32_t r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const T* row = hidden + (uint64_t)r * width;
   const uint32_t target = w.targets ? w.targets[r] : kInvalid;
@@ -1234,10 +1304,13 @@ few_rows_join_kernel(Wanted w, const T* hidden, const T* table, uint32_t width, 
   if (lane == 0) dots[warp] = dot;
   __syncthreads();
   if (warp) return;
+  // The inputs were complete before this kernel could start: every kernel here
+  // lets the next one start only after its own wait for the one before.
   dot = lane < kJoinThreads / 32 ? dots[lane] : 0.f;
 #pragma unroll
   for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
-  pdl_wait();  // what came before was not written by the previous kernel
+  pdl_wait();
+  pdl_trigger();
   float m = -INFINITY, l = 0.f;
 #pragma unroll 5
   for (uint32_t s = lane; s < slots; s += 32) join(m, l, part[(uint64_t)s * rows + r]);
@@ -1249,22 +1322,40 @@ few_rows_join_kernel(Wanted w, const T* hidden, const T* table, uint32_t width, 
 }
 
 // d_hidden: the splits' sums in a fixed order, scaled and rounded; four columns
-// a thread.
-template <typename T>
-__global__ void __launch_bounds__(128) finish_kernel(const float* planes, uint32_t splits,
-                                                     const RowGrad* rg, T* out, uint32_t rows,
-                                                     uint32_t width) {
-  pdl_wait();
-  const uint64_t i = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) * 4;
+// a thread, and with many splits eight threads for the same columns, each with
+// every eighth split.
+constexpr uint32_t kFinishThreads = 256;
+template <typename T, uint32_t kGroups>
+__global__ void __launch_bounds__(kFinishThreads)
+finish_kernel(const float* planes, uint32_t splits, const RowGrad* rg, T* out, uint32_t rows,
+              uint32_t width) {
+  constexpr uint32_t kColumns = kFinishThreads / kGroups;
+  __shared__ float4 part[kGroups][kColumns];
+  const uint32_t c = threadIdx.x % kColumns, group = threadIdx.x / kColumns;
+  const uint64_t i = ((uint64_t)blockIdx.x * kColumns + c) * 4;
   const uint64_t n = (uint64_t)rows * width;
-  if (i >= n) return;
+  pdl_wait();
+  pdl_trigger();
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (uint32_t s = 0; s < splits; ++s) {
-    const float4 a = *reinterpret_cast<const float4*>(planes + s * n + i);
-    v = make_float4(v.x + a.x, v.y + a.y, v.z + a.z, v.w + a.w);
+  if (i < n) {
+#pragma unroll 4
+    for (uint32_t s = group; s < splits; s += kGroups) {
+      const float4 a = __ldcg(reinterpret_cast<const float4*>(planes + s * n + i));
+      v = make_float4(v.x + a.x, v.y + a.y, v.z + a.z, v.w + a.w);
+    }
   }
-  const RowGrad g = rg[i / width];
+  if (kGroups > 1) {
+    part[group][c] = v;
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (uint32_t g = 1; g < kGroups; ++g) {
+      const float4 a = part[g][c];
+      v = make_float4(v.x + a.x, v.y + a.y, v.z + a.z, v.w + a.w);
+    }
+  }
+  if (i >= n) return;
+  const RowGrad g = rg[(uint32_t)(i / width)];
   const bool in = g.coef != 0.f;
   *reinterpret_cast<uint2*>(out + i) =
       make_uint2(Type<T>::pack(in ? v.x * g.scale : 0.f, in ? v.y * g.scale : 0.f),
@@ -1329,6 +1420,7 @@ struct BackwardPlan {
   uint32_t bn, bn_tiles;  // product tiles along the hidden width
   uint32_t blocks;        // row blocks that share a product tile's B
   uint32_t splits, per_split;
+  uint32_t sets;          // pieces with planes of their own
   BackwardPlan(uint64_t rows, uint64_t width, uint64_t vocab) {
     m_tiles = (rows + 2 * kBM - 1) / (2 * kBM);
     uint64_t c = kPieceBytes / (2 * rows) / kBN * kBN;
@@ -1351,12 +1443,18 @@ struct BackwardPlan {
     splits = (uint32_t)((chunks + most - 1) / most);
     per_split = (uint32_t)((chunks + splits - 1) / splits);
     splits = (uint32_t)((chunks + per_split - 1) / per_split);
+    // Sums kept apart cost a store a piece and are joined at the end; adding at
+    // L2 from this layout (a row a thread) made a launch 25 us longer at 8,192 rows
+    const uint64_t set = (uint64_t)splits * rows * width * 4;
+    sets = (uint32_t)(kPieceBytes / set);
+    if (sets > pieces) sets = pieces;
+    if (sets < 1) sets = 1;
     stat = 0;
     rg = round_up(stat + rows * sizeof(float2), 256);
     gmax = round_up(rg + rows * sizeof(RowGrad), 256);
     scaled = gmax + 256;
     planes = round_up(scaled + rows * width * 2, 256);
-    piece[0] = round_up(planes + (uint64_t)splits * rows * width * 4, 256);
+    piece[0] = round_up(planes + sets * set, 256);
     const uint64_t one = round_up(rows * cols * 2, 256);
     piece[1] = piece[0] + (pieces > 1 ? one : 0);
     bytes = piece[1] + one;
@@ -1459,11 +1557,12 @@ cudaError_t resident_pairs(uint32_t* pairs) {
   return cudaSuccess;
 }
 
-// A launch that may begin while the previous kernel of the call drains; every
-// kernel waits for it before it reads or writes.
+// A launch that may begin while the previous kernel on the stream drains: every
+// kernel waits for it before it reads what it wrote or writes anything, and
+// lets its own successor begin only after that wait.
 template <typename... P, typename... A>
 cudaError_t launch_after(void (*kernel)(P...), uint64_t blocks, unsigned threads, size_t smem,
-                         cudaStream_t s, bool after, A... args) {
+                         cudaStream_t s, A... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks, 1, 1);
   cfg.blockDim = dim3(threads, 1, 1);
@@ -1473,7 +1572,7 @@ cudaError_t launch_after(void (*kernel)(P...), uint64_t blocks, unsigned threads
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = after ? 1 : 0;
+  cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
@@ -1485,6 +1584,12 @@ Params base_params(uint64_t rows, uint64_t width, uint64_t vocab) {
   p.vocab = (uint32_t)vocab;
   p.m_tiles = (uint32_t)((rows + 2 * kBM - 1) / (2 * kBM));
   p.w_chunks = (uint32_t)((width + kBK - 1) / kBK);
+  p.keep_hidden = p.w_chunks >= 5 && p.w_chunks <= 9;
+  p.s_ring = p.keep_hidden ? p.w_chunks * kChunkBytes : 0;
+  p.s_stage_bytes = (p.keep_hidden ? 1 : 2) * kChunkBytes;
+  p.s_stages = (kRingBytes - p.s_ring) / p.s_stage_bytes;
+  if (p.s_stages > kMaxStages) p.s_stages = kMaxStages;
+  if (p.keep_hidden && p.s_stages > p.w_chunks) p.s_stages = p.w_chunks;
   p.p_stages = 1;
   p.score_scale = 1.f + (float)width * kLostPerProduct;
   return p;
@@ -1539,7 +1644,7 @@ mf_status launched(cudaError_t e) {
 cudaError_t teacher_launch(const Wanted& w, uint64_t rows, uint64_t entries, uint64_t vocab,
                            cudaStream_t s) {
   const uint64_t blocks = (rows + 7) / 8;
-  return launch_after(teacher_kernel, blocks < 1184 ? blocks : 1184, 256, 0, s, false, w,
+  return launch_after(teacher_kernel, blocks < 1184 ? blocks : 1184, 256, 0, s, w,
                       (uint32_t)rows, (uint32_t)entries, (uint32_t)vocab);
 }
 
@@ -1600,10 +1705,10 @@ mf_status forward_few(const FewPlan& few, Wanted w, const T* hidden, const T* ta
   p.stages = few.stages;
   p.c2 = w.inv_t * (1.f + (float)width * kLostPerProduct) * kLog2e;
   p.partial = static_cast<Partial*>(partial);
-  cudaError_t e = launch_after(few_rows_kernel<T>, few.ctas, kFewThreads, few.smem, s, false, tm_h,
+  cudaError_t e = launch_after(few_rows_kernel<T>, few.ctas, kFewThreads, few.smem, s, tm_h,
                                tm_t, p);
   if (e == cudaSuccess)
-    e = launch_after(few_rows_join_kernel<T>, rows, kJoinThreads, 0, s, true, w, hidden, table,
+    e = launch_after(few_rows_join_kernel<T>, rows, kJoinThreads, 0, s, w, hidden, table,
                      (uint32_t)width, static_cast<const Partial*>(p.partial), few.ctas, p.rows,
                      (uint32_t)entries, p.vocab, losses, lse);
   return launched(e);
@@ -1659,10 +1764,10 @@ mf_status forward(Span hidden, Span embedding, Span targets, Span ids, Span logi
   p.n_tiles = (uint32_t)plan.n_tiles;
   p.partial = reinterpret_cast<Partial*>(ws + plan.partial);
   for (uint32_t i = 0; i <= pairs; ++i) p.score_at[i] = (uint32_t)(total * i / pairs);
-  e = launch_after(engine_kernel<T, true, kDistill>, 2 * pairs, kThreads, kSmemBytes, s, kDistill,
+  e = launch_after(engine_kernel<T, true, kDistill>, 2 * pairs, kThreads, kSmemBytes, s,
                    maps, p, w);
   if (e != cudaSuccess) return launched(e);
-  e = launch_after(merge_kernel<T>, (rows + 7) / 8, 256, 0, s, true, w,
+  e = launch_after(merge_kernel<T>, (rows + 7) / 8, 256, 0, s, w,
                    static_cast<const T*>(hidden.p), static_cast<const T*>(embedding.p), p.width,
                    static_cast<const Partial*>(p.partial), p.n_tiles, (uint32_t)total, pairs,
                    p.rows, p.vocab, static_cast<float*>(const_cast<void*>(losses.p)),
@@ -1715,23 +1820,21 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
   } else {
     w.targets = static_cast<const uint32_t*>(targets.p);
   }
-  err = launch_after(setup_kernel<T>, rows < 32 * 148 ? (rows + 31) / 32 : 148, kSetupThreads, 0, s, kDistill, w,
+  err = launch_after(setup_kernel<T>, rows < 32 * 148 ? (rows + 31) / 32 : 148, kSetupThreads, 0, s, w,
                      static_cast<const float*>(grad.p), static_cast<const T*>(hidden.p), scaled,
                      rg, gmax, (uint32_t)rows, (uint32_t)width, (uint32_t)vocab);
   if (err != cudaSuccess) return launched(err);
 
   Params p = base_params(rows, width, vocab);
-  p.pitch = plan.cols;
   p.lse = static_cast<const float*>(lse.p);
   p.rg = rg;
   p.bn = plan.bn;
   p.bn_tiles = plan.bn_tiles;
   p.blocks = plan.blocks;
-  p.h_groups = (p.m_tiles + p.blocks - 1) / p.blocks;
+  p.pitch = plan.cols;
   p.p_stage_bytes = p.blocks * kChunkBytes + p.bn * kBK;
   p.p_stages = kRingBytes / p.p_stage_bytes < kMaxStages ? kRingBytes / p.p_stage_bytes : kMaxStages;
   p.per_split = plan.per_split;
-  p.planes = planes;
   p.r_chunks = (uint32_t)((rows + kBK - 1) / kBK);
   p.gmax = gmax;
   p.wide_rows = width % 16 == 0 && (uintptr_t)de % 32 == 0;
@@ -1739,6 +1842,7 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
     const uint64_t left = vocab - (uint64_t)i * plan.cols;
     return (uint32_t)(left < plan.cols ? left : plan.cols);
   };
+  uint32_t n_planes = 0;
   // launch i makes piece i of d and the products of piece i - 1
   for (uint32_t i = 0; i <= plan.pieces; ++i) {
     double load[kMaxPairs] = {};
@@ -1747,16 +1851,19 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
       p.pv0 = (i - 1) * plan.cols;
       p.pcols = piece_cols(i - 1);
       p.p_chunks = (p.pcols + kBK - 1) / kBK;
-      p.add = i > 1;
+      p.add = i > plan.sets;
+      p.planes = planes + (uint64_t)((i - 1) % plan.sets) * plan.splits * rows * width;
       p.table_out = de ? de + (uint64_t)p.pv0 * width : nullptr;
       const void* d = ws + plan.piece[(i - 1) & 1];
       if (!make_map<T>(&maps.d_k, d, rows, p.pcols, plan.cols, kBK, kBM) ||
           !make_map<T>(&maps.d_m, d, rows, p.pcols, plan.cols, kBK, kBK))
         return fail(MF_CUDA_RUNTIME_FAILURE);
-      // a short last piece fills only the first splits
       const uint32_t splits = (p.p_chunks + p.per_split - 1) / p.per_split;
+      // a short last piece fills the first splits of its set; a set that is
+      // used again was filled by whole pieces before
+      n_planes = i <= plan.sets ? (i - 1) * plan.splits + splits : plan.sets * plan.splits;
       p.t_tiles = (p.pcols + 2 * kBM - 1) / (2 * kBM);
-      if (dh) n_hidden = splits * p.h_groups * p.bn_tiles;
+      if (dh) n_hidden = splits * ((p.m_tiles + p.blocks - 1) / p.blocks) * p.bn_tiles;
       if (de) n_table = (p.t_tiles + p.blocks - 1) / p.blocks * p.bn_tiles;
     }
     if (i < plan.pieces) {
@@ -1770,15 +1877,20 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
     auto cost = [](uint32_t n, uint32_t chunks) { return (double)n * (chunks < 4 ? 4 : chunks) + 64; };
     deal(n_hidden, cost(p.blocks * p.bn, p.per_split), pairs, load, p.hidden_at);
     deal(n_table, cost(p.blocks * p.bn, p.r_chunks), pairs, load, p.table_at);
-    deal(n_score, cost(kBN, p.w_chunks), pairs, load, p.score_at);
-    err = launch_after(engine_kernel<T, false, kDistill>, 2 * pairs, kThreads, kSmemBytes, s, true,
+    // a score tile takes a tenth longer than its columns x chunks
+    deal(n_score, 1.1 * cost(kBN, p.w_chunks), pairs, load, p.score_at);
+    err = launch_after(engine_kernel<T, false, kDistill>, 2 * pairs, kThreads, kSmemBytes, s,
                        maps, p, w);
     if (err != cudaSuccess) return launched(err);
   }
-  if (dh)
-    err = launch_after(finish_kernel<T>, (rows * width / 4 + 127) / 128, 128, 0, s, true,
-                       static_cast<const float*>(planes), plan.splits,
+  if (dh) {
+    const bool many = n_planes >= 8;
+    const uint64_t columns = kFinishThreads / (many ? 8 : 1) * 4;
+    err = launch_after(many ? finish_kernel<T, 8> : finish_kernel<T, 1>,
+                       (rows * width + columns - 1) / columns, kFinishThreads, 0, s,
+                       static_cast<const float*>(planes), n_planes,
                        static_cast<const RowGrad*>(rg), dh, p.rows, p.width);
+  }
   return launched(err);
 }
 

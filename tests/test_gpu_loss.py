@@ -548,12 +548,14 @@ def test_captured_and_replayed(mf, distill):
         want.append([t.clone() for t in (*out, *_backward(mf, loss, x, out[1], grad, **kw))])
     stream = torch.cuda.Stream()
     loss = mf.DenseLoss(e, rows, stream=stream)
-    x = h.clone()
+    x, source = h.clone(), h.clone()
     torch.cuda.synchronize()
     graphs = []
-    for _ in range(2):
+    for k in range(2):
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g, stream=stream):
+            if k == 0:
+                x.copy_(source)  # the first kernel comes after a copy node
             if distill:
                 out = loss.distill(x, *sets, 2.0)
                 out = (*out, *loss.distill_backward(x, *sets, 2.0, out[1], grad))
@@ -562,7 +564,7 @@ def test_captured_and_replayed(mf, distill):
                 out = (*out, *loss.cross_entropy_backward(x, targets, out[1], grad))
         graphs.append((g, out))
     for k, new in enumerate((h, h2, h)):
-        x.copy_(new)
+        source.copy_(new)
         torch.cuda.synchronize()
         for g, out in graphs:
             g.replay()

@@ -148,7 +148,8 @@ def test_workspace_bytes(lib):
             assert 0 < f(rows, 576, vocab) <= 4096 + rows * 3300
             # two pieces of d, the copy of the rows, FP32 sums of d_hidden
             pieces = 2 * max(128 << 20, 512 * rows)
-            assert rows * 576 * 6 < b(rows, 576, vocab) <= pieces + rows * 576 * 6 + (40 << 20)
+            sums = max(128 << 20, rows * 576 * 4)
+            assert rows * 576 * 6 < b(rows, 576, vocab) <= pieces + sums + rows * 576 * 2 + 4096 + rows * 24
 
 
 def test_class_checks_before_the_call():
