@@ -510,10 +510,9 @@ struct Cursor {
       at = min(end, at + 4 - n);
     }
   }
-  // Drops entries below v and tops the window up.
+  // Drops entries below v.
   __device__ __forceinline__ void skip_to(const Wanted& w, uint32_t v) {
     if constexpr (kDistill) {
-      fill(w);
       while (id[0] < v) next(w);
     }
   }
@@ -769,7 +768,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
     auto release = [&](uint32_t buf) {  // the accumulator has been read
       fence_before();
       __syncwarp();
-      if (lane == 0) bar_arrive_cluster(buf ? leader_acc_empty1 : leader_acc_empty0);
+      if (lane == 0) bar_arrive_cluster_relaxed(buf ? leader_acc_empty1 : leader_acc_empty0);
     };
     auto flush = [&]() {
       if (kForward && cur_m != 0xFFFFFFFFu && row < p.rows)
@@ -811,8 +810,8 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
             tlse2 = st.x * kLog2e;
           }
           cur.start(w, row, v, live);
+          cur.fill(w);
         }
-        cur.skip_to(w, v);
       }
       if (!dead && (*abort_flag || !bar_wait(acc_full(buf), (sub >> 1) & 1u))) {
         *abort_flag = 1u;
@@ -821,6 +820,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
       fence_after();
       const uint32_t acc = tmem + ((quad * 32u) << 16) + buf * kBN;
       if (t.kind == kScore) {
+        cur.skip_to(w, p.v0 + t.n * kBN + half * (kBN / 2));
         const uint32_t c_end = p.cols - min(p.cols, t.n * kBN);  // columns of the tile that exist
 #pragma unroll 1
         for (uint32_t c = half * (kBN / 2); c < (half + 1) * (kBN / 2); c += 64) {
@@ -961,6 +961,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
         continue;
       }
       release(buf);
+      cur.fill(w);  // loads that the next tile waits for, not this one
       t.next(p);
     }
     flush();

@@ -36,6 +36,14 @@ __device__ __forceinline__ void bar_arrive_cluster(uint32_t cluster_bar) {
                : "memory");
 }
 
+// The same without ordering this thread's earlier memory accesses (a release
+// waits until its global stores are performed, about 2,000 clocks): for readers
+// of TMEM only, after tcgen05.wait::ld and fence_before.
+__device__ __forceinline__ void bar_arrive_cluster_relaxed(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
+               : "memory");
+}
+
 // All threads of both CTAs of the pair; both CTAs always reach it (every
 // wait before it is bounded).
 __device__ __forceinline__ void cluster_sync() {
