@@ -309,6 +309,10 @@ __device__ __forceinline__ void mma_pair(uint32_t tmem_d, uint64_t adesc, uint64
       : "memory");
 }
 
+__device__ __forceinline__ void bar_arrive_relaxed_local(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
 // One CTA on its own: MMA, commit, load.
 __device__ __forceinline__ void mma_one(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
                                         uint32_t idesc, uint32_t accumulate) {
@@ -1275,6 +1279,349 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
                  : "memory");
 }
 
+// Gradients for up to 32 rows, in one pass over the table: each CTA takes its
+// range of table rows, 128 at a time.  The tile's rows stay in shared memory for
+// both products that read them, and with so few rows each element of d is
+// carried as a sum of two 16-bit numbers, which costs no memory traffic:
+//   S^T = E H^T     [128, n]      A = table tile (K-major), B = hidden (K-major)
+//   d^T in FP32 -> high and low halves, [128, 32 high | 32 low] in shared memory
+//   d H^T += E^T d  [width, n]    A = table tile (M-major), B = d (N-major)
+//   dE = d^T H      [128, width]  A = d (K-major), B = hidden (N-major)
+// d H^T stays in TMEM over the CTA's tiles and leaves as one FP32 plane per CTA;
+// dE leaves 128 columns at a time.  What bounds it is one read of the table and
+// one write of its gradient.
+constexpr uint32_t kFewGradRows = 32;
+constexpr uint32_t kFewGradChunks = 10;   // widths up to 640
+constexpr uint32_t kFewGradThreads = 320;
+constexpr uint32_t kDBytes = 128 * 128;   // d: 128 table rows x (32 high, 32 low)
+
+struct FewGradParams {
+  uint32_t rows, n;         // n: rows rounded up to 16
+  uint32_t width, w_chunks;
+  uint32_t vocab, range;    // table rows per CTA, a multiple of 32
+  float score_scale;
+  const void* hidden;
+  const float* grad;
+  const float* lse;
+  RowGrad* rg;
+  float* planes;            // [CTA][rows][width], or NULL
+  void* table_out;          // d_embedding, or NULL
+  uint32_t wide_rows;
+};
+
+// Shared-memory descriptor, M or N contiguous, 128-byte swizzle: atoms of 64
+// elements `lbo` bytes apart, groups of 8 K rows 1024 bytes apart.
+__device__ __forceinline__ uint64_t mn128_desc(uint32_t addr, uint32_t lbo) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | (uint64_t)(lbo >> 4) << 16 |
+         (uint64_t)(1024u >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+                 "=r"(r[7])
+               : "r"(taddr));
+  tmem_wait_ld();
+}
+__device__ __forceinline__ void bar_arrive_local(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void epilogue_sync() {  // the eight epilogue warps
+  asm volatile("bar.sync 1, 256;" ::: "memory");
+}
+
+template <typename T, bool kDistill>
+__global__ void __launch_bounds__(kFewGradThreads, 1)
+few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGradParams p, Wanted w) {
+  extern __shared__ unsigned char smem_raw[];
+  // table chunks full, table free, scores full, d full, dE full / empty [2], dH done
+  __shared__ uint64_t bars[kFewGradChunks + 8];
+  __shared__ uint32_t tmem_at, abort_word, loads;
+  __shared__ float s_coef[kFewGradRows], s_z2[kFewGradRows], s_tlse[kFewGradRows];
+  __shared__ uint32_t s_target[kFewGradRows];
+  __shared__ int32_t s_at[kFewGradRows], s_end[kFewGradRows];
+  __shared__ float s_gmax;
+  unsigned char* sm = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t tab = smem_u32(sm);
+  const uint32_t hid_chunk = p.n * 128;
+  const uint32_t hid = tab + p.w_chunks * kChunkBytes;
+  const uint32_t dt = hid + p.w_chunks * hid_chunk;
+  float* s_q = reinterpret_cast<float*>(sm + (dt - tab) + kDBytes);  // distillation: [n][128]
+  const uint32_t bar0 = smem_u32(bars);
+  auto e_full = [&](uint32_t kc) { return bar0 + 8 * kc; };
+  const uint32_t e_free = bar0 + 8 * kFewGradChunks, s_full = e_free + 8, d_full = e_free + 16;
+  auto de_full = [&](uint32_t b) { return e_free + 24 + 8 * b; };
+  auto de_empty = [&](uint32_t b) { return e_free + 40 + 8 * b; };
+  const uint32_t done = e_free + 56;
+  volatile uint32_t* abort_flag = &abort_word;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t v0 = blockIdx.x * p.range;
+  const uint32_t count = min(p.range, p.vocab - v0);
+  const uint32_t tiles = (count + 127) / 128;
+  const uint32_t passes = (p.w_chunks + 1) / 2;  // of 128 columns of dE
+  const uint32_t blocks = (p.w_chunks + 1) / 2;  // of 128 rows of d H^T
+  if (threadIdx.x == 0) {
+    for (uint32_t i = 0; i < kFewGradChunks + 8; ++i)
+      bar_init(bar0 + 8 * i, bar0 + 8 * i == d_full || bar0 + 8 * i == de_empty(0) ||
+                                     bar0 + 8 * i == de_empty(1) ? 8u : 1u);
+    abort_word = 0u;
+    loads = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&tmem_at)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait();
+  pdl_trigger();
+  if (warp == 0) {  // row weights: |weight| / largest, all of it carried by d
+    const float wr = lane < p.rows ? row_weight(w, p.grad, lane, p.vocab) : 0.f;
+    const float a = fabsf(wr);
+    const float g = warp_max(a < INFINITY ? a : 0.f);
+    const float coef = wr != 0.f ? wr / g * Type<T>::kScale : 0.f;
+    s_coef[lane] = coef;
+    s_z2[lane] = lane < p.rows ? p.lse[lane] * kLog2e : 0.f;
+    s_target[lane] = w.targets && lane < p.rows && coef != 0.f ? w.targets[lane] : kInvalid;
+    if (lane == 0) s_gmax = g;
+    if (blockIdx.x == 0 && lane < p.rows) p.rg[lane] = RowGrad{coef, g / Type<T>::kScale};
+    if (kDistill) {
+      s_at[lane] = s_end[lane] = 0;
+      if (coef != 0.f) {
+        s_tlse[lane] = w.stat[lane].x * kLog2e;
+        s_at[lane] = first_entry(w, lane, v0);
+        s_end[lane] = w.offsets[lane + 1];
+      }
+    }
+  }
+  __syncthreads();
+  // hidden rows as 64-wide chunks of 128-byte rows (128-byte swizzle); rows that
+  // take no part are zero
+  for (uint32_t i = threadIdx.x; i < p.w_chunks * p.n * 8; i += kFewGradThreads) {
+    const uint32_t j = i & 7u, r = (i >> 3) % p.n, kc = (i >> 3) / p.n, c = kc * kBK + j * 8;
+    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+    if (s_coef[r] != 0.f && c < p.width)
+      x = ld_v4(static_cast<const T*>(p.hidden) + (uint64_t)r * p.width + c);
+    *reinterpret_cast<uint4*>(sm + (hid - tab) + kc * hid_chunk + r * 128 + ((j ^ (r & 7u)) << 4)) = x;
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_at;
+  // TMEM columns: d H^T [blocks x n], scores [n], dE [2 x 128]
+  const uint32_t acc_h = tmem, acc_s = tmem + blocks * p.n, acc_e = tmem + 256;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      for (uint32_t t = 0; t < tiles && !*abort_flag; ++t) {
+        if (!bar_wait(e_free, (t & 1u) ^ 1u)) {
+          *abort_flag = 1u;
+          break;
+        }
+        for (uint32_t kc = 0; kc < p.w_chunks; ++kc) {
+          bar_expect_tx(e_full(kc), kChunkBytes);
+          tma_load_local(tab + kc * kChunkBytes, &tm_table, (int)(kc * kBK), (int)(v0 + t * 128),
+                         e_full(kc));
+        }
+        loads = t + 1;
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t kIdesc = (1u << 4) | (Type<T>::kFormat << 7) | (Type<T>::kFormat << 10) |
+                                  (8u << 24);  // F32 accumulator, type T, M = 128
+      const uint32_t idesc_s = kIdesc | ((p.n >> 3) << 17);
+      const uint32_t idesc_h = idesc_s | (1u << 15) | (1u << 16);
+      const uint32_t idesc_e = kIdesc | ((128u >> 3) << 17) | (1u << 16);
+      bool ok = true;
+      uint32_t pass = 0;  // dE buffers used so far
+      for (uint32_t t = 0; ok && t < tiles && !*abort_flag; ++t) {
+        for (uint32_t kc = 0; ok && kc < p.w_chunks; ++kc) {
+          ok = bar_wait(e_full(kc), t & 1u);
+          if (!ok) break;
+          const uint64_t a = sw128_desc(tab + kc * kChunkBytes), b = sw128_desc(hid + kc * hid_chunk);
+#pragma unroll
+          for (int k4 = 0; k4 < kBK / 16; ++k4)
+            mma_one(acc_s, a + 2 * k4, b + 2 * k4, idesc_s, (kc | (uint32_t)k4) != 0u);
+        }
+        if (!ok) break;
+        mma_commit_one(s_full);
+        ok = bar_wait(d_full, t & 1u);
+        if (!ok) break;
+        fence_after();
+        if (p.planes) {
+          for (uint32_t b = 0; b < blocks; ++b)
+#pragma unroll 2
+            for (uint32_t k = 0; k < 8; ++k) {  // 16 table rows
+              const uint64_t a = mn128_desc(tab + 2 * b * kChunkBytes + 2048 * k, kChunkBytes);
+              const uint32_t d = dt + 2048 * k;
+              mma_one(acc_h + b * p.n, a, mn128_desc(d, 1024), idesc_h, (t | k) != 0u);
+              mma_one(acc_h + b * p.n, a, mn128_desc(d + 64, 1024), idesc_h, 1u);
+            }
+        }
+        mma_commit_one(e_free);  // the table tile has been read
+        if (p.table_out) {
+          for (uint32_t j = 0; ok && j < passes; ++j, ++pass) {
+            const uint32_t buf = pass & 1u;
+            ok = bar_wait(de_empty(buf), ((pass >> 1) & 1u) ^ 1u);
+            if (!ok) break;
+            fence_after();
+            for (uint32_t k = 0; k < p.n / 16; ++k) {
+              const uint64_t b = mn128_desc(hid + 2 * j * hid_chunk + 2048 * k, hid_chunk);
+              mma_one(acc_e + buf * 128, sw128_desc(dt + 32 * k), b, idesc_e, k != 0u);
+              mma_one(acc_e + buf * 128, sw128_desc(dt + 64 + 32 * k), b, idesc_e, 1u);
+            }
+            mma_commit_one(de_full(buf));
+          }
+        }
+      }
+      if (!ok) *abort_flag = 1u;
+      mma_commit_one(done);
+      bar_wait(done, 0);
+    }
+  } else {
+    const uint32_t quad = warp & 3u, half = (warp - 2) >> 2;
+    const uint32_t lanes = (quad * 32u) << 16;
+    const uint32_t row = quad * 32 + lane;  // of the tile
+    const float c2 = w.inv_t * p.score_scale * kLog2e, t2 = w.inv_t * kLog2e;
+    const float scale = s_gmax / Type<T>::kScale;
+    const float nan = __uint_as_float(0x7FC00000u);
+    bool dead = false;
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      if (!dead && (*abort_flag || !bar_wait(bar, parity))) {
+        *abort_flag = 1u;
+        dead = true;
+      }
+      fence_after();
+    };
+    uint32_t pass = 0;
+    for (uint32_t t = 0; t < tiles; ++t) {
+      const uint32_t v = v0 + t * 128 + row;
+      const bool in = t * 128 + row < count;
+      if (kDistill) {  // the tile's entries, dense
+        epilogue_sync();  // the tile before has been read
+        for (uint32_t i = threadIdx.x - 64; i < p.n * 128; i += 256) s_q[i] = 0.f;
+        epilogue_sync();
+        const uint32_t first = v0 + t * 128, n_in = min(128u, count - t * 128);
+        for (uint32_t r = warp - 2; r < p.rows; r += 8) {
+          int32_t k = s_at[r];
+          const int32_t end = s_end[r];
+          for (;;) {
+            uint32_t id = 0xFFFFFFFFu;
+            if (k + (int32_t)lane < end) id = (uint32_t)w.ids[k + lane];
+            const bool mine = id - first < n_in;  // ascending: entries before `first` are behind k
+            if (mine)
+              s_q[r * 128 + (id - first)] = exp2_approx(fmaf(w.logits[k + lane], t2, -s_tlse[r]));
+            const uint32_t taken = __popc(__ballot_sync(0xFFFFFFFFu, mine));
+            k += (int32_t)taken;
+            if (taken < 32) break;
+          }
+          __syncwarp();
+          if (lane == 0) s_at[r] = k;
+        }
+        epilogue_sync();
+      }
+      wait(s_full, t & 1u);
+      for (uint32_t c = half * (p.n / 2); c < (half + 1) * (p.n / 2); c += 8) {
+        uint32_t r[8];
+        tmem_ld8(acc_s + lanes + c, r);
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          float x[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t n = c + j + e;
+            const float coef = s_coef[n];
+            float d = exp2_approx(fmaf(__uint_as_float(r[j + e]), c2, -s_z2[n]));
+            if (kDistill) d -= s_q[n * 128 + row];
+            else if (s_target[n] == v) d -= 1.f;
+            x[e] = coef == 0.f || !in ? 0.f : (dead ? nan : d * coef);
+          }
+          hi[j / 2] = Type<T>::pack(x[0], x[1]);
+          const T* h = reinterpret_cast<const T*>(&hi[j / 2]);
+          // a high half beyond the type's range stays alone
+          const float l0 = x[0] - Type<T>::to(h[0]), l1 = x[1] - Type<T>::to(h[1]);
+          lo[j / 2] = Type<T>::pack(fabsf(l0) < INFINITY ? l0 : 0.f, fabsf(l1) < INFINITY ? l1 : 0.f);
+        }
+        unsigned char* at = sm + (dt - tab) + row * 128;
+        *reinterpret_cast<uint4*>(at + (((c / 8) ^ (row & 7u)) << 4)) =
+            make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(at + (((4 + c / 8) ^ (row & 7u)) << 4)) =
+            make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive_local(d_full);
+      for (uint32_t j = 0; p.table_out && j < passes; ++j, ++pass) {
+        const uint32_t buf = pass & 1u;
+        wait(de_full(buf), (pass >> 1) & 1u);
+        uint32_t r[2][32];
+        tmem_ld32(acc_e + lanes + buf * 128 + half * 64, r[0]);
+        tmem_ld32(acc_e + lanes + buf * 128 + half * 64 + 32, r[1]);
+        tmem_wait_ld();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive_relaxed_local(de_empty(buf));
+        if (!in) continue;
+#pragma unroll
+        for (uint32_t q = 0; q < 2; ++q) {
+          const uint32_t col = j * 128 + half * 64 + 32 * q;
+          if (col >= p.width) continue;
+          const uint32_t groups = min(4u, (p.width - col) / 8);
+          T* out = static_cast<T*>(p.table_out) + (uint64_t)v * p.width + col;
+          const float by = dead ? nan : scale;
+          uint32_t x[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            x[i] = Type<T>::pack(__uint_as_float(r[q][2 * i]) * by,
+                                 __uint_as_float(r[q][2 * i + 1]) * by);
+          if (p.wide_rows) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i += 2)
+              if (i < groups) store_v8(out + 8 * i, x + 4 * i);
+          } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i)
+              if (i < groups)
+                *reinterpret_cast<uint4*>(out + 8 * i) =
+                    make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+          }
+        }
+      }
+    }
+    if (p.planes) {
+      wait(done, 0);
+      float* out = p.planes + (uint64_t)blockIdx.x * p.rows * p.width;
+      for (uint32_t b = 0; b < blocks; ++b) {
+        const uint32_t c = b * 128 + row;  // column of d_hidden
+        for (uint32_t n = half * (p.n / 2); n < (half + 1) * (p.n / 2); n += 8) {
+          uint32_t r[8];
+          tmem_ld8(acc_h + lanes + b * p.n + n, r);
+#pragma unroll
+          for (uint32_t j = 0; j < 8; ++j)
+            if (n + j < p.rows && c < p.width)
+              out[(uint64_t)(n + j) * p.width + c] = dead ? nan : __uint_as_float(r[j]);
+        }
+      }
+    }
+    fence_before();
+  }
+  __syncthreads();
+  if (abort_word != 0u && threadIdx.x == 0 && loads > 0u)  // copies in flight, bounded
+    for (uint32_t kc = 0; kc < p.w_chunks; ++kc) bar_wait(e_full(kc), (loads - 1u) & 1u);
+  __syncthreads();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(kTmemCols)
+                 : "memory");
+}
+
 // One block per row: the CTAs' sums, the wanted scores, the teacher's
 // distribution.
 constexpr uint32_t kJoinThreads = 256;
@@ -1455,7 +1802,10 @@ struct BackwardPlan {
     gmax = round_up(rg + rows * sizeof(RowGrad), 256);
     scaled = gmax + 256;
     planes = round_up(scaled + rows * width * 2, 256);
-    piece[0] = round_up(planes + sets * set, 256);
+    uint64_t sums = sets * set;
+    const uint64_t few = 2 * kMaxPairs * rows * width * 4;  // few_rows_grad_kernel's planes
+    if (rows <= kFewGradRows && sums < few) sums = few;
+    piece[0] = round_up(planes + sums, 256);
     const uint64_t one = round_up(rows * cols * 2, 256);
     piece[1] = piece[0] + (pieces > 1 ? one : 0);
     bytes = piece[1] + one;
@@ -1679,7 +2029,11 @@ cudaError_t device_sms(uint32_t* sms) {
   if (c == 0) {
     e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
     for (const void* k : {(const void*)few_rows_kernel<__half>,
-                          (const void*)few_rows_kernel<__nv_bfloat16>})
+                          (const void*)few_rows_kernel<__nv_bfloat16>,
+                          (const void*)few_rows_grad_kernel<__half, false>,
+                          (const void*)few_rows_grad_kernel<__half, true>,
+                          (const void*)few_rows_grad_kernel<__nv_bfloat16, false>,
+                          (const void*)few_rows_grad_kernel<__nv_bfloat16, true>})
       if (e == cudaSuccess)
         e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFewSmem);
     if (e != cudaSuccess) return e;
@@ -1688,6 +2042,22 @@ cudaError_t device_sms(uint32_t* sms) {
   *sms = c;
   return cudaSuccess;
 }
+
+// The same for the gradients; smem 0: the kernel does not take the call.
+struct FewGradPlan {
+  uint32_t n, range, ctas;
+  uint64_t smem = 0;
+  FewGradPlan(uint64_t rows, uint64_t width, uint64_t vocab, uint64_t sms, bool distill) {
+    const uint64_t chunks = (width + kBK - 1) / kBK;
+    if (rows > kFewGradRows || chunks > kFewGradChunks) return;
+    n = (uint32_t)round_up(rows, 16);
+    range = (uint32_t)round_up((vocab + sms - 1) / sms, 32);
+    ctas = (uint32_t)((vocab + range - 1) / range);
+    const uint64_t bytes =
+        chunks * (kChunkBytes + n * 128) + kDBytes + (distill ? n * 512 : 0) + 1024;
+    if (bytes <= kFewSmem) smem = bytes;
+  }
+};
 
 template <typename T>
 mf_status forward_few(const FewPlan& few, Wanted w, const T* hidden, const T* table, uint64_t entries,
@@ -1776,6 +2146,16 @@ mf_status forward(Span hidden, Span embedding, Span targets, Span ids, Span logi
   return launched(e);
 }
 
+template <typename T>
+cudaError_t finish_launch(const float* planes, uint32_t n_planes, const RowGrad* rg, T* out,
+                          uint64_t rows, uint64_t width, cudaStream_t s) {
+  const bool many = n_planes >= 8;
+  const uint64_t columns = kFinishThreads / (many ? 8 : 1) * 4;
+  return launch_after(many ? finish_kernel<T, 8> : finish_kernel<T, 1>,
+                      (rows * width + columns - 1) / columns, kFinishThreads, 0, s, planes, n_planes,
+                      rg, out, (uint32_t)rows, (uint32_t)width);
+}
+
 template <typename T, bool kDistill>
 mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span logits,
                    float temperature, Span lse, Span grad, Span d_hidden, Span d_embedding,
@@ -1794,8 +2174,9 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
   const BackwardPlan plan(rows, width, vocab);
   char* ws = static_cast<char*>(const_cast<void*>(workspace.p));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  uint32_t pairs = 0;
-  cudaError_t err = resident_pairs<T, false, kDistill>(&pairs);
+  uint32_t pairs = 0, sms = 0;
+  cudaError_t err = device_sms(&sms);
+  if (err == cudaSuccess) err = resident_pairs<T, false, kDistill>(&pairs);
   if (err != cudaSuccess) return fail(MF_CUDA_RUNTIME_FAILURE, (uint32_t)err);
   RowGrad* rg = reinterpret_cast<RowGrad*>(ws + plan.rg);
   float* gmax = reinterpret_cast<float*>(ws + plan.gmax);
@@ -1803,12 +2184,6 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
   float* planes = reinterpret_cast<float*>(ws + plan.planes);
   T* dh = static_cast<T*>(const_cast<void*>(d_hidden.p));
   T* de = static_cast<T*>(const_cast<void*>(d_embedding.p));
-  Maps maps = {};
-  if (!make_map<T>(&maps.hidden, hidden.p, rows, width, width, kBK, kBM) ||
-      !make_map<T>(&maps.table, embedding.p, vocab, width, width, kBK, kBN / 2) ||
-      !make_map<T>(&maps.table_n, embedding.p, vocab, width, width, 32, kBK) ||
-      !make_map<T>(&maps.scaled_n, scaled, rows, width, width, 32, kBK))
-    return fail(MF_CUDA_RUNTIME_FAILURE);
   Wanted w{};
   w.inv_t = kDistill ? 1.f / temperature : 1.f;
   if (kDistill) {
@@ -1821,6 +2196,37 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
   } else {
     w.targets = static_cast<const uint32_t*>(targets.p);
   }
+  const FewGradPlan few(rows, width, vocab, sms, kDistill);
+  if (few.smem > 0) {
+    CUtensorMap tm_t;
+    if (!make_map<T>(&tm_t, embedding.p, vocab, width, width, kBK, kBM))
+      return fail(MF_CUDA_RUNTIME_FAILURE);
+    FewGradParams f = {};
+    f.rows = (uint32_t)rows;
+    f.n = few.n;
+    f.width = (uint32_t)width;
+    f.w_chunks = (uint32_t)((width + kBK - 1) / kBK);
+    f.vocab = (uint32_t)vocab;
+    f.range = few.range;
+    f.score_scale = 1.f + (float)width * kLostPerProduct;
+    f.hidden = hidden.p;
+    f.grad = static_cast<const float*>(grad.p);
+    f.lse = static_cast<const float*>(lse.p);
+    f.rg = rg;
+    f.planes = dh ? planes : nullptr;
+    f.table_out = de;
+    f.wide_rows = width % 16 == 0 && (uintptr_t)de % 32 == 0;
+    err = launch_after(few_rows_grad_kernel<T, kDistill>, few.ctas, kFewGradThreads, few.smem, s,
+                       tm_t, f, w);
+    if (err == cudaSuccess && dh) err = finish_launch(planes, few.ctas, rg, dh, rows, width, s);
+    return launched(err);
+  }
+  Maps maps = {};
+  if (!make_map<T>(&maps.hidden, hidden.p, rows, width, width, kBK, kBM) ||
+      !make_map<T>(&maps.table, embedding.p, vocab, width, width, kBK, kBN / 2) ||
+      !make_map<T>(&maps.table_n, embedding.p, vocab, width, width, 32, kBK) ||
+      !make_map<T>(&maps.scaled_n, scaled, rows, width, width, 32, kBK))
+    return fail(MF_CUDA_RUNTIME_FAILURE);
   err = launch_after(setup_kernel<T>, rows < 32 * 148 ? (rows + 31) / 32 : 148, kSetupThreads, 0, s, w,
                      static_cast<const float*>(grad.p), static_cast<const T*>(hidden.p), scaled,
                      rg, gmax, (uint32_t)rows, (uint32_t)width, (uint32_t)vocab);
@@ -1884,14 +2290,7 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
                        maps, p, w);
     if (err != cudaSuccess) return launched(err);
   }
-  if (dh) {
-    const bool many = n_planes >= 8;
-    const uint64_t columns = kFinishThreads / (many ? 8 : 1) * 4;
-    err = launch_after(many ? finish_kernel<T, 8> : finish_kernel<T, 1>,
-                       (rows * width + columns - 1) / columns, kFinishThreads, 0, s,
-                       static_cast<const float*>(planes), n_planes,
-                       static_cast<const RowGrad*>(rg), dh, p.rows, p.width);
-  }
+  if (dh) err = finish_launch(planes, n_planes, rg, dh, rows, width, s);
   return launched(err);
 }
 

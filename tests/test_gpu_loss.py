@@ -147,7 +147,10 @@ class Reference:
         # holds d / (largest weight) times 2^15
         d_off = (s_off + self.lse_off)[:, None] * p * w.abs()[:, None] \
             + q * w.abs()[:, None] * 2.0 ** -19
-        tiny = biggest * 2.0 ** -40 if kind == "f16" else biggest * 2.0 ** -130
+        # an exponential below 2^-126, FP32's smallest normal number, may come out
+        # as 0 (p <= 2^-126 is then off by all of itself): for bf16, whose range is
+        # FP32's, that is the floor of d; fp16's own 2^-25 2^-15 lies far above it
+        tiny = biggest * 2.0 ** -40 if kind == "f16" else biggest * 2.0 ** -126
         d_off = d_off * (1 + u) + u * d.abs() + tiny * (w != 0)[:, None]
         # a hidden row carries its weight's power of two: exact but below fp16's range
         h_off = (2.0 ** -25 if kind == "f16" else 2.0 ** -133) * (
@@ -209,7 +212,8 @@ def _check(mf, h, e, kind, grad, targets=None, sets=None, temperature=1.0):
 # rows, vocabulary, width: single values, tile edges on both sides, odd ones
 SHAPES = [(1, 1, 8), (1, 17, 64), (2, 300, 72), (3, 8, 576), (63, 127, 64), (64, 128, 128),
           (65, 129, 136), (127, 255, 576), (128, 256, 192), (129, 257, 200), (255, 511, 328),
-          (256, 512, 576), (257, 513, 584), (300, 4099, 64), (520, 1000, 1024), (1, 5000, 2048)]
+          (256, 512, 576), (257, 513, 584), (300, 4099, 64), (520, 1000, 1024), (1, 5000, 2048),
+          (16, 95, 8), (17, 4800, 640), (32, 20_011, 576), (31, 45_000, 200), (33, 600, 576)]
 
 
 @pytest.mark.parametrize("kind", TYPES)
@@ -225,7 +229,7 @@ def test_cross_entropy(mf, rows, vocab, width, kind):
 
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("most,temperature", [(1, 1.0), (40, 2.0), (700, 0.7)])
-@pytest.mark.parametrize("rows,vocab,width", [s for s in SHAPES if s[1] <= 1000])
+@pytest.mark.parametrize("rows,vocab,width", [s for s in SHAPES if s[1] <= 1000 or s[0] in (17, 32)])
 def test_distill(mf, rows, vocab, width, most, temperature, kind):
     import torch
 
@@ -261,57 +265,61 @@ def test_wide_and_long(mf, kind):
 
 
 @pytest.mark.parametrize("kind", TYPES)
-def test_confident_rows(mf, kind):
+@pytest.mark.parametrize("rows", (100, 25))
+def test_confident_rows(mf, kind, rows):
     """Scores far apart: p is 0 or 1 to the last bit in many places, and lse is
     far from 0 on both sides."""
     import torch
 
-    h, e, gen = _problem(11, 100, 700, 128, kind, 60.0)
-    targets = _targets(gen, 100, 700, 0.1)
-    targets[:40] = (h.float() @ e.float().T).argmax(1)[:40].int()  # some are right
-    _check(mf, h, e, kind, torch.ones(100, device="cuda"), targets=targets)
+    h, e, gen = _problem(11, rows, 700, 128, kind, 60.0)
+    targets = _targets(gen, rows, 700, 0.1)
+    right = (h.float() @ e.float().T).argmax(1).int()
+    targets[:rows // 2] = right[:rows // 2]  # some are right
+    _check(mf, h, e, kind, torch.ones(rows, device="cuda"), targets=targets)
 
 
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("scale", (1.0, 1e-6, 4096.0))
-def test_weights_over_a_wide_range(mf, kind, scale):
+@pytest.mark.parametrize("rows", (200, 30))
+def test_weights_over_a_wide_range(mf, kind, scale, rows):
     """Weights from 1 down to 2^-12, zeros and negative ones among them."""
     import torch
 
-    h, e, gen = _problem(12, 200, 900, 96, kind, 2.0)
-    grad = scale * torch.exp2(-12 * torch.rand(200, generator=gen, device="cuda"))
+    h, e, gen = _problem(12, rows, 900, 96, kind, 2.0)
+    grad = scale * torch.exp2(-12 * torch.rand(rows, generator=gen, device="cuda"))
     grad[::7] = 0
     grad[::5] *= -1
-    ref, _, _, _, dh, _ = _check(mf, h, e, kind, grad, targets=_targets(gen, 200, 900, 0.1))
+    ref, _, _, _, dh, _ = _check(mf, h, e, kind, grad, targets=_targets(gen, rows, 900, 0.1))
     assert not bool(dh[::7].any())
 
 
-def _poisoned(kind):
+def _poisoned(kind, rows):
     """Rows that do not take part hold NaN and infinities."""
-    h, e, gen = _problem(13, 150, 500, 64, kind, 2.0)
+    h, e, gen = _problem(13, rows, 500, 64, kind, 2.0)
     clean = h.clone()
     h[3:9] = math.nan
-    h[20:140:10] = math.inf
+    h[20::10] = math.inf
     return h, clean, e, gen
 
 
 @pytest.mark.parametrize("kind", TYPES)
-def test_masked_rows_hold_anything(mf, kind):
+@pytest.mark.parametrize("rows", (150, 28))
+def test_masked_rows_hold_anything(mf, kind, rows):
     import torch
 
-    h, clean, e, gen = _poisoned(kind)
+    h, clean, e, gen = _poisoned(kind, rows)
     bad = ~torch.isfinite(h).all(1)
-    targets = _targets(gen, 150, 500, 0.0)
+    targets = _targets(gen, rows, 500, 0.0)
     targets[bad] = -1
     targets[torch.nonzero(bad)[0, 0]] = 700     # invalid
-    grad = torch.ones(150, device="cuda")
+    grad = torch.ones(rows, device="cuda")
     grad[3:9] = math.nan                        # of masked rows: not read
     live = torch.where(bad, torch.zeros_like(grad), grad)
     targets[4], grad[4] = 17, 0.0               # a target, but no weight
     ref = Reference(clean, e, kind, targets, None, 1.0, live)
     loss, (losses, lse) = _forward(mf, h, e, targets)
     assert math.isnan(float(losses[3])) and math.isnan(float(losses[4]))
-    rest = torch.arange(150, device="cuda") > 4
+    rest = torch.arange(rows, device="cuda") > 4
     _near(losses[rest], ref.losses[rest], ref.losses_off[rest], "losses")
     dh, de = _backward(mf, loss, h, lse, grad, targets)
     assert not bool(dh[bad].any())
@@ -320,51 +328,54 @@ def test_masked_rows_hold_anything(mf, kind):
 
 
 @pytest.mark.parametrize("kind", TYPES)
-def test_non_finite_rows_stay_their_own(mf, kind):
+@pytest.mark.parametrize("rows,bad", [(140, 77), (19, 8)])
+def test_non_finite_rows_stay_their_own(mf, kind, rows, bad):
     """A NaN hidden row that takes part: its loss and gradient are NaN, the
     other rows' are not."""
     import torch
 
-    h, e, gen = _problem(14, 140, 300, 64, kind, 2.0)
-    targets = _targets(gen, 140, 300, 0.0)
-    grad = torch.ones(140, device="cuda")
+    h, e, gen = _problem(14, rows, 300, 64, kind, 2.0)
+    targets = _targets(gen, rows, 300, 0.0)
+    grad = torch.ones(rows, device="cuda")
     ref = Reference(h, e, kind, targets, None, 1.0, grad)
-    h[77, 5] = math.nan
+    h[bad, 5] = math.nan
     loss, (losses, lse) = _forward(mf, h, e, targets)
-    others = torch.arange(140, device="cuda") != 77
-    assert math.isnan(float(losses[77])) and math.isnan(float(lse[77]))
+    others = torch.arange(rows, device="cuda") != bad
+    assert math.isnan(float(losses[bad])) and math.isnan(float(lse[bad]))
     _near(losses[others], ref.losses[others], ref.losses_off[others], "losses")
     dh, de = _backward(mf, loss, h, lse, grad, targets)
-    assert bool(torch.isnan(dh[77]).all()) and bool(torch.isnan(de).all())
+    assert bool(torch.isnan(dh[bad]).all()) and bool(torch.isnan(de).all())
     _near(dh[others], ref.d_hidden[others], ref.dh_off[others], "d_hidden")
 
 
-def test_infinite_weight_spoils_its_own_row(mf):
+@pytest.mark.parametrize("rows", (40, 20))
+def test_infinite_weight_spoils_its_own_row(mf, rows):
     import torch
 
-    h, e, gen = _problem(15, 40, 300, 64, "f16", 2.0)
-    targets = _targets(gen, 40, 300, 0.0)
-    grad = torch.ones(40, device="cuda")
+    h, e, gen = _problem(15, rows, 300, 64, "f16", 2.0)
+    targets = _targets(gen, rows, 300, 0.0)
+    grad = torch.ones(rows, device="cuda")
     ref = Reference(h, e, "f16", targets, None, 1.0, grad)
     grad[9] = math.inf
     loss, (_, lse) = _forward(mf, h, e, targets)
     dh, de = _backward(mf, loss, h, lse, grad, targets)
-    others = torch.arange(40, device="cuda") != 9
+    others = torch.arange(rows, device="cuda") != 9
     assert not bool(torch.isfinite(dh[9]).any()) and not bool(torch.isfinite(de).all())
     _near(dh[others], ref.d_hidden[others], ref.dh_off[others], "d_hidden")
 
 
 @pytest.mark.parametrize("kind", TYPES)
-def test_nothing_takes_part(mf, kind):
+@pytest.mark.parametrize("rows", (70, 7))
+def test_nothing_takes_part(mf, kind, rows):
     """Every row ignored, or every weight 0: losses and gradients are 0."""
     import torch
 
-    h, e, gen = _problem(16, 70, 300, 64, kind)
-    none = torch.full((70,), -1, dtype=torch.int32, device="cuda")
+    h, e, gen = _problem(16, rows, 300, 64, kind)
+    none = torch.full((rows,), -1, dtype=torch.int32, device="cuda")
     loss, (losses, lse) = _forward(mf, h, e, none)
     assert not bool(losses.any())
-    for targets, grad in ((none, torch.ones(70, device="cuda")),
-                          (_targets(gen, 70, 300, 0.0), torch.zeros(70, device="cuda"))):
+    for targets, grad in ((none, torch.ones(rows, device="cuda")),
+                          (_targets(gen, rows, 300, 0.0), torch.zeros(rows, device="cuda"))):
         dh, de = _backward(mf, loss, h, lse, grad, targets)
         assert not bool(dh.any()) and not bool(de.any())
 
@@ -463,12 +474,13 @@ def test_gradient_against_differences(mf, distill):
 
 
 @pytest.mark.parametrize("kind", TYPES)
-def test_one_gradient_alone(mf, kind):
+@pytest.mark.parametrize("rows", (130, 21))
+def test_one_gradient_alone(mf, kind, rows):
     import torch
 
-    h, e, gen = _problem(21, 130, 700, 72, kind)
-    targets = _targets(gen, 130, 700, 0.1)
-    grad = torch.rand(130, generator=gen, device="cuda")
+    h, e, gen = _problem(21, rows, 700, 72, kind)
+    targets = _targets(gen, rows, 700, 0.1)
+    grad = torch.rand(rows, generator=gen, device="cuda")
     loss, (_, lse) = _forward(mf, h, e, targets)
     dh, de = _backward(mf, loss, h, lse, grad, targets)
     a, none = _backward(mf, loss, h, lse, grad, targets, embedding_grad=False)
@@ -478,13 +490,14 @@ def test_one_gradient_alone(mf, kind):
 
 
 @pytest.mark.parametrize("kind", TYPES)
-def test_same_bits_every_time_and_nothing_kept(mf, kind):
+@pytest.mark.parametrize("rows", (600, 32))
+def test_same_bits_every_time_and_nothing_kept(mf, kind, rows):
     """Two runs give the same bits, whatever the workspace held before."""
     import torch
 
-    h, e, gen = _problem(22, 600, 5000, 96, kind)
-    sets = _sets(gen, 600, 5000, 60)
-    grad = torch.rand(600, generator=gen, device="cuda")
+    h, e, gen = _problem(22, rows, 5000, 96, kind)
+    sets = _sets(gen, rows, 5000, 60)
+    grad = torch.rand(rows, generator=gen, device="cuda")
     loss, first = _forward(mf, h, e, None, sets, 2.0)
     g1 = _backward(mf, loss, h, first[1], grad, None, sets, 2.0)
     loss.workspace.fill_(0xFF)
