@@ -1378,6 +1378,16 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
   }
   pdl_wait();
   pdl_trigger();
+  __syncthreads();  // barriers initialised
+  auto load_tile = [&](uint32_t t) {
+    for (uint32_t kc = 0; kc < p.w_chunks; ++kc) {
+      bar_expect_tx(e_full(kc), kChunkBytes);
+      tma_load_local(tab + kc * kChunkBytes, &tm_table, (int)(kc * kBK), (int)(v0 + t * 128),
+                     e_full(kc));
+    }
+    loads = t + 1;
+  };
+  if (threadIdx.x == 32) load_tile(0);  // under the set-up
   if (warp == 0) {  // row weights: |weight| / largest, all of it carried by d
     const float wr = lane < p.rows ? row_weight(w, p.grad, lane, p.vocab) : 0.f;
     const float a = fabsf(wr);
@@ -1417,17 +1427,12 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
 
   if (warp == 0) {
     if (lane == 0) {
-      for (uint32_t t = 0; t < tiles && !*abort_flag; ++t) {
+      for (uint32_t t = 1; t < tiles && !*abort_flag; ++t) {
         if (!bar_wait(e_free, (t & 1u) ^ 1u)) {
           *abort_flag = 1u;
           break;
         }
-        for (uint32_t kc = 0; kc < p.w_chunks; ++kc) {
-          bar_expect_tx(e_full(kc), kChunkBytes);
-          tma_load_local(tab + kc * kChunkBytes, &tm_table, (int)(kc * kBK), (int)(v0 + t * 128),
-                         e_full(kc));
-        }
-        loads = t + 1;
+        load_tile(t);
       }
     }
   } else if (warp == 1) {
@@ -1453,6 +1458,25 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
         ok = bar_wait(d_full, t & 1u);
         if (!ok) break;
         fence_after();
+        // two passes of dE first: the epilogue drains them under d H^T
+        uint32_t j = 0;
+        auto table_pass = [&]() {
+          const uint32_t buf = pass & 1u;
+          ok = bar_wait(de_empty(buf), ((pass >> 1) & 1u) ^ 1u);
+          if (!ok) return;
+          fence_after();
+          for (uint32_t k = 0; k < p.n / 16; ++k) {
+            const uint64_t b = mn128_desc(hid + 2 * j * hid_chunk + 2048 * k, hid_chunk);
+            mma_one(acc_e + buf * 128, sw128_desc(dt + 32 * k), b, idesc_e, k != 0u);
+            mma_one(acc_e + buf * 128, sw128_desc(dt + 64 + 32 * k), b, idesc_e, 1u);
+          }
+          mma_commit_one(de_full(buf));
+          ++j;
+          ++pass;
+        };
+        const uint32_t n_pass = p.table_out ? passes : 0;
+        while (ok && j < 2 && j < n_pass) table_pass();
+        if (!ok) break;
         if (p.planes) {
           for (uint32_t b = 0; b < blocks; ++b)
 #pragma unroll 2
@@ -1464,20 +1488,7 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
             }
         }
         mma_commit_one(e_free);  // the table tile has been read
-        if (p.table_out) {
-          for (uint32_t j = 0; ok && j < passes; ++j, ++pass) {
-            const uint32_t buf = pass & 1u;
-            ok = bar_wait(de_empty(buf), ((pass >> 1) & 1u) ^ 1u);
-            if (!ok) break;
-            fence_after();
-            for (uint32_t k = 0; k < p.n / 16; ++k) {
-              const uint64_t b = mn128_desc(hid + 2 * j * hid_chunk + 2048 * k, hid_chunk);
-              mma_one(acc_e + buf * 128, sw128_desc(dt + 32 * k), b, idesc_e, k != 0u);
-              mma_one(acc_e + buf * 128, sw128_desc(dt + 64 + 32 * k), b, idesc_e, 1u);
-            }
-            mma_commit_one(de_full(buf));
-          }
-        }
+        while (ok && j < n_pass) table_pass();
       }
       if (!ok) *abort_flag = 1u;
       mma_commit_one(done);
@@ -1642,10 +1653,35 @@ few_rows_join_kernel(Wanted w, const T* hidden, const T* table, uint32_t width, 
     st = teacher_stat(w, r, entries, vocab);
     if (!stat_empty(st) && !stat_invalid(st)) {
       const int32_t end = w.offsets[r + 1];
-      for (int32_t k = w.offsets[r] + (int32_t)warp; k < end; k += kJoinThreads / 32) {
-        const float q = expf(w.logits[k] * w.inv_t - st.x);
-        const float s = warp_score(row, table + (uint64_t)w.ids[k] * width, width);
-        if (q > 0.f) dot = fmaf(q, s * w.inv_t, dot);
+      constexpr int32_t kWarps = kJoinThreads / 32;
+      for (int32_t k = w.offsets[r] + (int32_t)warp; k < end; k += 4 * kWarps) {
+        const T* at[4];
+        float q[4], s[4] = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int32_t i = k + j * kWarps < end ? k + j * kWarps : k;
+          q[j] = k + j * kWarps < end ? expf(w.logits[i] * w.inv_t - st.x) : 0.f;
+          at[j] = table + (uint64_t)w.ids[i] * width;
+        }
+        for (uint32_t c = lane * 8; c < width; c += 256) {  // four rows in flight
+          const uint4 x = ld_v4(row + c);
+          uint4 y[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[j] = ld_v4(at[j] + c);
+          const T* xs = reinterpret_cast<const T*>(&x);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const T* ys = reinterpret_cast<const T*>(&y[j]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[j] = fmaf(Type<T>::to(xs[e]), Type<T>::to(ys[e]), s[j]);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int o = 16; o; o >>= 1) s[j] += __shfl_xor_sync(0xFFFFFFFFu, s[j], o);
+          if (q[j] > 0.f) dot = fmaf(q[j], s[j] * w.inv_t, dot);
+        }
       }
     }
   }
