@@ -1821,8 +1821,12 @@ struct BackwardPlan {
                                                               ((rows + kBK - 1) / kBK));
     uint64_t most = total / kMaxPairs / 2;
     if (most < 4) most = 4;
-    // two 256-row blocks a tile cost no accumulator to drain into: for long K
-    blocks = rows >= 32 * kBK && most >= 64 ? 2 : 1;
+    // Two 256-row blocks a tile read B once (backward, us, one block and two:
+    // 2,000 x 49,152 x 576 350 and 322, 4,096 rows 717 and 608, 1,001 x 32,003 x
+    // 328 100 and 91, 512 x 49,152 x 576 109 and 104), but leave no accumulator
+    // to drain into, which short K does not repay, and waste half a tile of an
+    // odd few (600 x 20,000 x 1,024, three row tiles: 95 and 114)
+    blocks = rows >= 8 * kBK && most >= 32 && (m_tiles % 2 == 0 || m_tiles >= 8) ? 2 : 1;
     if (blocks == 2) most /= 2;
     splits = (uint32_t)((chunks + most - 1) / most);
     per_split = (uint32_t)((chunks + splits - 1) / splits);

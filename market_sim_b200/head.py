@@ -678,7 +678,10 @@ class DenseLoss:
         if backward:
             nbytes = max(nbytes, dense_loss_backward_workspace_bytes(*sizes))
         self._backward, self._torch = backward, torch
-        self._device = embedding.device
+        self._i32, self._f32, self._kind = torch.int32, torch.float32, embedding.dtype
+        self._device, self._index = embedding.device, embedding.get_device()
+        self._table_shape = (self.vocab, self.hidden_size)
+        self._table_bytes, self._workspace_bytes = self.vocab * self.hidden_size * 2, nbytes
         kind = kinds[embedding.dtype]
         self._functions = {n: getattr(lib, f"mf_dense_{n}_{kind}")
                            for n in ("xent", "xent_backward", "distill", "distill_backward")}
@@ -694,67 +697,67 @@ class DenseLoss:
         return ValueError(f"{name}: a contiguous {dtype} tensor of shape {shape} on {self._device} "
                           f"is wanted, not {t.dtype} {tuple(t.shape)} on {t.device}")
 
-    def _in(self, args, name, t, dtype, shape):
+    def _in(self, args, name, t, dtype, shape, nbytes):
         """Checks an input and appends its address and bytes."""
-        if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() \
-                or t.device != self._device:
+        if t.dtype is not dtype or t.shape != shape or t.get_device() != self._index \
+                or not t.is_contiguous():
             raise self._wrong(name, t, dtype, shape)
-        args += (t.data_ptr(), t.numel() * t.element_size())
+        args += (t.data_ptr(), nbytes)
 
-    def _out(self, args, name, t, dtype, shape):
+    def _out(self, args, name, t, dtype, shape, nbytes):
         """The same for an output, which is made if it is not given: from the
         memory of the stream that writes it."""
-        torch = self._torch
         if t is None:
+            torch = self._torch
             with torch.cuda.device(self._device), torch.cuda.stream(self._on()):
                 t = torch.empty(shape, dtype=dtype, device=self._device)
-        self._in(args, name, t, dtype, shape)
+        self._in(args, name, t, dtype, shape, nbytes)
         return t
 
     def _begin(self, hidden):
+        """Rows, the shape and bytes of a float or int32 per row, and the call's
+        arguments so far."""
         rows = hidden.shape[0]
         if rows > self.max_rows:
             raise ValueError(f"batch of {rows} rows exceeds max_rows={self.max_rows}")
-        args, table = [], self.embedding
-        self._in(args, "hidden", hidden, table.dtype, (rows, self.hidden_size))
-        self._in(args, "embedding", table, table.dtype, (self.vocab, self.hidden_size))
-        return rows, args
+        args, width, kind = [], self.hidden_size, self._kind
+        self._in(args, "hidden", hidden, kind, (rows, width), rows * width * 2)
+        self._in(args, "embedding", self.embedding, kind, self._table_shape, self._table_bytes)
+        return rows, (rows,), rows * 4, args
 
     def _sets(self, args, rows, offsets, ids, teacher_logits, temperature):
-        torch, entries = self._torch, (ids.numel(),)
-        self._in(args, "offsets", offsets, torch.int32, (rows + 1,))
-        self._in(args, "ids", ids, torch.int32, entries)
-        self._in(args, "teacher_logits", teacher_logits, torch.float32, entries)
+        n = ids.numel()
+        self._in(args, "offsets", offsets, self._i32, (rows + 1,), rows * 4 + 4)
+        self._in(args, "ids", ids, self._i32, (n,), n * 4)
+        self._in(args, "teacher_logits", teacher_logits, self._f32, (n,), n * 4)
         args.append(float(temperature))
 
     def _call(self, name, args, rows):
-        torch = self._torch
-        if self._device.type == "cuda" and torch.cuda.current_device() != self._device.index:
-            with torch.cuda.device(self._device):
-                st = self._launch(name, args, rows)
+        if self._index >= 0 and self._torch.cuda.current_device() != self._index:
+            with self._torch.cuda.device(self._device):
+                code = self._launch(name, args, rows)
         else:
-            st = self._launch(name, args, rows)
-        if st.code:
-            raise RuntimeError(f"mf_dense_{name} failed: {_status(st)}")
+            code = self._launch(name, args, rows)
+        if code.code:
+            raise RuntimeError(f"mf_dense_{name} failed: {_status(code)}")
 
     def _launch(self, name, args, rows):
-        ws = self.workspace
         stream = self.stream
         if stream is None:
             stream = self._torch.cuda.current_stream(self._device)
-        return self._functions[name](*args, ws.data_ptr(), ws.numel(), rows, self.hidden_size,
-                                     self.vocab, _stream_handle(stream))
+        ws = self.workspace
+        return self._functions[name](*args, ws.data_ptr(), self._workspace_bytes, rows,
+                                     self.hidden_size, self.vocab, _stream_handle(stream))
 
-    def _losses(self, args, rows, losses, lse):
-        f32 = self._torch.float32
-        losses = self._out(args, "losses", losses, f32, (rows,))
-        return losses, self._out(args, "lse", lse, f32, (rows,))
+    def _losses(self, args, shape, nbytes, losses, lse):
+        losses = self._out(args, "losses", losses, self._f32, shape, nbytes)
+        return losses, self._out(args, "lse", lse, self._f32, shape, nbytes)
 
     def cross_entropy(self, hidden, targets, losses=None, lse=None):
         """targets int32 [rows]; -1 (``INVALID_TOKEN_ID``) ignores a row."""
-        rows, args = self._begin(hidden)
-        self._in(args, "targets", targets, self._torch.int32, (rows,))
-        out = self._losses(args, rows, losses, lse)
+        rows, shape, nbytes, args = self._begin(hidden)
+        self._in(args, "targets", targets, self._i32, shape, nbytes)
+        out = self._losses(args, shape, nbytes, losses, lse)
         self._call("xent", args, rows)
         return out
 
@@ -762,9 +765,9 @@ class DenseLoss:
                 lse=None):
         """The teacher's top logits as CSR: offsets int32 [rows + 1], ids int32
         (ascending within a row) and teacher_logits float32 [entries]."""
-        rows, args = self._begin(hidden)
+        rows, shape, nbytes, args = self._begin(hidden)
         self._sets(args, rows, offsets, ids, teacher_logits, temperature)
-        out = self._losses(args, rows, losses, lse)
+        out = self._losses(args, shape, nbytes, losses, lse)
         self._call("distill", args, rows)
         return out
 
@@ -772,17 +775,18 @@ class DenseLoss:
                    embedding_grad):
         if not self._backward:
             raise RuntimeError("this DenseLoss was made with backward=False")
-        f32, kind = self._torch.float32, self.embedding.dtype
-        self._in(args, "lse", lse, f32, (rows,))
-        self._in(args, "grad_losses", grad_losses, f32, (rows,))
+        shape, nbytes, width = (rows,), rows * 4, self.hidden_size
+        self._in(args, "lse", lse, self._f32, shape, nbytes)
+        self._in(args, "grad_losses", grad_losses, self._f32, shape, nbytes)
         if hidden_grad:
-            d_hidden = self._out(args, "d_hidden", d_hidden, kind, (rows, self.hidden_size))
+            d_hidden = self._out(args, "d_hidden", d_hidden, self._kind, (rows, width),
+                                 rows * width * 2)
         else:
             d_hidden = None
             args += (0, 0)
         if embedding_grad:
-            d_embedding = self._out(args, "d_embedding", d_embedding, kind,
-                                    (self.vocab, self.hidden_size))
+            d_embedding = self._out(args, "d_embedding", d_embedding, self._kind,
+                                    self._table_shape, self._table_bytes)
         else:
             d_embedding = None
             args += (0, 0)
@@ -792,8 +796,8 @@ class DenseLoss:
                                d_embedding=None, hidden_grad=True, embedding_grad=True):
         """Gradients of ``(grad_losses * losses).sum()``; ``lse`` as
         ``cross_entropy`` returned it."""
-        rows, args = self._begin(hidden)
-        self._in(args, "targets", targets, self._torch.int32, (rows,))
+        rows, shape, nbytes, args = self._begin(hidden)
+        self._in(args, "targets", targets, self._i32, shape, nbytes)
         out = self._gradients(args, rows, lse, grad_losses, d_hidden, d_embedding, hidden_grad,
                               embedding_grad)
         self._call("xent_backward", args, rows)
@@ -803,7 +807,7 @@ class DenseLoss:
                          d_hidden=None, d_embedding=None, hidden_grad=True, embedding_grad=True):
         """Gradients of ``(grad_losses * losses).sum()``; ``lse`` as ``distill``
         returned it with the same temperature."""
-        rows, args = self._begin(hidden)
+        rows, _, _, args = self._begin(hidden)
         self._sets(args, rows, offsets, ids, teacher_logits, temperature)
         out = self._gradients(args, rows, lse, grad_losses, d_hidden, d_embedding, hidden_grad,
                               embedding_grad)
