@@ -19,6 +19,14 @@
  *                  the target for cross entropy):
  *                  d_hidden = d . embedding, d_embedding = d^T . hidden
  *
+ * MF_LOSS_MAX_ROWS: the tensor core's sums lose up to 4e-9 a product of a sum
+ * that grows steadily, so d_embedding of more rows in one call would lose what
+ * its type holds; larger batches go in slices whose gradients the caller adds.
+ *
+ * Scores come from the tensor cores: relative to a score, an error of about
+ * 1e-9 to 3e-9 a product of its width remains.  The target's own score, and in
+ * batches of up to 64 rows a teacher set's, are summed with rounding to nearest.
+ *
  * Types: _f16 takes fp16 and _bf16 bfloat16 hidden rows and table; gradients
  * have the type of what they are the gradient of.  Losses, lse, grad_losses
  * and teacher logits are f32, every sum is held in FP32, and d is rounded once
@@ -27,10 +35,11 @@
  * Arguments are validated as mf_head.h says, before any launch, with these
  * additions: hidden_size is a multiple of 8 up to MF_LOSS_MAX_HIDDEN, rows at
  * most MF_LOSS_MAX_ROWS, vocab at most MF_LOSS_MAX_VOCAB, entries at most
- * INT32_MAX (MF_RESOURCE_LIMIT otherwise); hidden, embedding, d_hidden,
- * d_embedding and the workspace are 16-byte aligned, and no output and no
- * workspace overlaps another buffer (MF_INVALID_ARGUMENT otherwise).  The
- * current device must be the one that owns the buffers and the stream.
+ * INT32_MAX (MF_RESOURCE_LIMIT otherwise); hidden, embedding, d_hidden and
+ * d_embedding are 16-byte aligned and the workspace 256-byte (as cudaMalloc
+ * gives it), and no output and no workspace overlaps another buffer
+ * (MF_INVALID_ARGUMENT otherwise).  The current device must be the one that
+ * owns the buffers and the stream.
  *
  * Rows: a cross entropy row whose target is MF_INVALID_TOKEN (what the heads
  * write for a row without a candidate), and a distillation row with an empty
@@ -60,14 +69,14 @@
 extern "C" {
 #endif
 
-#define MF_LOSS_MAX_ROWS (1u << 20)
+#define MF_LOSS_MAX_ROWS (1u << 16)
 #define MF_LOSS_MAX_VOCAB (1u << 24)
 #define MF_LOSS_MAX_HIDDEN 8192u
 
-/* Bytes of device memory a forward call and a backward call need; 0 for sizes
- * outside the limits.  A backward call's holds two pieces of d of at most 128
- * MiB (512 bytes a row above 256 Ki rows), a copy of the hidden rows and FP32
- * sums of d_hidden of at most 128 MiB (4 bytes an element above 32 Mi elements). */
+/* Bytes of device memory that a forward call and a backward call of at most
+ * `rows` rows need; 0 for sizes outside the limits.  A backward call's holds up to two pieces of d of at most
+ * 128 MiB, a copy of the hidden rows, and FP32 sums of d_hidden of at most 128
+ * MiB (4 bytes an element above 32 Mi elements). */
 MF_API uint64_t mf_dense_loss_workspace_bytes(uint64_t rows, uint64_t hidden_size, uint64_t vocab);
 MF_API uint64_t mf_dense_loss_backward_workspace_bytes(uint64_t rows, uint64_t hidden_size,
                                                        uint64_t vocab);

@@ -57,12 +57,12 @@ constexpr uint64_t kPieceBytes = 128ull << 20; // one piece of d
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // The tensor core's additions drop the bits that fall below the sum's last
-// place, always towards zero, so a score comes out too small by a part that
-// grows with the width: measured 3.6e-9 to 4.5e-9 a product for scores that
-// grow steadily (64 to 1,024 products, standard deviation 0.2e-9), less where
-// the products cancel and the score is small.  Scores are scaled by 1 + width
-// 2^-28.
-constexpr float kLostPerProduct = 3.725290298461914e-9f;
+// place, so a score of K products comes out too small.  Measured, relative to
+// the score and per product, for K from 128 to 2,048: 1.1e-9 where the products
+// nearly cancel (cosine of the two rows 0.1), 1.4e-9 to 1.9e-9 at cosine 0.3,
+// 2.2e-9 to 2.7e-9 at 0.5, 4.2e-9 to 4.8e-9 at 0.9, with a standard deviation
+// of 1.3e-7 to 4.5e-7 of the score.  Scores are scaled by 1 + K 2^-29.
+constexpr float kLostPerProduct = 1.862645149230957e-9f;
 
 template <typename T>
 struct Type;
@@ -692,7 +692,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
         const uint32_t acc = tmem + (sub & 1u) * kBN;
         if (t.kind == kScore) {
           constexpr uint32_t idesc = kIdesc | ((uint32_t)(kBN >> 3) << 17);
-          bool ready = bar_try(s_full(sr.at), sr.fills & 1u);
+          bool ready = bar_test(s_full(sr.at), sr.fills & 1u);
           for (uint32_t kc = 0; kc < t.chunks; ++kc) {
             if (!ready && !bar_wait(s_full(sr.at), sr.fills & 1u)) {
               ok = false;
@@ -704,7 +704,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
                                              : b + kChunkBytes / 16;
             sr.next();
             // asked before the MMAs, whose issue takes as long as they do
-            ready = bar_try(s_full(sr.at), sr.fills & 1u);
+            ready = bar_test(s_full(sr.at), sr.fills & 1u);
 #pragma unroll
             for (int k4 = 0; k4 < kBK / 16; ++k4)
               mma_pair(acc, a + 2 * k4, b + 2 * k4, idesc, (kc | (uint32_t)k4) != 0u);
@@ -717,7 +717,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
           const uint32_t a_step = t.kind == kTable ? 2048 / 16 : 2;
           const uint32_t stage = p.p_stage_bytes / 16;
           const uint32_t acc1 = tmem + ((sub + 1) & 1u) * kBN;
-          bool ready = bar_try(p_full(pr.at), pr.fills & 1u);
+          bool ready = bar_test(p_full(pr.at), pr.fills & 1u);
           for (uint32_t kc = 0; kc < t.chunks; ++kc) {
             if (!ready && !bar_wait(p_full(pr.at), pr.fills & 1u)) {
               ok = false;
@@ -726,7 +726,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
             const uint32_t at = pr.at;
             const uint64_t b = n_major + at * stage, a = a0 + at * stage;
             pr.next();
-            ready = bar_try(p_full(pr.at), pr.fills & 1u);
+            ready = bar_test(p_full(pr.at), pr.fills & 1u);
 #pragma unroll
             for (int k4 = 0; k4 < kBK / 16; ++k4)
               mma_pair(acc, a + a_step * k4, b + 64 * k4, idesc, (kc | (uint32_t)k4) != 0u);
@@ -1090,7 +1090,9 @@ __global__ void merge_kernel(Wanted w, const T* hidden, const T* table, uint32_t
 // even to 32 rows), against the hidden rows, which stay in shared memory (N =
 // rows rounded up to 16).  All its scores fit in TMEM, so the softmax needs no
 // running maximum: one pass for each row's maximum over the CTA's range, one
-// for the sum.  The wanted scores come from the FP32 pipes in the join.
+// for the sum.  TMEM that is left holds each score in up to three segments of
+// its products, added in FP32.  The wanted scores come from the FP32 pipes in
+// the join.
 constexpr uint32_t kFewRows = 64;
 constexpr uint32_t kFewMaxStages = 12;
 constexpr uint32_t kFewThreads = 192;  // producer, MMA issuer, 4 epilogue warps
@@ -1100,6 +1102,7 @@ struct FewParams {
   uint32_t rows, n;         // n: rows rounded up to 16
   uint32_t vocab, range;    // table rows per CTA, a multiple of 32
   uint32_t w_chunks, stages;
+  uint32_t segments, seg_chunks;  // accumulators of a score, chunks in each
   float c2;                 // score scale / T in units of ln 2
   Partial* partial;         // [CTA][rows]
 };
@@ -1190,6 +1193,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
       Ring rg(p.stages);
       bool ok = bar_wait(h_full, 0);
       for (uint32_t t = 0; ok && t < tiles; ++t) {
+        uint32_t acc = tmem + t * p.segments * p.n, seg_end = p.seg_chunks;
         for (uint32_t kc = 0; kc < p.w_chunks; ++kc) {
           if (!bar_wait(full(rg.at), rg.fills & 1u)) {
             ok = false;
@@ -1198,9 +1202,11 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
           fence_after();
           const uint64_t a = sw128_desc(ring + rg.at * kChunkBytes);
           const uint64_t b = sw128_desc(hid + kc * hid_chunk);
+          if (kc == seg_end) acc += p.n, seg_end += p.seg_chunks;
+          const bool add = kc + p.seg_chunks != seg_end;
 #pragma unroll
           for (int k4 = 0; k4 < kBK / 16; ++k4)
-            mma_one(tmem + t * p.n, a + 2 * k4, b + 2 * k4, idesc, (kc | (uint32_t)k4) != 0u);
+            mma_one(acc, a + 2 * k4, b + 2 * k4, idesc, add || k4 != 0);
           mma_commit_one(empty(rg.at));
           rg.next();
         }
@@ -1214,13 +1220,23 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
     const bool ok = bar_wait(done, 0) && !*abort_flag;
     fence_after();
     const uint32_t acc = tmem + ((quad * 32u) << 16);
+    auto scores = [&](uint32_t t, uint32_t c, uint32_t (&r)[16]) {  // the segments' sum
+      tmem_ld16(acc + t * p.segments * p.n + c, r);
+      for (uint32_t g = 1; g < p.segments; ++g) {
+        uint32_t x[16];
+        tmem_ld16(acc + (t * p.segments + g) * p.n + c, x);
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(x[j]));
+      }
+    };
     for (uint32_t c = 0; c < p.n; c += 16) {
       float mx[16], l[16];
 #pragma unroll
       for (int j = 0; j < 16; ++j) mx[j] = -INFINITY, l[j] = 0.f;
       for (uint32_t t = 0; t < tiles; ++t) {
         uint32_t r[16];
-        tmem_ld16(acc + t * p.n + c, r);
+        scores(t, c, r);
         const bool in = t * 128 + quad * 32 + lane < count;
 #pragma unroll
         for (int j = 0; j < 16; ++j) mx[j] = fmaxf(mx[j], in ? __uint_as_float(r[j]) : -INFINITY);
@@ -1233,7 +1249,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
       float sum[16] = {};
       for (uint32_t t = 0; t < tiles; ++t) {
         uint32_t r[16];
-        tmem_ld16(acc + t * p.n + c, r);
+        scores(t, c, r);
         const bool in = t * 128 + quad * 32 + lane < count;
 #pragma unroll
         for (int j = 0; j < 16; ++j)
@@ -1806,8 +1822,11 @@ struct BackwardPlan {
   uint32_t splits, per_split;
   uint32_t sets;          // pieces with planes of their own
   BackwardPlan(uint64_t rows, uint64_t width, uint64_t vocab) {
+    // decided by the number of row tiles, so that within one the bytes grow
+    // with the rows
     m_tiles = (rows + 2 * kBM - 1) / (2 * kBM);
-    uint64_t c = kPieceBytes / (2 * rows) / kBN * kBN;
+    const uint64_t all_rows = m_tiles * 2 * kBM;
+    uint64_t c = kPieceBytes / (2 * all_rows) / kBN * kBN;
     if (c < kBN) c = kBN;
     pieces = (uint32_t)((vocab + c - 1) / c);
     cols = (uint32_t)round_up((vocab + pieces - 1) / pieces, kBN);
@@ -1818,7 +1837,7 @@ struct BackwardPlan {
     // pair's share of the two products
     const uint64_t chunks = ((cols < vocab ? cols : vocab) + kBK - 1) / kBK;
     const uint64_t total = bn_tiles * (m_tiles * chunks + (cols + 2 * kBM - 1) / (2 * kBM) *
-                                                              ((rows + kBK - 1) / kBK));
+                                                              (all_rows / kBK));
     uint64_t most = total / kMaxPairs / 2;
     if (most < 4) most = 4;
     // Two 256-row blocks a tile read B once (backward, us, one block and two:
@@ -1826,7 +1845,7 @@ struct BackwardPlan {
     // 328 100 and 91, 512 x 49,152 x 576 109 and 104), but leave no accumulator
     // to drain into, which short K does not repay, and waste half a tile of an
     // odd few (600 x 20,000 x 1,024, three row tiles: 95 and 114)
-    blocks = rows >= 8 * kBK && most >= 32 && (m_tiles % 2 == 0 || m_tiles >= 8) ? 2 : 1;
+    blocks = all_rows >= 8 * kBK && most >= 32 && (m_tiles % 2 == 0 || m_tiles >= 8) ? 2 : 1;
     if (blocks == 2) most /= 2;
     splits = (uint32_t)((chunks + most - 1) / most);
     per_split = (uint32_t)((chunks + splits - 1) / splits);
@@ -1834,7 +1853,7 @@ struct BackwardPlan {
     // Sums kept apart cost a store a piece and are joined at the end; adding at
     // L2 from this layout (a row a thread) made a launch 25 us longer at 8,192 rows
     const uint64_t set = (uint64_t)splits * rows * width * 4;
-    sets = (uint32_t)(kPieceBytes / set);
+    sets = (uint32_t)(kPieceBytes / ((uint64_t)splits * all_rows * width * 4));
     if (sets > pieces) sets = pieces;
     if (sets < 1) sets = 1;
     stat = 0;
@@ -1851,6 +1870,19 @@ struct BackwardPlan {
     bytes = piece[1] + one;
   }
 };
+
+// What a batch of at most `rows` rows needs: the most that any needs.  Within a
+// row tile, and up to `few` rows, a plan's bytes grow with the rows.
+template <typename F>
+uint64_t most_bytes(uint64_t rows, uint64_t few, F bytes) {
+  uint64_t most = bytes(rows);
+  auto at = [&](uint64_t r) {
+    if (r < rows && bytes(r) > most) most = bytes(r);
+  };
+  at(few);
+  for (uint64_t r = 2 * kBM; r < rows; r += 2 * kBM) at(r);
+  return most;
+}
 
 // The checks that all calls share; `wanted` gives the rows' targets or sets.
 mf_status check(uint64_t rows, uint64_t width, uint64_t vocab, void* stream, Span hidden,
@@ -1869,7 +1901,7 @@ mf_status check(uint64_t rows, uint64_t width, uint64_t vocab, void* stream, Spa
   if (hidden.p == nullptr || hidden.bytes != rows * width * 2 || embedding.p == nullptr ||
       embedding.bytes != vocab * width * 2 || workspace.p == nullptr || workspace.bytes < needed ||
       (uintptr_t)hidden.p % 16 != 0 || (uintptr_t)embedding.p % 16 != 0 ||
-      (uintptr_t)workspace.p % 16 != 0)
+      (uintptr_t)workspace.p % 256 != 0)
     return fail(MF_INVALID_ARGUMENT);
   for (const Span& s : row_f32)
     if (s.p == nullptr || s.bytes != rows * 4 || (uintptr_t)s.p % 4 != 0)
@@ -2041,14 +2073,19 @@ cudaError_t teacher_launch(const Wanted& w, uint64_t rows, uint64_t entries, uin
 
 // How the few-rows kernel takes a call; stages 0: it does not.
 struct FewPlan {
-  uint32_t n, range, ctas, stages = 0;
+  uint32_t n, range, ctas, segments, seg_chunks, stages = 0;
   uint64_t smem;
   FewPlan(uint64_t rows, uint64_t width, uint64_t vocab, uint64_t sms) {
     if (rows > kFewRows) return;
     n = (uint32_t)round_up(rows, 16);
     range = (uint32_t)round_up((vocab + sms - 1) / sms, 32);
     ctas = (uint32_t)((vocab + range - 1) / range);
-    if ((uint64_t)(range + 127) / 128 * n > kTmemCols) return;  // scores beyond TMEM
+    const uint32_t columns = (range + 127) / 128 * n;
+    if (columns > kTmemCols) return;  // scores beyond TMEM
+    const uint32_t chunks = (uint32_t)((width + kBK - 1) / kBK);
+    segments = kTmemCols / columns < 3 ? kTmemCols / columns : 3;
+    seg_chunks = (chunks + segments - 1) / segments;
+    segments = (chunks + seg_chunks - 1) / seg_chunks;
     const uint64_t hid = round_up((width + kBK - 1) / kBK * n * 128, 1024);
     if (hid + 4 * kChunkBytes + 1024 > kFewSmem) return;  // no room for a ring
     const uint64_t room = (kFewSmem - 1024 - hid) / kChunkBytes;
@@ -2114,7 +2151,9 @@ mf_status forward_few(const FewPlan& few, Wanted w, const T* hidden, const T* ta
   p.range = few.range;
   p.w_chunks = (uint32_t)((width + kBK - 1) / kBK);
   p.stages = few.stages;
-  p.c2 = w.inv_t * (1.f + (float)width * kLostPerProduct) * kLog2e;
+  p.segments = few.segments;
+  p.seg_chunks = few.seg_chunks;
+  p.c2 = w.inv_t * (1.f + (float)(few.seg_chunks * kBK) * kLostPerProduct) * kLog2e;
   p.partial = static_cast<Partial*>(partial);
   cudaError_t e = launch_after(few_rows_kernel<T>, few.ctas, kFewThreads, few.smem, s, tm_h,
                                tm_t, p);
@@ -2342,13 +2381,17 @@ using mfb::loss::Span;
 
 extern "C" uint64_t mf_dense_loss_workspace_bytes(uint64_t rows, uint64_t hidden_size,
                                                   uint64_t vocab) {
-  return loss::sizes_ok(rows, hidden_size, vocab) ? loss::ForwardPlan(rows, vocab).bytes : 0;
+  if (!loss::sizes_ok(rows, hidden_size, vocab)) return 0;
+  return loss::most_bytes(rows, loss::kFewRows,
+                          [&](uint64_t r) { return loss::ForwardPlan(r, vocab).bytes; });
 }
 
 extern "C" uint64_t mf_dense_loss_backward_workspace_bytes(uint64_t rows, uint64_t hidden_size,
                                                            uint64_t vocab) {
-  return loss::sizes_ok(rows, hidden_size, vocab)
-             ? loss::BackwardPlan(rows, hidden_size, vocab).bytes : 0;
+  if (!loss::sizes_ok(rows, hidden_size, vocab)) return 0;
+  return loss::most_bytes(rows, loss::kFewGradRows, [&](uint64_t r) {
+    return loss::BackwardPlan(r, hidden_size, vocab).bytes;
+  });
 }
 
 #define MF_LOSS_ENTRY_POINTS(SUFFIX, TYPE)                                                         \

@@ -70,6 +70,19 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
   return done != 0u;
 }
 
+// Whether that phase is over, without waiting.
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 q, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0u;
+}
+
 // Wait for the phase of parity `parity` of `bar`, for at most kWaitLimitNs.
 // The clock is read only once a wait turns out to be a long one.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {

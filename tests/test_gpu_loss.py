@@ -665,3 +665,52 @@ def test_current_stream_is_used_and_checked(mf):
     torch.cuda.synchronize()
     ref = Reference(h, e, "f16", targets)
     _near(losses, ref.losses, ref.losses_off, "losses")
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_one_object_for_batches_of_every_size(mf, kind):
+    """One workspace, batches that grow and shrink over it."""
+    import torch
+
+    _, e, _ = _problem(50, 1, 1500, 96, kind)
+    stream = gpu_stream()
+    loss = mf.DenseLoss(e, 900, stream=stream)
+    for rows in (900, 1, 65, 64, 257, 32, 33, 600, 256):
+        h, _, gen = _problem(51 + rows, rows, 1, 96, kind)
+        targets = _targets(gen, rows, 1500, 0.1)
+        sets = _sets(gen, rows, 1500, 30)
+        grad = torch.rand(rows, generator=gen, device="cuda")
+        torch.cuda.synchronize()
+        for kw in (dict(targets=targets), dict(sets=sets, temperature=2.0)):
+            ref = Reference(h, e, kind, grad=grad, **kw)
+            losses, lse = (loss.cross_entropy(h, targets) if "targets" in kw
+                           else loss.distill(h, *sets, 2.0))
+            torch.cuda.synchronize()
+            _near(losses, ref.losses, ref.losses_off, "losses")
+            dh, de = _backward(mf, loss, h, lse, grad, **kw)
+            _near(dh, ref.d_hidden, ref.dh_off, "d_hidden")
+            _near(de, ref.d_embedding, ref.de_off, "d_embedding")
+
+
+def test_outputs_that_are_only_16_byte_aligned(mf):
+    """Inputs and gradients that start 16 bytes into their memory."""
+    import torch
+
+    for rows, vocab, width in ((20, 700, 96), (150, 700, 96)):
+        h, e, gen = _problem(60, rows, vocab, width, "f16")
+        targets = _targets(gen, rows, vocab, 0.1)
+        grad = torch.rand(rows, generator=gen, device="cuda")
+
+        def shifted(t):
+            out = torch.empty(t.numel() + 8, dtype=t.dtype, device="cuda")[8:].view(t.shape)
+            out.copy_(t)
+            return out
+
+        want_loss, (_, lse) = _forward(mf, h, e, targets)
+        want = _backward(mf, want_loss, h, lse, grad, targets)
+        h2, e2 = shifted(h), shifted(e)
+        loss, (_, lse2) = _forward(mf, h2, e2, targets)
+        assert torch.equal(lse, lse2)
+        got = _backward(mf, loss, h2, lse2, grad, targets, d_hidden=shifted(h),
+                        d_embedding=shifted(e))
+        assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])

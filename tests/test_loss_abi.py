@@ -86,7 +86,7 @@ def test_sizes(lib, E, call, kind, backward):
     assert call(lib, kind, backward, stream=0) == E.invalid_argument
     assert call(lib, kind, backward, width=60) == E.resource_limit  # a multiple of 8
     assert call(lib, kind, backward, width=8200) == E.resource_limit
-    assert call(lib, kind, backward, rows=(1 << 20) + 1) == E.resource_limit
+    assert call(lib, kind, backward, rows=(1 << 16) + 1) == E.resource_limit
     assert call(lib, kind, backward, vocab=(1 << 24) + 1) == E.resource_limit
 
 
@@ -112,7 +112,8 @@ def test_buffers(lib, E, call, kind, backward):
     need = (lib.mf_dense_loss_backward_workspace_bytes if backward
             else lib.mf_dense_loss_workspace_bytes)(ROWS, HIDDEN, VOCAB)
     assert call(lib, kind, backward, workspace=(at, need - 1)) == E.invalid_argument
-    assert call(lib, kind, backward, workspace=(at + 8, need)) == E.invalid_argument
+    for off in (8, 16, 32, 128):  # the workspace starts on 256 bytes
+        assert call(lib, kind, backward, workspace=(at + off, need)) == E.invalid_argument
     # an output or the workspace that overlaps another buffer, by its last bytes
     out = "lse" if not backward else "d_hidden"
     size = ROWS * 4 if not backward else ROWS * HIDDEN * 2
@@ -140,16 +141,27 @@ def test_distill_only(lib, E, kind, backward):
 
 def test_workspace_bytes(lib):
     f, b = lib.mf_dense_loss_workspace_bytes, lib.mf_dense_loss_backward_workspace_bytes
-    for bad in ((0, 64, 8), (8, 0, 8), (8, 64, 0), (8, 65, 8), ((1 << 20) + 1, 64, 8),
+    for bad in ((0, 64, 8), (8, 0, 8), (8, 64, 0), (8, 65, 8), ((1 << 16) + 1, 64, 8),
                 (8, 64, (1 << 24) + 1), (8, 8200, 8)):
         assert f(*bad) == 0 and b(*bad) == 0
-    for rows in (1, 100, 8192, 1 << 19):
+    for rows in (1, 100, 8192, 1 << 16):
         for vocab in (1, 1000, 49152):
             assert 0 < f(rows, 576, vocab) <= 4096 + rows * 3300
             # two pieces of d, the copy of the rows, FP32 sums of d_hidden
-            pieces = 2 * max(128 << 20, 512 * rows)
+            pieces = 2 * (128 << 20)
             sums = max(128 << 20, rows * 576 * 4)
             assert rows * 576 * 6 < b(rows, 576, vocab) <= pieces + sums + rows * 576 * 2 + 4096 + rows * 24
+
+
+def test_a_workspace_holds_every_smaller_batch(lib):
+    """A user keeps one workspace for the largest batch."""
+    f, b = lib.mf_dense_loss_workspace_bytes, lib.mf_dense_loss_backward_workspace_bytes
+    steps = [1, 2, 16, 31, 32, 33, 63, 64, 65, 100, 255, 256, 257, 300, 511, 512, 513, 700, 768,
+             1000, 1024, 1025, 2000, 4096, 5000, 8192, 20_000, 65_536]
+    for width, vocab in ((576, 49152), (64, 300), (1024, 20_000), (8, 1)):
+        for g in (f, b):
+            sizes = [g(r, width, vocab) for r in steps]
+            assert sizes == sorted(sizes)
 
 
 def test_class_checks_before_the_call():
