@@ -514,16 +514,19 @@ struct Cursor {
       at = min(end, at + 4 - n);
     }
   }
+  // Takes the first entry off in the lanes that say so.  All lanes of the warp
+  // call it: where one has used its window up, all top theirs up, so that a
+  // tile waits for memory a few times and not once for every lane.
+  __device__ __forceinline__ void drop(const Wanted& w, bool mine) {
+    if (mine) pop();
+    if constexpr (kDistill)
+      if (__any_sync(0xFFFFFFFFu, id[0] == 0xFFFFFFFFu && at < end)) fill(w);
+  }
   // Drops entries below v.
   __device__ __forceinline__ void skip_to(const Wanted& w, uint32_t v) {
     if constexpr (kDistill) {
-      while (id[0] < v) next(w);
+      while (__any_sync(0xFFFFFFFFu, id[0] < v)) drop(w, id[0] < v);
     }
-  }
-  __device__ __forceinline__ void next(const Wanted& w) {
-    pop();
-    if constexpr (kDistill)
-      if (id[0] == 0xFFFFFFFFu && at < end) fill(w);
   }
   // The weight of the first entry; `tlse2` in units of ln 2.
   __device__ __forceinline__ float weight(float t2, float tlse2) const {
@@ -870,11 +873,12 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
             run_l = l[0].x + l[0].y;
             while (__any_sync(0xFFFFFFFFu, cur.id[0] - col < 64u)) {
               const float s = pick64(r, cur.id[0] - col);
-              if (cur.id[0] - col < 64u) {
+              const bool mine = cur.id[0] - col < 64u;
+              if (mine) {
                 const float q = cur.weight(t2, tlse2);
                 if (q > 0.f) dot = fmaf(q, s * inv_t, dot);
-                cur.next(w);
               }
+              cur.drop(w, mine);
             }
           } else {
             // |coef| goes into the exponent
@@ -895,11 +899,12 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
             }
             while (__any_sync(0xFFFFFFFFu, cur.id[0] - col < 64u)) {
               const float s = pick64(r, cur.id[0] - col);
-              if (cur.id[0] - col < 64u) {  // p - q in FP32, over the element just stored
+              const bool mine = cur.id[0] - col < 64u;
+              if (mine) {  // p - q in FP32, over the element just stored
                 const float x = exp2_approx(fmaf(s, c2, -z2)) - cur.weight(t2, tlse2);
                 out[cur.id[0] - col] = Type<T>::from(x * coef);
-                cur.next(w);
               }
+              cur.drop(w, mine);
             }
           }
         }
