@@ -354,7 +354,8 @@ struct Params {
   uint32_t keep_hidden;         // the hidden tile stays in shared memory
   uint32_t s_ring, s_stages, s_stage_bytes;
   float score_scale;            // 1 + what the tensor core's additions lose
-  Partial* partial;             // forward: [slots][rows]
+  Partial* partial;             // forward: [rows][slots]
+  uint32_t slots;
   void* d;                      // backward: the piece being made
   uint32_t pitch;
   const float* lse;
@@ -779,7 +780,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
     };
     auto flush = [&]() {
       if (kForward && cur_m != 0xFFFFFFFFu && row < p.rows)
-        p.partial[(uint64_t)slot * p.rows + row] =
+        p.partial[(uint64_t)row * p.slots + slot] =
             Partial{dead ? nan : run_m, dead ? nan : run_l, dot, 0.f};
     };
     uint32_t sub = 0;
@@ -1038,6 +1039,38 @@ __device__ __forceinline__ void join(float& m, float& l, const Partial& q) {
   m = mn;
 }
 
+// Joins a row's slots over the lanes of a warp; the loads of 160 slots (a call
+// has at most 148 a row, but for few column tiles of many rows) are in flight
+// together.
+__device__ __forceinline__ void join_slots(const Partial* part, uint32_t slots, float& m, float& l,
+                                           float& dot) {
+  const uint32_t lane = threadIdx.x & 31;
+  m = -INFINITY;
+  l = dot = 0.f;
+  for (uint32_t s0 = lane; s0 < slots; s0 += 160) {
+    float4 q[5];
+#pragma unroll
+    for (uint32_t j = 0; j < 5; ++j)
+      q[j] = s0 + 32 * j < slots
+                 ? *reinterpret_cast<const float4*>(part + s0 + 32 * j)
+                 : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    float top = fmaxf(fmaxf(fmaxf(q[0].x, q[1].x), fmaxf(q[2].x, q[3].x)), q[4].x);
+    top = fmaxf(top, m);
+    // a walk without a column has l = 0 at m = -inf
+    float sum = m == top ? l : l * exp2_approx(m - top);
+#pragma unroll
+    for (int j = 0; j < 5; ++j) {
+      sum += q[j].x == top ? q[j].y : q[j].y * exp2_approx(q[j].x - top);
+      dot += q[j].z;
+    }
+    m = top;
+    l = sum;
+  }
+  warp_join(m, l);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
+}
+
 __device__ __forceinline__ float set_loss(const Wanted& w, float2 s, float z, float dot) {
   const float t = 1.f / w.inv_t;
   return stat_empty(s) ? 0.f : (stat_invalid(s) ? s.x : t * t * (s.y + (z - dot)));
@@ -1052,8 +1085,9 @@ __device__ __forceinline__ float target_loss(uint32_t target, uint32_t vocab, fl
 // a loss is a difference of two numbers that a sure row has nearly equal.
 template <typename T>
 __global__ void merge_kernel(Wanted w, const T* hidden, const T* table, uint32_t width,
-                             const Partial* part, uint32_t n_tiles, uint32_t total, uint32_t pairs,
-                             uint32_t rows, uint32_t vocab, float* losses, float* lse) {
+                             const Partial* part, uint32_t row_slots, uint32_t n_tiles,
+                             uint32_t total, uint32_t pairs, uint32_t rows, uint32_t vocab,
+                             float* losses, float* lse) {
   const uint32_t r = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
   if (r >= rows) return;
   const uint32_t target = w.targets ? w.targets[r] : kInvalid;
@@ -1067,16 +1101,8 @@ __global__ void merge_kernel(Wanted w, const T* hidden, const T* table, uint32_t
   const uint32_t first = (uint32_t)(((x0 + 1) * pairs - 1) / total);
   const uint32_t last = (uint32_t)(((x1 + 1) * pairs - 1) / total);
   const uint32_t slots = 2 * (last - first + 1);
-  float m = -INFINITY, l = 0.f, dot = 0.f;
-#pragma unroll 5
-  for (uint32_t s = lane; s < slots; s += 32) {
-    const Partial q = part[(uint64_t)s * rows + r];
-    join(m, l, q);
-    dot += q.dot;
-  }
-  warp_join(m, l);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
+  float m, l, dot;
+  join_slots(part + (uint64_t)r * row_slots, slots, m, l, dot);
   if (target < vocab) {
     l += exp2_approx(fmaf(score, kLog2e, -m)) - exp2_approx(fmaf(dot, kLog2e, -m));
     dot = score;
@@ -1109,7 +1135,7 @@ struct FewParams {
   uint32_t w_chunks, stages;
   uint32_t segments, seg_chunks;  // accumulators of a score, chunks in each
   float c2;                 // score scale / T in units of ln 2
-  Partial* partial;         // [CTA][rows]
+  Partial* partial;         // [rows][CTA]
 };
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -1284,7 +1310,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
       float m = -INFINITY, l = 0.f;
 #pragma unroll
       for (int q = 0; q < 4; ++q) join(m, l, Partial{part[q][r].x, part[q][r].y, 0.f, 0.f});
-      p.partial[(uint64_t)blockIdx.x * p.rows + r] = Partial{m, l, 0.f, 0.f};
+      p.partial[(uint64_t)r * gridDim.x + blockIdx.x] = Partial{m, l, 0.f, 0.f};
     }
   }
   __syncthreads();
@@ -1716,10 +1742,8 @@ few_rows_join_kernel(Wanted w, const T* hidden, const T* table, uint32_t width, 
   for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
   pdl_wait();
   pdl_trigger();
-  float m = -INFINITY, l = 0.f;
-#pragma unroll 5
-  for (uint32_t s = lane; s < slots; s += 32) join(m, l, part[(uint64_t)s * rows + r]);
-  warp_join(m, l);
+  float m, l, none;
+  join_slots(part + (uint64_t)r * slots, slots, m, l, none);
   if (lane) return;
   const float z = (m + log2f(l)) * kLn2;
   lse[r] = z;
@@ -1801,7 +1825,7 @@ bool sizes_ok(uint64_t rows, uint64_t width, uint64_t vocab) {
 }
 
 struct ForwardPlan {
-  uint64_t m_tiles, n_tiles, stat, partial, bytes;
+  uint64_t m_tiles, n_tiles, slots, stat, partial, bytes;
   ForwardPlan(uint64_t rows, uint64_t vocab) {
     m_tiles = (rows + 2 * kBM - 1) / (2 * kBM);
     n_tiles = (vocab + kBN - 1) / kBN;
@@ -1809,7 +1833,7 @@ struct ForwardPlan {
     // floor(m n / pairs) tiles
     uint64_t per = m_tiles * n_tiles / kMaxPairs;
     if (per < 1) per = 1;
-    uint64_t slots = (n_tiles + per - 1) / per + 1;
+    slots = (n_tiles + per - 1) / per + 1;
     if (slots > n_tiles) slots = n_tiles;
     // the few-rows kernel: one slot per CTA
     if (rows <= kFewRows && slots < kMaxPairs) slots = kMaxPairs;
@@ -1839,11 +1863,13 @@ struct BackwardPlan {
     bn_tiles = (uint32_t)((width + kBN - 1) / kBN);
     bn = (uint32_t)round_up((width + bn_tiles - 1) / bn_tiles, 64);
     // d E is split along the piece so that no tile is longer than half a
-    // pair's share of the two products
+    // pair's share of the two products, or the whole share where score tiles
+    // fill the rest (a split costs a plane of sums: 4,096 x 49,152 x 576
+    // backward 603 us with half, 558 with the whole, 580 with two)
     const uint64_t chunks = ((cols < vocab ? cols : vocab) + kBK - 1) / kBK;
     const uint64_t total = bn_tiles * (m_tiles * chunks + (cols + 2 * kBM - 1) / (2 * kBM) *
                                                               (all_rows / kBK));
-    uint64_t most = total / kMaxPairs / 2;
+    uint64_t most = total / kMaxPairs / (pieces > 1 ? 1 : 2);
     if (most < 4) most = 4;
     // Two 256-row blocks a tile read B once (backward, us, one block and two:
     // 2,000 x 49,152 x 576 350 and 322, 4,096 rows 717 and 608, 1,001 x 32,003 x
@@ -2218,13 +2244,14 @@ mf_status forward(Span hidden, Span embedding, Span targets, Span ids, Span logi
   p.cols = (uint32_t)vocab;
   p.n_tiles = (uint32_t)plan.n_tiles;
   p.partial = reinterpret_cast<Partial*>(ws + plan.partial);
+  p.slots = (uint32_t)(2 * plan.slots);
   for (uint32_t i = 0; i <= pairs; ++i) p.score_at[i] = (uint32_t)(total * i / pairs);
   e = launch_after(engine_kernel<T, true, kDistill>, 2 * pairs, kThreads, kSmemBytes, s,
                    maps, p, w);
   if (e != cudaSuccess) return launched(e);
   e = launch_after(merge_kernel<T>, (rows + 7) / 8, 256, 0, s, w,
                    static_cast<const T*>(hidden.p), static_cast<const T*>(embedding.p), p.width,
-                   static_cast<const Partial*>(p.partial), p.n_tiles, (uint32_t)total, pairs,
+                   static_cast<const Partial*>(p.partial), p.slots, p.n_tiles, (uint32_t)total, pairs,
                    p.rows, p.vocab, static_cast<float*>(const_cast<void*>(losses.p)),
                    static_cast<float*>(const_cast<void*>(lse.p)));
   return launched(e);

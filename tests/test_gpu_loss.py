@@ -428,8 +428,12 @@ def test_distillation_of_one_sure_token_is_cross_entropy(mf):
     grad = torch.rand(90, generator=gen, device="cuda")
     _, (a, lse_a) = _forward(mf, h, e, targets)
     loss, (b, lse_b) = _forward(mf, h, e, None, sets)
-    assert torch.equal(lse_a, lse_b)
-    torch.testing.assert_close(a, b, rtol=2.0 ** -22, atol=0)
+    # the target's score is summed with rounding to nearest in one and by the
+    # tensor core in the other: both lie within the formula's bounds
+    ref = Reference(h, e, "f16", targets)
+    for lse, losses in ((lse_a, a), (lse_b, b)):
+        _near(lse, ref.lse, ref.lse_off, "lse")
+        _near(losses, ref.losses, ref.losses_off, "losses")
     x = _backward(mf, loss, h, lse_a, grad, targets)
     y = _backward(mf, loss, h, lse_a, grad, None, sets)
     u = _half_step("f16")
