@@ -30,14 +30,15 @@
  * Types: _f16 takes fp16 and _bf16 bfloat16 hidden rows and table; gradients
  * have the type of what they are the gradient of.  Losses, lse, grad_losses
  * and teacher logits are f32, every sum is held in FP32, and d is rounded once
- * to the 16-bit type for the two gradient products.
+ * to the 16-bit type for the two gradient products (up to 32 rows: to the sum
+ * of two such numbers).
  *
  * Arguments are validated as mf_head.h says, before any launch, with these
  * additions: hidden_size is a multiple of 8 up to MF_LOSS_MAX_HIDDEN, rows at
  * most MF_LOSS_MAX_ROWS, vocab at most MF_LOSS_MAX_VOCAB, entries at most
- * INT32_MAX (MF_RESOURCE_LIMIT otherwise); hidden, embedding, d_hidden and
- * d_embedding are 16-byte aligned and the workspace 256-byte (as cudaMalloc
- * gives it), and no output and no workspace overlaps another buffer
+ * MF_LOSS_MAX_ENTRIES (MF_RESOURCE_LIMIT otherwise); hidden, embedding,
+ * d_hidden and d_embedding are 16-byte aligned and the workspace 256-byte (as
+ * cudaMalloc gives it), and no output and no workspace overlaps another buffer
  * (MF_INVALID_ARGUMENT otherwise).  The current device must be the one that
  * owns the buffers and the stream.
  *
@@ -45,13 +46,12 @@
  * write for a row without a candidate), and a distillation row with an empty
  * set or only -inf teacher logits, is ignored: loss 0, no gradient.  A row
  * with any other target >= vocab, an id outside the vocabulary, ids that do
- * not ascend strictly, or a NaN or +inf teacher logit, is invalid: loss NaN,
- * no gradient; malformed offsets (offsets[0] != 0, decreasing, or
- * offsets[rows] != entries) make every row invalid.  Neither kind, nor a row
- * whose grad_losses is 0, takes part in the gradients: its d_hidden row is 0
- * and what its hidden row holds (NaN included) does not reach d_embedding.
- * lse is written for every row.  Elsewhere a non-finite score gives its row
- * a NaN loss and NaN gradients.
+ * not ascend strictly (the same id twice included), a NaN or +inf teacher
+ * logit, or offsets that decrease or leave [0, entries], is invalid: loss NaN,
+ * no gradient.  Neither kind, nor a row whose grad_losses is 0, takes part in
+ * the gradients: its d_hidden row is 0 and what its hidden row holds (NaN
+ * included) does not reach d_embedding.  lse is written for every row.
+ * Elsewhere a non-finite score gives its row a NaN loss and NaN gradients.
  *
  * Every wait inside the kernels is bounded (100 ms); one that runs out gives
  * NaN in the outputs it covers, and the context stays usable.
@@ -72,6 +72,8 @@ extern "C" {
 #define MF_LOSS_MAX_ROWS (1u << 16)
 #define MF_LOSS_MAX_VOCAB (1u << 24)
 #define MF_LOSS_MAX_HIDDEN 8192u
+/* of a teacher's sets: 32-bit indices that step past their end stay positive */
+#define MF_LOSS_MAX_ENTRIES ((1u << 31) - 1024u)
 
 /* Bytes of device memory that a forward call and a backward call of at most
  * `rows` rows need; 0 for sizes outside the limits.  A backward call's holds up to two pieces of d of at most

@@ -1956,7 +1956,7 @@ mf_status check(uint64_t rows, uint64_t width, uint64_t vocab, void* stream, Spa
     if (ids.bytes % 4 != 0 || ids.bytes != logits.bytes || (uintptr_t)ids.p % 4 != 0 ||
         (uintptr_t)logits.p % 4 != 0 || (ids.bytes != 0 && (ids.p == nullptr || logits.p == nullptr)))
       return fail(MF_INVALID_ARGUMENT);
-    if (ids.bytes / 4 > (uint64_t)INT32_MAX) return fail(MF_RESOURCE_LIMIT);
+    if (ids.bytes / 4 > MF_LOSS_MAX_ENTRIES) return fail(MF_RESOURCE_LIMIT);
   }
   return ok();
 }

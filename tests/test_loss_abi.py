@@ -134,7 +134,7 @@ def test_distill_only(lib, E, kind, backward):
     assert _distill(lib, kind, backward, ids=(0, ENTRIES * 4)) == E.invalid_argument
     assert _distill(lib, kind, backward, teacher_logits=(at + 2, ENTRIES * 4)) \
         == E.invalid_argument
-    big = 1 << 33
+    big = ((1 << 31) - 1023) * 4  # one entry too many
     assert _distill(lib, kind, backward, ids=(1 << 55, big), teacher_logits=(1 << 56, big)) \
         == E.resource_limit
 
