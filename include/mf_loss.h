@@ -26,6 +26,7 @@
  * Scores come from the tensor cores: relative to a score, an error of about
  * 1e-9 to 3e-9 a product of its width remains.  The target's own score, and in
  * batches of up to 64 rows a teacher set's, are summed with rounding to nearest.
+ * Scores over T beyond 1e9 in magnitude may give infinities.
  *
  * Types: _f16 takes fp16 and _bf16 bfloat16 hidden rows and table; gradients
  * have the type of what they are the gradient of.  Losses, lse, grad_losses
@@ -51,7 +52,7 @@
  * no gradient.  Neither kind, nor a row whose grad_losses is 0, takes part in
  * the gradients: its d_hidden row is 0 and what its hidden row holds (NaN
  * included) does not reach d_embedding.  lse is written for every row.
- * Elsewhere a non-finite score gives its row a NaN loss and NaN gradients.
+ * Elsewhere a score of NaN or +inf gives its row a NaN loss and NaN gradients.
  *
  * Every wait inside the kernels is bounded (100 ms); one that runs out gives
  * NaN in the outputs it covers, and the context stays usable.

@@ -87,6 +87,11 @@ struct Type<__half> {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
+  static __device__ __forceinline__ uint32_t least(uint32_t a, uint32_t b) {  // NaN stays
+    uint32_t d;
+    asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
 };
 template <>
 struct Type<__nv_bfloat16> {
@@ -98,6 +103,11 @@ struct Type<__nv_bfloat16> {
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ uint32_t least(uint32_t a, uint32_t b) {  // NaN stays
+    uint32_t d;
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
   }
 };
 
@@ -117,7 +127,7 @@ __device__ __forceinline__ bool stat_invalid(float2 s) { return s.x != s.x; }
 
 // Of one row over one walk through the vocabulary, half of every tile's
 // columns: the largest score in units of ln 2, the sum of exp relative to it,
-// the sum of q s / T.
+// and the sum of q s / T, or the target's score as the tensor core gave it.
 struct __align__(16) Partial {
   float m, l, dot, unused;
 };
@@ -244,6 +254,11 @@ setup_kernel(Wanted w, const float* grad, const T* hidden, T* scaled, RowGrad* r
 
 // ---- the tile engine ----------------------------------------------------
 
+__device__ __forceinline__ float min_nan(float a, float b) {  // NaN stays
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -778,7 +793,9 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
     bool live = false;
     float tlse2 = 0.f, run_m = -INFINITY, run_l = 0.f, dot = 0.f, z2 = 0.f, coef = 0.f;
     float e2 = 0.f;                // log2 |coef| - z2
-    uint32_t keep = 0, sign = 0;   // of the packed pairs of d
+    // of the packed pairs of d; p is at most 1, however far the errors of scores
+    // of 1e6 lie beyond lse
+    uint32_t most = 0, keep = 0, sign = 0;
     Cursor<kDistill> cur;
     cur.none();
     auto release = [&](uint32_t buf) {  // the accumulator has been read
@@ -816,6 +833,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
             coef = p.rg[row].coef;
             z2 = p.lse[row] * kLog2e;
             e2 = log2f(fabsf(coef)) - z2;
+            most = Type<T>::pack(fabsf(coef), fabsf(coef));
             keep = coef != 0.f ? 0xFFFFFFFFu : 0u;
             sign = coef < 0.f ? 0x80008000u : 0u;
             live = coef != 0.f;
@@ -885,7 +903,8 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
               const bool mine = cur.id[0] - col < 64u;
               if (mine) {
                 const float q = cur.weight(t2, tlse2);
-                if (q > 0.f) dot = fmaf(q, s * inv_t, dot);
+                if (!kDistill) dot = s;
+                else if (q > 0.f) dot = fmaf(q, s * inv_t, dot);
               }
               cur.drop(w, mine);
             }
@@ -901,7 +920,8 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
                 for (int e = 0; e < 8; ++e) {
                   const float2 x = fma2(make_float2(__uint_as_float(r[j + 2 * e]),
                                                     __uint_as_float(r[j + 2 * e + 1])), cc, ee);
-                  v[e] = (Type<T>::pack(exp2_approx(x.x), exp2_approx(x.y)) & keep) ^ sign;
+                  v[e] = (Type<T>::least(Type<T>::pack(exp2_approx(x.x), exp2_approx(x.y)), most) &
+                          keep) ^ sign;
                 }
                 store_v8(out + j, v);
               }
@@ -910,7 +930,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
               const float s = pick64(r, cur.id[0] - col);
               const bool mine = cur.id[0] - col < 64u;
               if (mine) {  // p - q in FP32, over the element just stored
-                const float x = exp2_approx(fmaf(s, c2, -z2)) - cur.weight(t2, tlse2);
+                const float x = min_nan(exp2_approx(fmaf(s, c2, -z2)), 1.f) - cur.weight(t2, tlse2);
                 out[cur.id[0] - col] = Type<T>::from(x * coef);
               }
               cur.drop(w, mine);
@@ -1083,8 +1103,29 @@ __device__ __forceinline__ float set_loss(const Wanted& w, float2 s, float z, fl
   const float t = 1.f / w.inv_t;
   return stat_empty(s) ? 0.f : (stat_invalid(s) ? s.x : t * t * (s.y + (z - dot)));
 }
-__device__ __forceinline__ float target_loss(uint32_t target, uint32_t vocab, float z, float dot) {
-  return target == kInvalid ? 0.f : (target >= vocab ? __uint_as_float(0x7FC00000u) : z - dot);
+// Of a row without a target: ignored or invalid.
+__device__ __forceinline__ float no_target_loss(uint32_t target) {
+  return target == kInvalid ? 0.f : __uint_as_float(0x7FC00000u);
+}
+
+// The target's score `dot` as it came from the tensor core (c2: its scale, in
+// units of ln 2) leaves a row's sum (m, l), where it is exp2(dot c2 - m), and
+// `score` from the FP32 pipes takes its place.  Returns
+// the loss: ln of the sum over the target's term, which lse's rounding does not
+// reach.  The two scores may lie further apart than an exponential's range
+// (scores of 1e8).
+__device__ __forceinline__ float put_target(float& m, float& l, float dot, float c2,
+                                            float score) {
+  float rest = l - exp2_approx(fmaf(dot, c2, -m));
+  if (rest < 0.f) rest = 0.f;  // rounding; a NaN stays
+  const float above = fmaf(score, kLog2e, -m);
+  if (above > 0.f || rest == 0.f) {  // the target is the largest
+    l = 1.f + (rest == 0.f ? 0.f : rest * exp2_approx(-above));
+    m += above;
+    return log2f(l) * kLn2;
+  }
+  l = rest + exp2_approx(above);
+  return (log2f(l) - above) * kLn2;
 }
 
 // One warp per row joins the walks' partial sums.  Row tile m's n_tiles tiles
@@ -1095,7 +1136,7 @@ template <typename T>
 __global__ void merge_kernel(Wanted w, const T* hidden, const T* table, uint32_t width,
                              const Partial* part, uint32_t row_slots, uint32_t n_tiles,
                              uint32_t total, uint32_t pairs, uint32_t rows, uint32_t vocab,
-                             float* losses, float* lse) {
+                             float c2, float* losses, float* lse) {
   const uint32_t r = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
   if (r >= rows) return;
   const uint32_t target = w.targets ? w.targets[r] : kInvalid;
@@ -1111,14 +1152,12 @@ __global__ void merge_kernel(Wanted w, const T* hidden, const T* table, uint32_t
   const uint32_t slots = 2 * (last - first + 1);
   float m, l, dot;
   join_slots(part + (uint64_t)r * row_slots, slots, m, l, dot);
-  if (target < vocab) {
-    l += exp2_approx(fmaf(score, kLog2e, -m)) - exp2_approx(fmaf(dot, kLog2e, -m));
-    dot = score;
-  }
   if (lane) return;
+  float loss = no_target_loss(target);
+  if (target < vocab) loss = put_target(m, l, dot, c2, score);
   const float z = (m + log2f(l)) * kLn2;
   lse[r] = z;
-  losses[r] = w.targets ? target_loss(target, vocab, z, dot) : set_loss(w, w.stat[r], z, dot);
+  losses[r] = w.targets ? loss : set_loss(w, w.stat[r], z, dot);
 }
 
 // ---- few rows ------------------------------------------------------------
@@ -1131,7 +1170,7 @@ __global__ void merge_kernel(Wanted w, const T* hidden, const T* table, uint32_t
 // running maximum: one pass for each row's maximum over the CTA's range, one
 // for the sum.  TMEM that is left holds each score in up to three segments of
 // its products, added in FP32.  The wanted scores come from the FP32 pipes in
-// the join.  Measured (49,152 x 576, fp16, table from DRAM): 13.9 us for 1 row
+// the join, where the target's takes the place of the tensor core's.  Measured (49,152 x 576, fp16, table from DRAM): 13.9 us for 1 row
 // (4.1 TB/s; a read of the table alone takes 8.6 us at 6.55 TB/s), against 24.6
 // us with the tile engine; the join adds 1.4 us.
 constexpr uint32_t kFewRows = 64;
@@ -1145,7 +1184,8 @@ struct FewParams {
   uint32_t w_chunks, stages;
   uint32_t segments, seg_chunks;  // accumulators of a score, chunks in each
   float c2;                 // score scale / T in units of ln 2
-  Partial* partial;         // [rows][CTA]
+  const uint32_t* targets;  // or NULL
+  Partial* partial;         // [rows][CTA]; dot: the target's, where it is in the range
 };
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -1154,6 +1194,13 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
   tmem_wait_ld();
+}
+
+__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+  tmem_wait_ld();
+  return __uint_as_float(r);
 }
 
 __device__ __forceinline__ float warp_max(float v) {
@@ -1170,6 +1217,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
   __shared__ uint64_t bars[2 * kFewMaxStages + 2];
   __shared__ uint32_t tmem_at, abort_word, filled;
   __shared__ float2 part[4][kFewRows];
+  __shared__ float s_dot[kFewRows];
   const uint32_t hid = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t hid_chunk = p.n * 128;
   const uint32_t ring = hid + ((p.w_chunks * hid_chunk + 1023u) & ~1023u);
@@ -1258,6 +1306,15 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
     }
   } else {
     const uint32_t quad = warp & 3;
+    uint32_t target[2];  // of rows lane and lane + 32, from v0 on; the warp's own, if any
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+      const uint32_t r = lane + 32 * i;
+      target[i] = p.targets && r < p.rows ? p.targets[r] - v0 : kInvalid;
+      if (target[i] >= count || ((target[i] >> 5) & 3u) != quad) target[i] = kInvalid;
+      if (warp == 2) s_dot[r] = 0.f;
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");  // the epilogue warps
     const bool ok = bar_wait(done, 0) && !*abort_flag;
     fence_after();
     const uint32_t acc = tmem + ((quad * 32u) << 16);
@@ -1313,6 +1370,17 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
       if ((lane & 1u) == 0)
         part[quad][c + lane / 2] = make_float2(mx[0], ok ? sum[0] : __uint_as_float(0x7FC00000u));
     }
+    // the targets' scores: of all rows' targets, few lie in one CTA's range
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i)
+      for (uint32_t todo = __ballot_sync(0xFFFFFFFFu, target[i] != kInvalid); todo; todo &= todo - 1) {
+        const uint32_t from = __ffs(todo) - 1;
+        const uint32_t v = __shfl_sync(0xFFFFFFFFu, target[i], from), c = from + 32 * i;
+        float x = 0.f;
+        for (uint32_t g = 0; g < p.segments; ++g)
+          x += tmem_ld1(acc + ((v / 128) * p.segments + g) * p.n + c);
+        if (lane == (v & 31u)) s_dot[c] = x;
+      }
     fence_before();
     asm volatile("bar.sync 1, 128;" ::: "memory");  // the epilogue warps
     const uint32_t r = threadIdx.x - 64;
@@ -1320,7 +1388,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
       float m = -INFINITY, l = 0.f;
 #pragma unroll
       for (int q = 0; q < 4; ++q) join(m, l, Partial{part[q][r].x, part[q][r].y, 0.f, 0.f});
-      p.partial[(uint64_t)r * gridDim.x + blockIdx.x] = Partial{m, l, 0.f, 0.f};
+      p.partial[(uint64_t)r * gridDim.x + blockIdx.x] = Partial{m, l, s_dot[r], 0.f};
     }
   }
   __syncthreads();
@@ -1607,7 +1675,7 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
           for (int e = 0; e < 2; ++e) {
             const uint32_t n = c + j + e;
             const float coef = s_coef[n];
-            float d = exp2_approx(fmaf(__uint_as_float(r[j + e]), c2, -s_z2[n]));
+            float d = min_nan(exp2_approx(fmaf(__uint_as_float(r[j + e]), c2, -s_z2[n])), 1.f);
             if (kDistill) d -= s_q[n * 128 + row];
             else if (s_target[n] == v) d -= 1.f;
             x[e] = coef == 0.f || !in ? 0.f : (dead ? nan : d * coef);
@@ -1699,7 +1767,7 @@ template <typename T>
 __global__ void __launch_bounds__(kJoinThreads)
 few_rows_join_kernel(Wanted w, const T* hidden, const T* table, uint32_t width, const Partial* part,
                      uint32_t slots, uint32_t rows, uint32_t entries, uint32_t vocab,
-                     float* losses, float* lse) {
+                     float c2, float* losses, float* lse) {
   __shared__ float dots[kJoinThreads / 32];
   const uint32_t r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const T* row = hidden + (uint64_t)r * width;
@@ -1754,12 +1822,14 @@ few_rows_join_kernel(Wanted w, const T* hidden, const T* table, uint32_t width, 
   for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
   pdl_wait();
   pdl_trigger();
-  float m, l, none;
-  join_slots(part + (uint64_t)r * slots, slots, m, l, none);
+  float m, l, tensor;
+  join_slots(part + (uint64_t)r * slots, slots, m, l, tensor);
   if (lane) return;
+  float loss = no_target_loss(target);
+  if (target < vocab) loss = put_target(m, l, tensor, c2, dot);
   const float z = (m + log2f(l)) * kLn2;
   lse[r] = z;
-  losses[r] = w.targets ? target_loss(target, vocab, z, dot) : set_loss(w, st, z, dot);
+  losses[r] = w.targets ? loss : set_loss(w, st, z, dot);
 }
 
 // d_hidden: the splits' sums in a fixed order, scaled and rounded; four columns
@@ -2197,13 +2267,14 @@ mf_status forward_few(const FewPlan& few, Wanted w, const T* hidden, const T* ta
   p.segments = few.segments;
   p.seg_chunks = few.seg_chunks;
   p.c2 = w.inv_t * (1.f + (float)(few.seg_chunks * kBK) * kLostPerProduct) * kLog2e;
+  p.targets = w.targets;
   p.partial = static_cast<Partial*>(partial);
   cudaError_t e = launch_after(few_rows_kernel<T>, few.ctas, kFewThreads, few.smem, s, tm_h,
                                tm_t, p);
   if (e == cudaSuccess)
     e = launch_after(few_rows_join_kernel<T>, rows, kJoinThreads, 0, s, w, hidden, table,
                      (uint32_t)width, static_cast<const Partial*>(p.partial), few.ctas, p.rows,
-                     (uint32_t)entries, p.vocab, losses, lse);
+                     (uint32_t)entries, p.vocab, p.c2, losses, lse);
   return launched(e);
 }
 
@@ -2264,7 +2335,8 @@ mf_status forward(Span hidden, Span embedding, Span targets, Span ids, Span logi
   e = launch_after(merge_kernel<T>, (rows + 7) / 8, 256, 0, s, w,
                    static_cast<const T*>(hidden.p), static_cast<const T*>(embedding.p), p.width,
                    static_cast<const Partial*>(p.partial), p.slots, p.n_tiles, (uint32_t)total, pairs,
-                   p.rows, p.vocab, static_cast<float*>(const_cast<void*>(losses.p)),
+                   p.rows, p.vocab, w.inv_t * p.score_scale * kLog2e,
+                   static_cast<float*>(const_cast<void*>(losses.p)),
                    static_cast<float*>(const_cast<void*>(lse.p)));
   return launched(e);
 }

@@ -279,6 +279,49 @@ def test_confident_rows(mf, kind, rows):
 
 
 @pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows", (100, 25))
+def test_scores_of_hundreds_of_millions(mf, kind, rows):
+    """Scores of 3.5e8, whose errors are beyond an exponential's range: losses and
+    gradients stay finite and within the formulas' bounds, a sure row's loss is 0."""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(21)
+    e = (100.0 * torch.randn(700, 576, generator=gen, device="cuda").sign()).to(_dtype(kind))
+    right = torch.randint(0, 700, (rows,), generator=gen, device="cuda", dtype=torch.int32)
+    h = (e[right.long()] * 60).contiguous()
+    targets = _targets(gen, rows, 700, 0.1)
+    targets[:rows // 2] = right[:rows // 2]
+    _, _, losses, _, _, _ = _check(mf, h, e, kind, torch.full((rows,), 1e-3, device="cuda"),
+                                   targets=targets)
+    assert not bool(losses[:rows // 2].any())
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows", (100, 25))
+def test_sure_rows_lose_no_less_than_nothing(mf, kind, rows):
+    """A loss is lse's distance from a score that it contains, however far the
+    rounding of scores of 1,000 goes."""
+    import torch
+
+    h, e, gen = _problem(22, rows, 3000, 576, kind, 2.0)
+    right = torch.randint(0, 3000, (rows,), generator=gen, device="cuda", dtype=torch.int32)
+    h = (e[right.long()].float() * 400).to(_dtype(kind))
+    loss, (losses, lse) = _forward(mf, h, e, right)
+    # e^(-loss) is a share of a sum of at least its own term: a few roundings of 1
+    assert float(losses.min()) >= -2.0 ** -20
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows", (300, 64, 30))
+def test_one_target_for_all_rows(mf, kind, rows):
+    import torch
+
+    h, e, _ = _problem(23, rows, 5000, 128, kind, 2.0)
+    _check(mf, h, e, kind, torch.ones(rows, device="cuda"),
+           targets=torch.full((rows,), 4999, device="cuda", dtype=torch.int32))
+
+
+@pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("scale", (1.0, 1e-6, 4096.0))
 @pytest.mark.parametrize("rows", (200, 30))
 def test_weights_over_a_wide_range(mf, kind, scale, rows):
