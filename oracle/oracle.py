@@ -45,7 +45,7 @@ def build(ref: bool = False) -> None:
     reference sources are present)."""
     targets = ["all"]
     root = reference_root() if ref else None
-    if root:
+    if root and os.path.isdir(os.path.join(root, "src")):
         targets += ["ref", f"REF={root}"]
     subprocess.run(["make", "-s", "-C", HERE, *targets], check=True)
 
