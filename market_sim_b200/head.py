@@ -733,7 +733,9 @@ class DenseLoss:
         args.append(float(temperature))
 
     def _call(self, name, args, rows):
-        if self._index >= 0 and self._torch.cuda.current_device() != self._index:
+        if self._index < 0:
+            raise ValueError(f"the table and its batches lie on {self._device}, not on a GPU")
+        if self._torch.cuda.current_device() != self._index:
             with self._torch.cuda.device(self._device):
                 code = self._launch(name, args, rows)
         else:

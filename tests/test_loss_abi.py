@@ -189,3 +189,20 @@ def test_class_checks_before_the_call():
     with pytest.raises(RuntimeError):
         head.DenseLoss(table, 4, backward=False).cross_entropy_backward(
             hidden, targets, torch.zeros(3), torch.zeros(3))
+
+
+def test_class_refuses_host_memory():
+    """A table and batch that agree with each other, but not on a GPU."""
+    torch = pytest.importorskip("torch")
+    from market_sim_b200 import head
+
+    loss = head.DenseLoss(torch.zeros(40, 16, dtype=torch.float16), 4)
+    launched = []
+    loss._launch = lambda *a: launched.append(a)
+    hidden, targets = torch.zeros(3, 16, dtype=torch.float16), torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="not on a GPU"):
+        loss.cross_entropy(hidden, targets, losses=torch.zeros(3), lse=torch.zeros(3))
+    with pytest.raises(ValueError, match="not on a GPU"):
+        loss.cross_entropy_backward(hidden, targets, torch.zeros(3), torch.zeros(3),
+                                    d_hidden=torch.zeros_like(hidden), embedding_grad=False)
+    assert not launched
