@@ -33,6 +33,9 @@
  * and teacher logits are f32, every sum is held in FP32, and d is rounded once
  * to the 16-bit type for the two gradient products (up to 32 rows: to the sum
  * of two such numbers).
+ * fp16 gradients beyond 65504 become infinite; in d_embedding, what a row of a
+ * small weight adds is good to 2^-25 of the call's largest weight, which fp16
+ * keeps of a hidden element times its row's share of that weight.
  *
  * Arguments are validated as mf_head.h says, before any launch, with these
  * additions: hidden_size is a multiple of 8 up to MF_LOSS_MAX_HIDDEN, rows at
