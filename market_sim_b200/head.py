@@ -193,6 +193,48 @@ def _torch_stream(s):
     return s
 
 
+def _made_on(stream, device, make):
+    """``make()``'s tensor, from the memory of ``stream`` (None: the current
+    stream).  A stream's memory is handed on in that stream's order, so nothing
+    made for one stream is first written, or still in use, on another."""
+    import torch
+
+    if stream is None or device.type != "cuda":
+        return make()
+    with torch.cuda.device(device), torch.cuda.stream(_torch_stream(stream)):
+        return make()
+
+
+class _Workspace:
+    """A workspace that outlives its calls on the streams that use it.
+
+    With a ``stream`` it belongs to that stream.  Without one it is made on the
+    current stream, which the constructor waits for (work queued there may
+    still use the memory, and fills it), and every stream that a call uses it
+    on is made known to the allocator, which then holds the memory back from
+    others until that stream's work is done.
+    """
+
+    def __init__(self, make, device, stream):
+        import torch
+
+        self.tensor = _made_on(stream, device, make)
+        self._seen = None  # a stream was given: its memory, its order
+        if stream is None and device.type == "cuda":
+            self._seen, self._torch = set(), torch
+            with torch.cuda.device(device):
+                if not torch.cuda.is_current_stream_capturing():
+                    torch.cuda.current_stream().synchronize()
+
+    def used_on(self, stream) -> None:
+        """Before a call on ``stream`` (where the constructor got none)."""
+        if self._seen is not None:
+            handle = _stream_handle(stream)
+            if handle not in self._seen:
+                self.tensor.record_stream(_torch_stream(stream))
+                self._seen.add(handle)
+
+
 def _pb(b: Buffer):
     return ctypes.c_void_p(_addr(b) or None), ctypes.c_uint64(_size(b))
 
@@ -657,9 +699,15 @@ class DenseLoss:
     gradient is left out (None) with ``hidden_grad=False`` /
     ``embedding_grad=False``.  With ``backward=False`` only the forward
     workspace is kept.  ``stream`` defaults to the current stream, which must
-    not be the legacy default stream; tensors made on another stream have to
-    be ordered before the call (``Stream.wait_stream``).  Calls of one object
-    share its workspace: they must not overlap on the GPU.
+    not be the legacy default stream; without one the constructor waits for the
+    work queued on the current stream.  The workspace is safe on every stream
+    that calls use, and the object may be dropped while they run.  The caller
+    orders what was made on another stream before the call
+    (``Stream.wait_stream``), keeps its memory until the call is done
+    (``Tensor.record_stream``), as for any tensor used on another stream than
+    its own, and keeps the object for as long as a graph captured from its
+    calls is replayed.  Calls of one object share its workspace: they must not
+    overlap on the GPU.
     """
 
     def __init__(self, embedding, max_rows: int, stream=None, backward: bool = True):
@@ -685,7 +733,9 @@ class DenseLoss:
         kind = kinds[embedding.dtype]
         self._functions = {n: getattr(lib, f"mf_dense_{n}_{kind}")
                            for n in ("xent", "xent_backward", "distill", "distill_backward")}
-        self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=self._device)
+        self._memory = _Workspace(
+            lambda: torch.empty(nbytes, dtype=torch.uint8, device=self._device), self._device, stream)
+        self.workspace = self._memory.tensor
 
     def _on(self):
         """The stream of the call, as torch knows it."""
@@ -747,6 +797,7 @@ class DenseLoss:
         stream = self.stream
         if stream is None:
             stream = self._torch.cuda.current_stream(self._device)
+            self._memory.used_on(stream)
         ws = self.workspace
         return self._functions[name](*args, ws.data_ptr(), self._workspace_bytes, rows,
                                      self.hidden_size, self.vocab, _stream_handle(stream))
