@@ -205,6 +205,19 @@ def _made_on(stream, device, make):
         return make()
 
 
+def _output_on(stream, device, make):
+    """An output for the caller from the memory of ``stream``, which writes it;
+    a caller on another current stream may read it there and drop it."""
+    t = _made_on(stream, device, make)
+    if stream is not None and device.type == "cuda":
+        import torch
+
+        current = torch.cuda.current_stream(device)
+        if current.cuda_stream != _stream_handle(stream):
+            t.record_stream(current)
+    return t
+
+
 class _Workspace:
     """A workspace that outlives its calls on the streams that use it.
 
@@ -535,7 +548,8 @@ class RaggedHead:
 
     ``embedding`` stays resident; each ``__call__`` takes a batch of hidden
     rows and its CSR allowed sets (device tensors) and returns
-    ``(token_ids, scores)`` device tensors.
+    ``(token_ids, scores)`` device tensors.  Without a ``stream`` the
+    constructor waits for the work queued on the current stream.
     """
 
     def __init__(self, embedding, max_rows: int, stream=None):
@@ -544,8 +558,10 @@ class RaggedHead:
         self.embedding = embedding
         self.vocab, self.hidden_size = int(embedding.shape[0]), int(embedding.shape[1])
         self.max_rows = int(max_rows)
-        self.workspace = torch.zeros(head_workspace_bytes(self.max_rows), dtype=torch.uint8,
-                                     device=embedding.device)
+        self._memory = _Workspace(
+            lambda: torch.zeros(head_workspace_bytes(self.max_rows), dtype=torch.uint8,
+                                device=embedding.device), embedding.device, stream)
+        self.workspace = self._memory.tensor
         self.stream = stream
 
     def __call__(self, hidden, offsets, ids, out_ids=None, out_scores=None):
@@ -554,12 +570,18 @@ class RaggedHead:
         rows = int(hidden.shape[0])
         if rows > self.max_rows:
             raise ValueError(f"batch of {rows} rows exceeds max_rows={self.max_rows}")
+        device = hidden.device
         if out_ids is None:
-            out_ids = torch.empty(rows, dtype=torch.int32, device=hidden.device)
+            out_ids = _output_on(self.stream, device,
+                                 lambda: torch.empty(rows, dtype=torch.int32, device=device))
         if out_scores is None:
-            out_scores = torch.empty(rows, dtype=torch.float32, device=hidden.device)
+            out_scores = _output_on(self.stream, device,
+                                    lambda: torch.empty(rows, dtype=torch.float32, device=device))
         ws = self.workspace[: head_workspace_bytes(rows)]
-        stream = self.stream if self.stream is not None else torch.cuda.current_stream()
+        stream = self.stream
+        if stream is None:
+            stream = torch.cuda.current_stream()
+            self._memory.used_on(stream)
         st = restricted_output_head_csr_f16(hidden, self.embedding, offsets, ids, out_ids,
                                             out_scores, ws, rows, self.hidden_size, self.vocab,
                                             stream)
