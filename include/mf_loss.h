@@ -56,6 +56,12 @@
  * the gradients: its d_hidden row is 0 and what its hidden row holds (NaN
  * included) does not reach d_embedding.  lse is written for every row.
  * Elsewhere a score of NaN or +inf gives its row a NaN loss and NaN gradients.
+ * A score of -inf (a table row masked by a bias column) has p = 0: it adds
+ * nothing to lse, and a loss that asks for it is +inf; so do scores over T below
+ * -1.5e9 beside others that are not.  A row whose scores are all -inf has lse
+ * -inf and a NaN loss.  Products with an infinite table element make d_hidden
+ * NaN as 0 times it is; a masked table that trains holds a large negative
+ * number, whose products with 0 are 0.
  *
  * Every wait inside the kernels is bounded (100 ms); one that runs out gives
  * NaN in the outputs it covers, and the context stays usable.

@@ -71,6 +71,10 @@ constexpr float kLn2 = 0.6931471805599453f;
 // 2.2e-9 to 2.7e-9 at 0.5, 4.2e-9 to 4.8e-9 at 0.9, with a standard deviation
 // of 1.3e-7 to 4.5e-7 of the score.  Scores are scaled by 1 + K 2^-29.
 constexpr float kLostPerProduct = 1.862645149230957e-9f;
+// A maximum below this (units of ln 2) is that of masked columns: -inf, whose
+// exponential relative to itself is NaN, or a score whose rounding is more than
+// an exponential's range.  Their exponentials are taken as they are, that is 0.
+constexpr float kMasked = -2147483648.f;
 
 template <typename T>
 struct Type;
@@ -887,11 +891,12 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
                   mx[e] = fmaxf(mx[e], __uint_as_float(r[j + e]));
             const float m =
                 fmaxf(run_m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c2);
-            float2 l[2] = {make_float2(run_l * exp2_approx(run_m - m), 0.f), make_float2(0.f, 0.f)};
+            const float from = m < kMasked ? 0.f : m;
+            float2 l[2] = {make_float2(run_l * exp2_approx(run_m - from), 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
             for (int j = 0; j < 64; j += 2) {
               const float2 x = fma2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])),
-                                    make_float2(c2, c2), make_float2(-m, -m));
+                                    make_float2(c2, c2), make_float2(-from, -from));
               l[(j >> 1) & 1] =
                   add2(l[(j >> 1) & 1], make_float2(exp2_approx(x.x), exp2_approx(x.y)));
             }
@@ -1116,6 +1121,7 @@ __device__ __forceinline__ float no_target_loss(uint32_t target) {
 // (scores of 1e8).
 __device__ __forceinline__ float put_target(float& m, float& l, float dot, float c2,
                                             float score) {
+  if (m == -INFINITY) return __uint_as_float(0x7FC00000u);  // no score but -inf: lse stays so
   float rest = l - exp2_approx(fmaf(dot, c2, -m));
   if (rest < 0.f) rest = 0.f;  // rounding; a NaN stays
   const float above = fmaf(score, kLog2e, -m);
@@ -1342,7 +1348,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         mx[j] = warp_max(mx[j]) * p.c2;
-        l[j] = mx[j] > -INFINITY ? mx[j] : 0.f;  // a warp without a table row sums zeros
+        l[j] = mx[j] < kMasked ? 0.f : mx[j];  // a warp without a table row sums zeros
       }
       float sum[16] = {};
       for (uint32_t t = 0; t < tiles; ++t) {
