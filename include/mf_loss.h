@@ -26,6 +26,8 @@
  * Scores come from the tensor cores: relative to a score, an error of about
  * 1e-9 to 3e-9 a product of its width remains.  The target's own score, and in
  * batches of up to 64 rows a teacher set's, are summed with rounding to nearest.
+ * The target's gradient takes p - 1 from that score's distance to lse, an f32
+ * number: it is good to 2^-24 |lse|.
  * Scores over T beyond 1e9 in magnitude may give infinities.
  *
  * Types: _f16 takes fp16 and _bf16 bfloat16 hidden rows and table; gradients

@@ -196,6 +196,7 @@ __device__ __forceinline__ int32_t first_entry(const Wanted& w, uint32_t r, uint
 struct RowGrad {  // one row's factors of d
   float coef;     // d16 = (p - q) * coef
   float scale;    // d_hidden = (d16 . E) * scale
+  float target;   // cross entropy: d16 at the target
 };
 
 __device__ __forceinline__ float row_weight(const Wanted& w, const float* grad, uint32_t r,
@@ -205,13 +206,50 @@ __device__ __forceinline__ float row_weight(const Wanted& w, const float* grad, 
   return stat_empty(s) || stat_invalid(s) ? 0.f : grad[r] / w.inv_t;
 }
 
+__device__ __forceinline__ float min_nan(float a, float b) {  // NaN stays
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// hidden row . table row by one warp on the FP32 pipes, rounding to nearest.
+template <typename T>
+__device__ __forceinline__ float warp_score(const T* a, const T* b, uint32_t width) {
+  float s0 = 0.f, s1 = 0.f;
+  for (uint32_t c = (threadIdx.x & 31) * 8; c < width; c += 256) {
+    const uint4 x = ld_v4(a + c), y = ld_v4(b + c);
+    const T *xs = reinterpret_cast<const T*>(&x), *ys = reinterpret_cast<const T*>(&y);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      s0 = fmaf(Type<T>::to(xs[j]), Type<T>::to(ys[j]), s0);
+      s1 = fmaf(Type<T>::to(xs[j + 1]), Type<T>::to(ys[j + 1]), s1);
+    }
+  }
+  float s = s0 + s1;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+  return s;
+}
+
+// p - 1 of a row's target, by one warp.  lse holds the target's score as
+// warp_score gives it (put_target), so that is the score here too: with the
+// tensor core's, which loses up to 2e-6 of a score of 576 products, a target with
+// 1 - p = 1e-5 at a score of 30 had a gradient several times too large, or none.
+// What is left is lse's own rounding, 2^-24 |lse|.
+template <typename T>
+__device__ __forceinline__ float target_short(const T* hidden, const T* table, uint32_t r,
+                                              uint32_t target, uint32_t width, float lse) {
+  const float s = warp_score(hidden + (uint64_t)r * width, table + (uint64_t)target * width, width);
+  return min_nan(expm1f(s - lse), 0.f);
+}
+
 // Row factors and the copy of the hidden rows that d_embedding is made of.
 // Every block finds the largest weight by itself (8 bytes a row from L2, many
 // in flight); then a warp per row.
 template <typename T>
-__global__ void __launch_bounds__(kSetupThreads)
-setup_kernel(Wanted w, const float* grad, const T* hidden, T* scaled, RowGrad* rg, float* gmax_out,
-             uint32_t rows, uint32_t width, uint32_t vocab) {
+__global__ void __launch_bounds__(kSetupThreads, 1)
+setup_kernel(Wanted w, const float* grad, const T* hidden, const T* table, const float* lse, T* scaled,
+             RowGrad* rg, float* gmax_out, uint32_t rows, uint32_t width, uint32_t vocab) {
   __shared__ float s_max[kSetupThreads / 32];
   pdl_wait();
   pdl_trigger();
@@ -242,7 +280,10 @@ setup_kernel(Wanted w, const float* grad, const T* hidden, T* scaled, RowGrad* r
       if (fabsf(mant) == 0.5f) mant *= 2.f, e -= 1;
       two_e = ldexpf(1.f, e);
     }
-    if (lane == 0) rg[r] = RowGrad{mant * Type<T>::kScale, g * two_e / Type<T>::kScale};
+    const float coef = mant * Type<T>::kScale;
+    const float miss = w.targets && wr != 0.f
+                           ? target_short(hidden, table, r, w.targets[r], width, lse[r]) : 0.f;
+    if (lane == 0) rg[r] = RowGrad{coef, g * two_e / Type<T>::kScale, miss * coef};
     for (uint32_t c = lane * 8; c < width; c += 256) {
       uint4 x = make_uint4(0u, 0u, 0u, 0u);
       if (wr != 0.f) {
@@ -258,11 +299,6 @@ setup_kernel(Wanted w, const float* grad, const T* hidden, T* scaled, RowGrad* r
 
 // ---- the tile engine ----------------------------------------------------
 
-__device__ __forceinline__ float min_nan(float a, float b) {  // NaN stays
-  float d;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -796,6 +832,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
     uint32_t cur_m = 0xFFFFFFFFu, row = 0, slot = 0;
     bool live = false;
     float tlse2 = 0.f, run_m = -INFINITY, run_l = 0.f, dot = 0.f, z2 = 0.f, coef = 0.f;
+    float at_target = 0.f;         // d of cross entropy there
     float e2 = 0.f;                // log2 |coef| - z2
     // of the packed pairs of d; p is at most 1, however far the errors of scores
     // of 1e6 lie beyond lse
@@ -835,6 +872,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
             run_l = dot = 0.f;
           } else if (live) {
             coef = p.rg[row].coef;
+            if (!kDistill) at_target = p.rg[row].target;
             z2 = p.lse[row] * kLog2e;
             e2 = log2f(fabsf(coef)) - z2;
             most = Type<T>::pack(fabsf(coef), fabsf(coef));
@@ -931,14 +969,22 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
                 store_v8(out + j, v);
               }
             }
-            while (__any_sync(0xFFFFFFFFu, cur.id[0] - col < 64u)) {
-              const float s = pick64(r, cur.id[0] - col);
+            if constexpr (!kDistill) {  // over the element just stored
               const bool mine = cur.id[0] - col < 64u;
-              if (mine) {  // p - q in FP32, over the element just stored
-                const float x = min_nan(exp2_approx(fmaf(s, c2, -z2)), 1.f) - cur.weight(t2, tlse2);
-                out[cur.id[0] - col] = Type<T>::from(x * coef);
+              if (__any_sync(0xFFFFFFFFu, mine)) {
+                if (mine) out[cur.id[0] - col] = Type<T>::from(dead ? nan : at_target);
+                __syncwarp();
               }
-              cur.drop(w, mine);
+            } else {
+              while (__any_sync(0xFFFFFFFFu, cur.id[0] - col < 64u)) {
+                const float s = pick64(r, cur.id[0] - col);
+                const bool mine = cur.id[0] - col < 64u;
+                if (mine) {  // p - q in FP32
+                  const float x = min_nan(exp2_approx(fmaf(s, c2, -z2)), 1.f) - cur.weight(t2, tlse2);
+                  out[cur.id[0] - col] = Type<T>::from(x * coef);
+                }
+                cur.drop(w, mine);
+              }
             }
           }
         }
@@ -1036,25 +1082,6 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
                  : "memory");
 }
 
-// hidden row . table row by one warp on the FP32 pipes, rounding to nearest.
-template <typename T>
-__device__ __forceinline__ float warp_score(const T* a, const T* b, uint32_t width) {
-  float s0 = 0.f, s1 = 0.f;
-  for (uint32_t c = (threadIdx.x & 31) * 8; c < width; c += 256) {
-    const uint4 x = ld_v4(a + c), y = ld_v4(b + c);
-    const T *xs = reinterpret_cast<const T*>(&x), *ys = reinterpret_cast<const T*>(&y);
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      s0 = fmaf(Type<T>::to(xs[j]), Type<T>::to(ys[j]), s0);
-      s1 = fmaf(Type<T>::to(xs[j + 1]), Type<T>::to(ys[j + 1]), s1);
-    }
-  }
-  float s = s0 + s1;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-  return s;
-}
-
 // Joins the (m, l) of the lanes of a warp.
 __device__ __forceinline__ void warp_join(float& m, float& l) {
 #pragma unroll
@@ -1134,6 +1161,12 @@ __device__ __forceinline__ float put_target(float& m, float& l, float dot, float
   return (log2f(l) - above) * kLn2;
 }
 
+// A sure row's lse is score + loss, rounded once: the gradient takes p - 1 from
+// the distance of the two.
+__device__ __forceinline__ float row_lse(float m, float l, float score, float loss) {
+  return loss < 1.f ? score + loss : (m + log2f(l)) * kLn2;
+}
+
 // One warp per row joins the walks' partial sums.  Row tile m's n_tiles tiles
 // lie in the ranges of a few consecutive pairs.  A target's score is computed
 // again on the FP32 pipes and takes the place of the tensor core's in the sum:
@@ -1161,7 +1194,7 @@ __global__ void merge_kernel(Wanted w, const T* hidden, const T* table, uint32_t
   if (lane) return;
   float loss = no_target_loss(target);
   if (target < vocab) loss = put_target(m, l, dot, c2, score);
-  const float z = (m + log2f(l)) * kLn2;
+  const float z = target < vocab ? row_lse(m, l, score, loss) : (m + log2f(l)) * kLn2;
   lse[r] = z;
   losses[r] = w.targets ? loss : set_loss(w, w.stat[r], z, dot);
 }
@@ -1433,7 +1466,7 @@ struct FewGradParams {
   uint32_t width, w_chunks;
   uint32_t vocab, range;    // table rows per CTA, a multiple of 32
   float score_scale;
-  const void* hidden;
+  const void *hidden, *table;
   const float* grad;
   const float* lse;
   RowGrad* rg;
@@ -1472,6 +1505,7 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
   __shared__ uint32_t tmem_at, abort_word, loads;
   __shared__ float s_coef[kFewGradRows], s_z2[kFewGradRows], s_tlse[kFewGradRows];
   __shared__ uint32_t s_target[kFewGradRows];
+  __shared__ float s_short[kFewGradRows];  // p - 1 of the targets in the CTA's range
   __shared__ int32_t s_at[kFewGradRows], s_end[kFewGradRows];
   __shared__ float s_gmax;
   unsigned char* sm = reinterpret_cast<unsigned char*>(
@@ -1530,7 +1564,7 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
     s_z2[lane] = lane < p.rows ? p.lse[lane] * kLog2e : 0.f;
     s_target[lane] = w.targets && lane < p.rows && coef != 0.f ? w.targets[lane] : kInvalid;
     if (lane == 0) s_gmax = g;
-    if (blockIdx.x == 0 && lane < p.rows) p.rg[lane] = RowGrad{coef, g / Type<T>::kScale};
+    if (blockIdx.x == 0 && lane < p.rows) p.rg[lane] = RowGrad{coef, g / Type<T>::kScale, 0.f};
     if (kDistill) {
       s_at[lane] = s_end[lane] = 0;
       if (coef != 0.f) {
@@ -1541,6 +1575,14 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
     }
   }
   __syncthreads();
+  if (!kDistill) {
+    for (uint32_t r = warp; r < p.rows; r += kFewGradThreads / 32) {
+      if (s_target[r] - v0 >= count) continue;
+      const float x = target_short(static_cast<const T*>(p.hidden), static_cast<const T*>(p.table), r,
+                                   s_target[r], p.width, p.lse[r]);
+      if (lane == 0) s_short[r] = x;
+    }
+  }
   // hidden rows as 64-wide chunks of 128-byte rows (128-byte swizzle); rows that
   // take no part are zero
   for (uint32_t i = threadIdx.x; i < p.w_chunks * p.n * 8; i += kFewGradThreads) {
@@ -1683,7 +1725,7 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
             const float coef = s_coef[n];
             float d = min_nan(exp2_approx(fmaf(__uint_as_float(r[j + e]), c2, -s_z2[n])), 1.f);
             if (kDistill) d -= s_q[n * 128 + row];
-            else if (s_target[n] == v) d -= 1.f;
+            else if (s_target[n] == v) d = s_short[n];
             x[e] = coef == 0.f || !in ? 0.f : (dead ? nan : d * coef);
           }
           hi[j / 2] = Type<T>::pack(x[0], x[1]);
@@ -1833,7 +1875,7 @@ few_rows_join_kernel(Wanted w, const T* hidden, const T* table, uint32_t width, 
   if (lane) return;
   float loss = no_target_loss(target);
   if (target < vocab) loss = put_target(m, l, tensor, c2, dot);
-  const float z = (m + log2f(l)) * kLn2;
+  const float z = target < vocab ? row_lse(m, l, dot, loss) : (m + log2f(l)) * kLn2;
   lse[r] = z;
   losses[r] = w.targets ? loss : set_loss(w, st, z, dot);
 }
@@ -2411,6 +2453,7 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
     f.range = few.range;
     f.score_scale = 1.f + (float)width * kLostPerProduct;
     f.hidden = hidden.p;
+    f.table = embedding.p;
     f.grad = static_cast<const float*>(grad.p);
     f.lse = static_cast<const float*>(lse.p);
     f.rg = rg;
@@ -2429,8 +2472,9 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
       !make_map<T>(&maps.scaled_n, scaled, rows, width, width, 32, kBK))
     return fail(MF_CUDA_RUNTIME_FAILURE);
   err = launch_after(setup_kernel<T>, rows < 32 * 148 ? (rows + 31) / 32 : 148, kSetupThreads, 0, s, w,
-                     static_cast<const float*>(grad.p), static_cast<const T*>(hidden.p), scaled,
-                     rg, gmax, (uint32_t)rows, (uint32_t)width, (uint32_t)vocab);
+                     static_cast<const float*>(grad.p), static_cast<const T*>(hidden.p),
+                     static_cast<const T*>(embedding.p), static_cast<const float*>(lse.p), scaled, rg,
+                     gmax, (uint32_t)rows, (uint32_t)width, (uint32_t)vocab);
   if (err != cudaSuccess) return launched(err);
 
   Params p = base_params(rows, width, vocab);
