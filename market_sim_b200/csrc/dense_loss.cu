@@ -115,6 +115,15 @@ struct Type<__nv_bfloat16> {
   }
 };
 
+// A teacher's distribution over its set: q = exp((t - top) / T) * share.  The
+// largest logit and 1 / (sum of the exponentials) stay apart: in one FP32 number
+// top / T + log sum, logits around 10,000 leave q's sum off by 5e-4.
+struct Teacher {
+  float top;       // of the logits; -inf: no entry that counts, NaN: invalid
+  float share;
+  float entropy;   // sum q log q
+};
+
 // What a row wants: one target, or a teacher's set.
 struct Wanted {
   const uint32_t* targets;   // cross entropy
@@ -122,12 +131,11 @@ struct Wanted {
   const int32_t* ids;
   const float* logits;
   float inv_t;               // 1 / temperature (1 for cross entropy)
-  float2* stat;              // distillation: {log sum exp of t / T, sum q log q}
+  Teacher* stat;             // distillation
 };
 
-// stat.x of a row without entries, and of an invalid row
-__device__ __forceinline__ bool stat_empty(float2 s) { return s.x == -INFINITY; }
-__device__ __forceinline__ bool stat_invalid(float2 s) { return s.x != s.x; }
+__device__ __forceinline__ bool stat_empty(const Teacher& s) { return s.top == -INFINITY; }
+__device__ __forceinline__ bool stat_invalid(const Teacher& s) { return s.top != s.top; }
 
 // Of one row over one walk through the vocabulary, half of every tile's
 // columns: the largest score in units of ln 2, the sum of exp relative to it,
@@ -136,39 +144,37 @@ struct __align__(16) Partial {
   float m, l, dot, unused;
 };
 
-// The teacher's normaliser and entropy of row r, by one warp.
-__device__ __forceinline__ float2 teacher_stat(const Wanted& w, uint32_t r, uint32_t entries,
-                                               uint32_t vocab) {
+// The teacher's distribution in row r, by one warp.
+__device__ __forceinline__ Teacher teacher_stat(const Wanted& w, uint32_t r, uint32_t entries,
+                                                uint32_t vocab) {
   const uint32_t lane = threadIdx.x & 31;
   const int32_t a = w.offsets[r], b = w.offsets[r + 1];
   bool bad = a < 0 || b < a || (uint32_t)b > entries;
-  float m = -INFINITY;
+  Teacher st{-INFINITY, 0.f, 0.f};
   if (!bad) {
     for (int32_t k = a + (int32_t)lane; k < b; k += 32) {
       const int32_t id = w.ids[k];
       const float t = w.logits[k];
       bad |= id < 0 || (uint32_t)id >= vocab || (k > a && w.ids[k - 1] >= id) || t != t ||
              t == INFINITY;
-      m = fmaxf(m, t * w.inv_t);
+      st.top = fmaxf(st.top, t);
     }
   }
   bad = __any_sync(0xFFFFFFFFu, bad);
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-  float2 st = make_float2(-INFINITY, 0.f);
+  for (int o = 16; o; o >>= 1) st.top = fmaxf(st.top, __shfl_xor_sync(0xFFFFFFFFu, st.top, o));
   if (bad) {
-    st.x = __uint_as_float(0x7FC00000u);
-  } else if (m > -INFINITY) {
+    st.top = __uint_as_float(0x7FC00000u);
+  } else if (st.top > -INFINITY) {
     float l = 0.f;
-    for (int32_t k = a + (int32_t)lane; k < b; k += 32) l += expf(w.logits[k] * w.inv_t - m);
+    for (int32_t k = a + (int32_t)lane; k < b; k += 32) l += expf((w.logits[k] - st.top) * w.inv_t);
     for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
-    st.x = m + logf(l);
-    float ent = 0.f;
+    st.share = 1.f / l;
+    const float log_l = logf(l);
     for (int32_t k = a + (int32_t)lane; k < b; k += 32) {
-      const float lq = w.logits[k] * w.inv_t - st.x, q = expf(lq);
-      if (q > 0.f) ent += q * lq;
+      const float x = (w.logits[k] - st.top) * w.inv_t, q = expf(x) * st.share;
+      if (q > 0.f) st.entropy += q * (x - log_l);
     }
-    for (int o = 16; o; o >>= 1) ent += __shfl_xor_sync(0xFFFFFFFFu, ent, o);
-    st.y = ent;
+    for (int o = 16; o; o >>= 1) st.entropy += __shfl_xor_sync(0xFFFFFFFFu, st.entropy, o);
   }
   return st;
 }
@@ -178,7 +184,7 @@ __global__ void teacher_kernel(Wanted w, uint32_t rows, uint32_t entries, uint32
   pdl_trigger();
   for (uint32_t r = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; r < rows;
        r += (gridDim.x * blockDim.x) >> 5) {
-    const float2 st = teacher_stat(w, r, entries, vocab);
+    const Teacher st = teacher_stat(w, r, entries, vocab);
     if ((threadIdx.x & 31) == 0) w.stat[r] = st;
   }
 }
@@ -202,7 +208,7 @@ struct RowGrad {  // one row's factors of d
 __device__ __forceinline__ float row_weight(const Wanted& w, const float* grad, uint32_t r,
                                             uint32_t vocab) {
   if (w.targets) return w.targets[r] < vocab ? grad[r] : 0.f;
-  const float2 s = w.stat[r];
+  const Teacher s = w.stat[r];
   return stat_empty(s) || stat_invalid(s) ? 0.f : grad[r] / w.inv_t;
 }
 
@@ -592,9 +598,9 @@ struct Cursor {
       while (__any_sync(0xFFFFFFFFu, id[0] < v)) drop(w, id[0] < v);
     }
   }
-  // The weight of the first entry; `tlse2` in units of ln 2.
-  __device__ __forceinline__ float weight(float t2, float tlse2) const {
-    if constexpr (kDistill) return exp2_approx(fmaf(t[0], t2, -tlse2));
+  // The weight of the first entry; t2: 1 / T in units of ln 2.
+  __device__ __forceinline__ float weight(float t2, float top, float share) const {
+    if constexpr (kDistill) return exp2_approx((t[0] - top) * t2) * share;
     return 1.f;
   }
 };
@@ -831,7 +837,8 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
     // state of the row this thread holds while it walks along score tiles
     uint32_t cur_m = 0xFFFFFFFFu, row = 0, slot = 0;
     bool live = false;
-    float tlse2 = 0.f, run_m = -INFINITY, run_l = 0.f, dot = 0.f, z2 = 0.f, coef = 0.f;
+    float top = 0.f, share = 0.f;  // of the teacher
+    float run_m = -INFINITY, run_l = 0.f, dot = 0.f, z2 = 0.f, coef = 0.f;
     float at_target = 0.f;         // d of cross entropy there
     float e2 = 0.f;                // log2 |coef| - z2
     // of the packed pairs of d; p is at most 1, however far the errors of scores
@@ -881,9 +888,10 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
             live = coef != 0.f;
           }
           if (kDistill && live) {
-            const float2 st = w.stat[row];
+            const Teacher st = w.stat[row];
             live = !stat_empty(st) && !stat_invalid(st);
-            tlse2 = st.x * kLog2e;
+            top = st.top;
+            share = st.share;
           }
           cur.start(w, row, v, live);
           cur.fill(w);
@@ -945,7 +953,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
               const float s = pick64(r, cur.id[0] - col);
               const bool mine = cur.id[0] - col < 64u;
               if (mine) {
-                const float q = cur.weight(t2, tlse2);
+                const float q = cur.weight(t2, top, share);
                 if (!kDistill) dot = s;
                 else if (q > 0.f) dot = fmaf(q, s * inv_t, dot);
               }
@@ -980,7 +988,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
                 const float s = pick64(r, cur.id[0] - col);
                 const bool mine = cur.id[0] - col < 64u;
                 if (mine) {  // p - q in FP32
-                  const float x = min_nan(exp2_approx(fmaf(s, c2, -z2)), 1.f) - cur.weight(t2, tlse2);
+                  const float x = min_nan(exp2_approx(fmaf(s, c2, -z2)), 1.f) - cur.weight(t2, top, share);
                   out[cur.id[0] - col] = Type<T>::from(x * coef);
                 }
                 cur.drop(w, mine);
@@ -1131,9 +1139,9 @@ __device__ __forceinline__ void join_slots(const Partial* part, uint32_t slots, 
   for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
 }
 
-__device__ __forceinline__ float set_loss(const Wanted& w, float2 s, float z, float dot) {
+__device__ __forceinline__ float set_loss(const Wanted& w, const Teacher& s, float z, float dot) {
   const float t = 1.f / w.inv_t;
-  return stat_empty(s) ? 0.f : (stat_invalid(s) ? s.x : t * t * (s.y + (z - dot)));
+  return stat_empty(s) ? 0.f : (stat_invalid(s) ? s.top : t * t * (s.entropy + (z - dot)));
 }
 // Of a row without a target: ignored or invalid.
 __device__ __forceinline__ float no_target_loss(uint32_t target) {
@@ -1503,7 +1511,8 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
   // table chunks full, table free, scores full, d full, dE full / empty [2], dH done
   __shared__ uint64_t bars[kFewGradChunks + 8];
   __shared__ uint32_t tmem_at, abort_word, loads;
-  __shared__ float s_coef[kFewGradRows], s_z2[kFewGradRows], s_tlse[kFewGradRows];
+  __shared__ float s_coef[kFewGradRows], s_z2[kFewGradRows];
+  __shared__ float s_top[kFewGradRows], s_share[kFewGradRows];
   __shared__ uint32_t s_target[kFewGradRows];
   __shared__ float s_short[kFewGradRows];  // p - 1 of the targets in the CTA's range
   __shared__ int32_t s_at[kFewGradRows], s_end[kFewGradRows];
@@ -1568,7 +1577,8 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
     if (kDistill) {
       s_at[lane] = s_end[lane] = 0;
       if (coef != 0.f) {
-        s_tlse[lane] = w.stat[lane].x * kLog2e;
+        s_top[lane] = w.stat[lane].top;
+        s_share[lane] = w.stat[lane].share;
         s_at[lane] = first_entry(w, lane, v0);
         s_end[lane] = w.offsets[lane + 1];
       }
@@ -1701,7 +1711,7 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
             if (k + (int32_t)lane < end) id = (uint32_t)w.ids[k + lane];
             const bool mine = id - first < n_in;  // ascending: entries before `first` are behind k
             if (mine)
-              s_q[r * 128 + (id - first)] = exp2_approx(fmaf(w.logits[k + lane], t2, -s_tlse[r]));
+              s_q[r * 128 + (id - first)] = exp2_approx((w.logits[k + lane] - s_top[r]) * t2) * s_share[r];
             const uint32_t taken = __popc(__ballot_sync(0xFFFFFFFFu, mine));
             k += (int32_t)taken;
             if (taken < 32) break;
@@ -1820,7 +1830,7 @@ few_rows_join_kernel(Wanted w, const T* hidden, const T* table, uint32_t width, 
   const uint32_t r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const T* row = hidden + (uint64_t)r * width;
   const uint32_t target = w.targets ? w.targets[r] : kInvalid;
-  float2 st = make_float2(-INFINITY, 0.f);
+  Teacher st{-INFINITY, 0.f, 0.f};
   float dot = 0.f;  // of the row's wanted scores, as weighted
   if (target < vocab) {
     if (warp == 0) dot = warp_score(row, table + (uint64_t)target * width, width);
@@ -1835,7 +1845,7 @@ few_rows_join_kernel(Wanted w, const T* hidden, const T* table, uint32_t width, 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int32_t i = k + j * kWarps < end ? k + j * kWarps : k;
-          q[j] = k + j * kWarps < end ? expf(w.logits[i] * w.inv_t - st.x) : 0.f;
+          q[j] = k + j * kWarps < end ? expf((w.logits[i] - st.top) * w.inv_t) * st.share : 0.f;
           at[j] = table + (uint64_t)w.ids[i] * width;
         }
         for (uint32_t c = lane * 8; c < width; c += 256) {  // four rows in flight
@@ -1968,7 +1978,7 @@ struct ForwardPlan {
     // the few-rows kernel: one slot per CTA
     if (rows <= kFewRows && slots < kMaxPairs) slots = kMaxPairs;
     stat = 0;
-    partial = round_up(rows * sizeof(float2), 256);
+    partial = round_up(rows * sizeof(Teacher), 256);
     bytes = round_up(partial + 2 * slots * rows * sizeof(Partial), 256);
   }
 };
@@ -2018,7 +2028,7 @@ struct BackwardPlan {
     if (sets > pieces) sets = pieces;
     if (sets < 1) sets = 1;
     stat = 0;
-    rg = round_up(stat + rows * sizeof(float2), 256);
+    rg = round_up(stat + rows * sizeof(Teacher), 256);
     gmax = round_up(rg + rows * sizeof(RowGrad), 256);
     scaled = gmax + 256;
     planes = round_up(scaled + rows * width * 2, 256);
@@ -2345,7 +2355,7 @@ mf_status forward(Span hidden, Span embedding, Span targets, Span ids, Span logi
     w.offsets = static_cast<const int32_t*>(targets.p);
     w.ids = static_cast<const int32_t*>(ids.p);
     w.logits = static_cast<const float*>(logits.p);
-    w.stat = reinterpret_cast<float2*>(ws + plan.stat);
+    w.stat = reinterpret_cast<Teacher*>(ws + plan.stat);
   } else {
     w.targets = static_cast<const uint32_t*>(targets.p);
   }
@@ -2433,7 +2443,7 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
     w.offsets = static_cast<const int32_t*>(targets.p);
     w.ids = static_cast<const int32_t*>(ids.p);
     w.logits = static_cast<const float*>(logits.p);
-    w.stat = reinterpret_cast<float2*>(ws + plan.stat);
+    w.stat = reinterpret_cast<Teacher*>(ws + plan.stat);
     err = teacher_launch(w, rows, ids.bytes / 4, vocab, s);
     if (err != cudaSuccess) return launched(err);
   } else {
