@@ -2034,7 +2034,7 @@ struct BackwardPlan {
     planes = round_up(scaled + rows * width * 2, 256);
     uint64_t sums = sets * set;
     const uint64_t few = 2 * kMaxPairs * rows * width * 4;  // few_rows_grad_kernel's planes
-    if (rows <= kFewGradRows && sums < few) sums = few;
+    if (rows <= kFewGradRows && width <= kFewGradChunks * kBK && sums < few) sums = few;
     piece[0] = round_up(planes + sums, 256);
     const uint64_t one = round_up(rows * cols * 2, 256);
     piece[1] = piece[0] + (pieces > 1 ? one : 0);

@@ -206,3 +206,21 @@ def test_class_refuses_host_memory():
         loss.cross_entropy_backward(hidden, targets, torch.zeros(3), torch.zeros(3),
                                     d_hidden=torch.zeros_like(hidden), embedding_grad=False)
     assert not launched
+
+
+def test_workspace_of_few_wide_rows(lib):
+    """Up to 32 rows keep a plane of sums for each CTA, where their kernel takes the
+    width (up to 640): the sums stay within 128 MiB, or 4 bytes an element."""
+    b = lib.mf_dense_loss_backward_workspace_bytes
+    for width in (8, 576, 640, 648, 1024, 4096, 8192):
+        for rows in (1, 31, 32, 33, 64, 300):
+            for vocab in (1, 1000, 49152, 1 << 24):
+                whole = 2 * rows * ((vocab + 255) // 256 * 256)  # d of all the vocabulary
+                pieces = min(whole, 2 * (128 << 20))
+                sums = max(128 << 20, rows * width * 4)
+                assert b(rows, width, vocab) <= pieces + sums + rows * width * 2 + 4096 + rows * 24, \
+                    (width, rows, vocab)
+    # no planes above 640: 32 rows need what the tile engine needs for one row more than 31
+    assert b(32, 640, 1000) > 148 * 32 * 640 * 4
+    assert b(32, 648, 1000) < 148 * 32 * 648 * 4 // 4
+    assert b(32, 8192, 1000) < 32 << 20
