@@ -24,10 +24,10 @@
  * its type holds; larger batches go in slices whose gradients the caller adds.
  *
  * Scores come from the tensor cores: relative to a score, an error of about
- * 1e-9 to 3e-9 a product of its width remains.  The target's own score, and in
- * batches of up to 64 rows a teacher set's, are summed with rounding to nearest.
- * The target's gradient takes p - 1 from that score's distance to lse, an f32
- * number: it is good to 2^-24 |lse|.
+ * 1e-9 to 3e-9 a product of its width remains.  A target's own score is summed
+ * with rounding to nearest.  A call's losses, lse and gradients are made of the
+ * same scores, so where p and q are nearly equal, p - q is good to lse's
+ * rounding to f32, 2^-24 |lse|, and the loss to a few 2^-24.
  * Scores over T beyond 1e9 in magnitude may give infinities.
  *
  * Types: _f16 takes fp16 and _bf16 bfloat16 hidden rows and table; gradients

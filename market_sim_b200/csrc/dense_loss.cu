@@ -62,8 +62,8 @@ constexpr uint32_t kTmemCols = 512;
 constexpr int kSetupThreads = 1024;
 constexpr uint32_t kMaxPairs = 74;             // pairs of the persistent grid
 constexpr uint64_t kPieceBytes = 128ull << 20; // one piece of d
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = (float)(1.4426950408889634 - (double)kLog2e);
+constexpr float kLn2 = 0.6931471805599453f, kLn2Low = (float)(0.6931471805599453 - (double)kLn2);
 // The tensor core's additions drop the bits that fall below the sum's last
 // place, so a score of K products comes out too small.  Measured, relative to
 // the score and per product, for K from 128 to 2,048: 1.1e-9 where the products
@@ -138,11 +138,32 @@ __device__ __forceinline__ bool stat_empty(const Teacher& s) { return s.top == -
 __device__ __forceinline__ bool stat_invalid(const Teacher& s) { return s.top != s.top; }
 
 // Of one row over one walk through the vocabulary, half of every tile's
-// columns: the largest score in units of ln 2, the sum of exp relative to it,
-// and the sum of q s / T, or the target's score as the tensor core gave it.
+// columns: the largest score m in units of ln 2 and the sum of exp relative to
+// it.  Distillation: the sum of q (s / T - m) and that of q; a loss is a small
+// difference of the two where teacher and student are sure of the same id, so
+// it is never made of numbers of the scores' size.  Cross entropy: the target's
+// score as the tensor core gave it, and 0.
 struct __align__(16) Partial {
-  float m, l, dot, unused;
+  float m, l, dot, q;
 };
+
+// What a sum with the maximum m is relative to: masked columns have no part in it.
+__device__ __forceinline__ float base_of(float m) { return m < kMasked ? 0.f : m; }
+
+// lse = (m + log2 l) ln 2, rounded once: backward takes p from its distance to
+// the scores.
+__device__ __forceinline__ float lse_of(float m, float l) {
+  const float g = log2f(l), z = m + g;
+  if (!(fabsf(z) < INFINITY)) return z;
+  const float low = fabsf(m) > fabsf(g) ? (m - z) + g : (g - z) + m;
+  return fmaf(z, kLn2, fmaf(z, kLn2Low, low * kLn2));
+}
+
+// The same way back: lse in units of ln 2 and what that rounds off.
+__device__ __forceinline__ float2 lse_units(float lse) {
+  const float z = lse * kLog2e;
+  return make_float2(z, fmaf(lse, kLog2e, -z) + lse * kLog2eLow);
+}
 
 // The teacher's distribution in row r, by one warp.
 __device__ __forceinline__ Teacher teacher_stat(const Wanted& w, uint32_t r, uint32_t entries,
@@ -830,15 +851,16 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
     const uint32_t leader_acc_empty1 = mapa(acc_empty(1), 0);
     const float nan = __uint_as_float(0x7FC00000u);
     const float t2 = w.inv_t * kLog2e;  // of the teacher's logits
-    const float inv_t = w.inv_t * p.score_scale;
-    const float c2 = inv_t * kLog2e;
+    const float c2 = w.inv_t * p.score_scale * kLog2e;
     const float scale = kForward || p.gmax == nullptr ? 1.f : *p.gmax / Type<T>::kScale;  // of d^T H
     bool dead = false;
     // state of the row this thread holds while it walks along score tiles
     uint32_t cur_m = 0xFFFFFFFFu, row = 0, slot = 0;
     bool live = false;
     float top = 0.f, share = 0.f;  // of the teacher
-    float run_m = -INFINITY, run_l = 0.f, dot = 0.f, z2 = 0.f, coef = 0.f;
+    float run_m = -INFINITY, run_l = 0.f, dot = 0.f, coef = 0.f;
+    float run_q = 0.f;             // sum of the q seen
+    float2 z2 = make_float2(0.f, 0.f);
     float at_target = 0.f;         // d of cross entropy there
     float e2 = 0.f;                // log2 |coef| - z2
     // of the packed pairs of d; p is at most 1, however far the errors of scores
@@ -854,7 +876,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
     auto flush = [&]() {
       if (kForward && cur_m != 0xFFFFFFFFu && row < p.rows)
         p.partial[(uint64_t)row * p.slots + slot] =
-            Partial{dead ? nan : run_m, dead ? nan : run_l, dot, 0.f};
+            Partial{dead ? nan : run_m, dead ? nan : run_l, dot, run_q};
     };
     uint32_t sub = 0;
     for (uint32_t block = 0; !t.done(); ++sub) {
@@ -876,12 +898,12 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
             }
             slot = 2 * (pair - lo) + half;
             run_m = -INFINITY;
-            run_l = dot = 0.f;
+            run_l = dot = run_q = 0.f;
           } else if (live) {
             coef = p.rg[row].coef;
             if (!kDistill) at_target = p.rg[row].target;
-            z2 = p.lse[row] * kLog2e;
-            e2 = log2f(fabsf(coef)) - z2;
+            z2 = lse_units(p.lse[row]);
+            e2 = (log2f(fabsf(coef)) - z2.y) - z2.x;
             most = Type<T>::pack(fabsf(coef), fabsf(coef));
             keep = coef != 0.f ? 0xFFFFFFFFu : 0u;
             sign = coef < 0.f ? 0x80008000u : 0u;
@@ -937,7 +959,8 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
                   mx[e] = fmaxf(mx[e], __uint_as_float(r[j + e]));
             const float m =
                 fmaxf(run_m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c2);
-            const float from = m < kMasked ? 0.f : m;
+            const float from = base_of(m);
+            if (kDistill) dot = fmaf(run_q, base_of(run_m) - from, dot);
             float2 l[2] = {make_float2(run_l * exp2_approx(run_m - from), 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
             for (int j = 0; j < 64; j += 2) {
@@ -954,8 +977,12 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
               const bool mine = cur.id[0] - col < 64u;
               if (mine) {
                 const float q = cur.weight(t2, top, share);
-                if (!kDistill) dot = s;
-                else if (q > 0.f) dot = fmaf(q, s * inv_t, dot);
+                if (!kDistill) {
+                  dot = s;
+                } else if (q > 0.f) {
+                  dot = fmaf(q, fmaf(s, c2, -from), dot);
+                  run_q += q;
+                }
               }
               cur.drop(w, mine);
             }
@@ -988,7 +1015,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
                 const float s = pick64(r, cur.id[0] - col);
                 const bool mine = cur.id[0] - col < 64u;
                 if (mine) {  // p - q in FP32
-                  const float x = min_nan(exp2_approx(fmaf(s, c2, -z2)), 1.f) - cur.weight(t2, top, share);
+                  const float x = min_nan(exp2_approx(fmaf(s, c2, -z2.x) - z2.y), 1.f) - cur.weight(t2, top, share);
                   out[cur.id[0] - col] = Type<T>::from(x * coef);
                 }
                 cur.drop(w, mine);
@@ -1100,48 +1127,69 @@ __device__ __forceinline__ void warp_join(float& m, float& l) {
     m = mn;
   }
 }
-__device__ __forceinline__ void join(float& m, float& l, const Partial& q) {
-  const float mn = fmaxf(m, q.m);
+__device__ __forceinline__ void join(float& m, float& l, float2 q) {
+  const float mn = fmaxf(m, q.x);
   // a walk without a column has l = 0 at m = -inf
-  l = l * (m == mn ? 1.f : exp2_approx(m - mn)) + q.l * (q.m == mn ? 1.f : exp2_approx(q.m - mn));
+  l = l * (m == mn ? 1.f : exp2_approx(m - mn)) + q.y * (q.x == mn ? 1.f : exp2_approx(q.x - mn));
   m = mn;
 }
 
 // Joins a row's slots over the lanes of a warp; the loads of 160 slots (a call
 // has at most 148 a row, but for few column tiles of many rows) are in flight
-// together.
-__device__ __forceinline__ void join_slots(const Partial* part, uint32_t slots, float& m, float& l,
+// together.  `local` (or NULL): the largest logit of each slot's entries, which
+// its q are relative to.
+__device__ __forceinline__ void join_slots(const Partial* part, const float* local, uint32_t slots,
+                                           const Teacher& st, float inv_t, float& m, float& l,
                                            float& dot) {
   const uint32_t lane = threadIdx.x & 31;
   m = -INFINITY;
   l = dot = 0.f;
+  float sum_q = 0.f;
   for (uint32_t s0 = lane; s0 < slots; s0 += 160) {
     float4 q[5];
+    float t[5];
 #pragma unroll
-    for (uint32_t j = 0; j < 5; ++j)
-      q[j] = s0 + 32 * j < slots
-                 ? *reinterpret_cast<const float4*>(part + s0 + 32 * j)
-                 : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    for (uint32_t j = 0; j < 5; ++j) {
+      const uint32_t i = s0 + 32 * j;
+      q[j] = i < slots ? *reinterpret_cast<const float4*>(part + i)
+                       : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+      t[j] = local && i < slots ? local[i] : -INFINITY;
+    }
+    if (local) {
+#pragma unroll
+      for (int j = 0; j < 5; ++j) {
+        const float by = t[j] > -INFINITY ? expf((t[j] - st.top) * inv_t) * st.share : 0.f;
+        q[j].z = by > 0.f ? q[j].z * by : 0.f;
+        q[j].w *= by;
+      }
+    }
     float top = fmaxf(fmaxf(fmaxf(q[0].x, q[1].x), fmaxf(q[2].x, q[3].x)), q[4].x);
     top = fmaxf(top, m);
     // a walk without a column has l = 0 at m = -inf
     float sum = m == top ? l : l * exp2_approx(m - top);
+    dot = fmaf(sum_q, base_of(m) - base_of(top), dot);
 #pragma unroll
     for (int j = 0; j < 5; ++j) {
       sum += q[j].x == top ? q[j].y : q[j].y * exp2_approx(q[j].x - top);
-      dot += q[j].z;
+      dot += fmaf(q[j].w, base_of(q[j].x) - base_of(top), q[j].z);
+      sum_q += q[j].w;
     }
     m = top;
     l = sum;
   }
+  const float mine = base_of(m);
   warp_join(m, l);
+  dot = fmaf(sum_q, mine - base_of(m), dot);
 #pragma unroll
   for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
 }
 
-__device__ __forceinline__ float set_loss(const Wanted& w, const Teacher& s, float z, float dot) {
+// T^2 (sum q log q + log l - dot): the scores' size cancels before it comes in.
+__device__ __forceinline__ float set_loss(const Wanted& w, const Teacher& s, float l, float dot) {
   const float t = 1.f / w.inv_t;
-  return stat_empty(s) ? 0.f : (stat_invalid(s) ? s.top : t * t * (s.entropy + (z - dot)));
+  if (stat_empty(s)) return 0.f;
+  if (stat_invalid(s) || !(l > 0.f)) return __uint_as_float(0x7FC00000u);
+  return t * t * (s.entropy + (log2f(l) - dot) * kLn2);
 }
 // Of a row without a target: ignored or invalid.
 __device__ __forceinline__ float no_target_loss(uint32_t target) {
@@ -1172,7 +1220,7 @@ __device__ __forceinline__ float put_target(float& m, float& l, float dot, float
 // A sure row's lse is score + loss, rounded once: the gradient takes p - 1 from
 // the distance of the two.
 __device__ __forceinline__ float row_lse(float m, float l, float score, float loss) {
-  return loss < 1.f ? score + loss : (m + log2f(l)) * kLn2;
+  return loss < 1.f ? score + loss : lse_of(m, l);
 }
 
 // One warp per row joins the walks' partial sums.  Row tile m's n_tiles tiles
@@ -1198,13 +1246,13 @@ __global__ void merge_kernel(Wanted w, const T* hidden, const T* table, uint32_t
   const uint32_t last = (uint32_t)(((x1 + 1) * pairs - 1) / total);
   const uint32_t slots = 2 * (last - first + 1);
   float m, l, dot;
-  join_slots(part + (uint64_t)r * row_slots, slots, m, l, dot);
+  const Teacher st = w.targets ? Teacher{} : w.stat[r];
+  join_slots(part + (uint64_t)r * row_slots, nullptr, slots, st, w.inv_t, m, l, dot);
   if (lane) return;
   float loss = no_target_loss(target);
   if (target < vocab) loss = put_target(m, l, dot, c2, score);
-  const float z = target < vocab ? row_lse(m, l, score, loss) : (m + log2f(l)) * kLn2;
-  lse[r] = z;
-  losses[r] = w.targets ? loss : set_loss(w, w.stat[r], z, dot);
+  lse[r] = target < vocab ? row_lse(m, l, score, loss) : lse_of(m, l);
+  losses[r] = w.targets ? loss : set_loss(w, st, l, dot);
 }
 
 // ---- few rows ------------------------------------------------------------
@@ -1215,15 +1263,19 @@ __global__ void merge_kernel(Wanted w, const T* hidden, const T* table, uint32_t
 // even to 32 rows), against the hidden rows, which stay in shared memory (N =
 // rows rounded up to 16).  All its scores fit in TMEM, so the softmax needs no
 // running maximum: one pass for each row's maximum over the CTA's range, one
-// for the sum.  TMEM that is left holds each score in up to three segments of
-// its products, added in FP32.  The wanted scores come from the FP32 pipes in
-// the join, where the target's takes the place of the tensor core's.  Measured (49,152 x 576, fp16, table from DRAM): 13.9 us for 1 row
+// for the sum.  Cross entropy: TMEM that is left holds each score in up to three
+// segments of its products, added in FP32, and the target's score comes from the
+// FP32 pipes in the join, in place of the tensor core's.  Distillation: the
+// entries in the CTA's range are listed while the table streams, and their scores
+// read out of TMEM, the same numbers that lse and the gradients are made of.  Measured (49,152 x 576, fp16, table from DRAM): 13.9 us for 1 row
 // (4.1 TB/s; a read of the table alone takes 8.6 us at 6.55 TB/s), against 24.6
 // us with the tile engine; the join adds 1.4 us.
 constexpr uint32_t kFewRows = 64;
 constexpr uint32_t kFewMaxStages = 12;
 constexpr uint32_t kFewThreads = 192;  // producer, MMA issuer, 4 epilogue warps
 constexpr uint32_t kFewSmem = 222 * 1024;
+constexpr uint32_t kFewEntries = 256;        // of a teacher's sets, listed at a time
+constexpr uint32_t kFewListBytes = kFewEntries * 12;
 
 struct FewParams {
   uint32_t rows, n;         // n: rows rounded up to 16
@@ -1231,8 +1283,9 @@ struct FewParams {
   uint32_t w_chunks, stages;
   uint32_t segments, seg_chunks;  // accumulators of a score, chunks in each
   float c2;                 // score scale / T in units of ln 2
-  const uint32_t* targets;  // or NULL
+  uint32_t entries;         // of the teacher's sets
   Partial* partial;         // [rows][CTA]; dot: the target's, where it is in the range
+  float* local;             // distillation: [rows][CTA], what q in dot is relative to
 };
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -1243,9 +1296,13 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   tmem_wait_ld();
 }
 
-__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
+__device__ __forceinline__ uint32_t tmem_ld1_begin(uint32_t taddr) {  // valid after tmem_wait_ld
   uint32_t r;
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+  return r;
+}
+__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
+  const uint32_t r = tmem_ld1_begin(taddr);
   tmem_wait_ld();
   return __uint_as_float(r);
 }
@@ -1256,15 +1313,17 @@ __device__ __forceinline__ float warp_max(float v) {
   return m;
 }
 
-template <typename T>
+template <typename T, bool kDistill>
 __global__ void __launch_bounds__(kFewThreads, 1)
 few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
-                const __grid_constant__ CUtensorMap tm_table, const FewParams p) {
+                const __grid_constant__ CUtensorMap tm_table, const FewParams p, const Wanted w) {
   extern __shared__ unsigned char smem_raw[];
   __shared__ uint64_t bars[2 * kFewMaxStages + 2];
   __shared__ uint32_t tmem_at, abort_word, filled;
   __shared__ float2 part[4][kFewRows];
   __shared__ float s_dot[kFewRows];
+  __shared__ int32_t s_at[kDistill ? 2 * kFewRows : 1];       // first entries in the range, and behind it
+  __shared__ uint32_t s_first[kDistill ? kFewRows + 1 : 1];  // their places in the list
   const uint32_t hid = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t hid_chunk = p.n * 128;
   const uint32_t ring = hid + ((p.w_chunks * hid_chunk + 1023u) & ~1023u);
@@ -1352,16 +1411,89 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
       bar_wait(done, 0);
     }
   } else {
-    const uint32_t quad = warp & 3;
+    const uint32_t quad = warp & 3, e = threadIdx.x - 64;
+    auto together = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };  // the epilogue warps
     uint32_t target[2];  // of rows lane and lane + 32, from v0 on; the warp's own, if any
+    uint32_t listed = 0;  // entries in the range, row after row
+    // list: row and place in the range, or none; logit, then weight; score
+    uint32_t* list = reinterpret_cast<uint32_t*>(smem_raw + (ring - smem_u32(smem_raw)) +
+                                                 p.stages * kChunkBytes);
+    float* list_t = reinterpret_cast<float*>(list + kFewEntries);
+    float* list_s = list_t + kFewEntries;
+    auto fill = [&](uint32_t from) {
+      for (uint32_t i = e; i < kFewEntries && from + i < listed; i += 128) {
+        uint32_t r = 0;  // the last row that begins at or before the entry
 #pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) {
-      const uint32_t r = lane + 32 * i;
-      target[i] = p.targets && r < p.rows ? p.targets[r] - v0 : kInvalid;
-      if (target[i] >= count || ((target[i] >> 5) & 3u) != quad) target[i] = kInvalid;
-      if (warp == 2) s_dot[r] = 0.f;
+        for (uint32_t step = kFewRows / 2; step > 0; step >>= 1)
+          if (s_first[r + step] <= from + i) r += step;
+        const int32_t k = s_at[r] + (int32_t)(from + i - s_first[r]);
+        const uint32_t v = (uint32_t)w.ids[k] - v0;
+        list[i] = v < count ? r << 16 | v : kInvalid;  // ids of an invalid set lie anywhere
+        list_t[i] = v < count ? w.logits[k] : -INFINITY;
+      }
+    };
+    float dot = 0.f, sum_q = 0.f, top = -INFINITY;  // of row e: weights relative to `top`
+    // The listed logits of row e become weights.
+    auto weigh = [&](uint32_t from) {
+      if (e >= p.rows) return;
+      const uint32_t begin = max(s_first[e], from) - from;
+      const uint32_t end = min(s_first[e + 1] - min(s_first[e + 1], from), kFewEntries);
+      float m = top;
+      for (uint32_t i = begin; i < end; ++i) m = fmaxf(m, list_t[i]);
+      if (m > top) {
+        const float by = expf((top - m) * w.inv_t);
+        sum_q *= by;
+        dot = by > 0.f ? dot * by : 0.f;  // an infinite score that no longer counts
+        top = m;
+      }
+      for (uint32_t i = begin; i < end; ++i) {
+        const float t = list_t[i], q = t > -INFINITY ? expf((t - top) * w.inv_t) : 0.f;
+        list_t[i] = q;
+        sum_q += q;
+      }
+    };
+    if constexpr (kDistill) {
+      const uint32_t r = e & (kFewRows - 1);
+      int32_t at = 0;
+      if (r < p.rows) {
+        const int32_t a = w.offsets[r], b = w.offsets[r + 1];
+        if (a >= 0 && b >= a && (uint32_t)b <= p.entries)
+          at = first_entry(w, r, e < kFewRows ? v0 : v0 + count);
+      }
+      s_at[e] = at;
+      together();
+      if (warp == 2) {
+        uint32_t n[2], sum[2];
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+          // an ascending set has at most one entry a table row; an invalid one is cut
+          n[i] = min(count, (uint32_t)max(0, s_at[kFewRows + 32 * i + lane] - s_at[32 * i + lane]));
+          sum[i] = n[i];
+          for (uint32_t o = 1; o < 32; o <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, sum[i], o);
+            if (lane >= o) sum[i] += x;
+          }
+        }
+        const uint32_t half = __shfl_sync(0xFFFFFFFFu, sum[0], 31);
+        s_first[lane] = sum[0] - n[0];
+        s_first[lane + 32] = half + sum[1] - n[1];
+        if (lane == 31) s_first[kFewRows] = half + sum[1];
+      }
+      together();
+      listed = s_first[kFewRows];
+      fill(0);
+      together();
+      weigh(0);
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < 2; ++i) {
+        const uint32_t r = lane + 32 * i;
+        target[i] = r < p.rows ? w.targets[r] - v0 : kInvalid;
+        if (target[i] >= count || ((target[i] >> 5) & 3u) != quad) target[i] = kInvalid;
+        if (warp == 2) s_dot[r] = 0.f;
+      }
     }
-    asm volatile("bar.sync 1, 128;" ::: "memory");  // the epilogue warps
+    together();
     const bool ok = bar_wait(done, 0) && !*abort_flag;
     fence_after();
     const uint32_t acc = tmem + ((quad * 32u) << 16);
@@ -1417,25 +1549,73 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
       if ((lane & 1u) == 0)
         part[quad][c + lane / 2] = make_float2(mx[0], ok ? sum[0] : __uint_as_float(0x7FC00000u));
     }
-    // the targets' scores: of all rows' targets, few lie in one CTA's range
+    float m = -INFINITY, l = 0.f;  // of row e
+    auto join_quads = [&]() {
+      if (e < p.rows)
 #pragma unroll
-    for (uint32_t i = 0; i < 2; ++i)
-      for (uint32_t todo = __ballot_sync(0xFFFFFFFFu, target[i] != kInvalid); todo; todo &= todo - 1) {
-        const uint32_t from = __ffs(todo) - 1;
-        const uint32_t v = __shfl_sync(0xFFFFFFFFu, target[i], from), c = from + 32 * i;
-        float x = 0.f;
-        for (uint32_t g = 0; g < p.segments; ++g)
-          x += tmem_ld1(acc + ((v / 128) * p.segments + g) * p.n + c);
-        if (lane == (v & 31u)) s_dot[c] = x;
+        for (int q = 0; q < 4; ++q) join(m, l, part[q][e]);
+    };
+    if constexpr (!kDistill) {
+      // the targets' scores: of all rows' targets, few lie in one CTA's range
+#pragma unroll
+      for (uint32_t i = 0; i < 2; ++i)
+        for (uint32_t todo = __ballot_sync(0xFFFFFFFFu, target[i] != kInvalid); todo; todo &= todo - 1) {
+          const uint32_t from = __ffs(todo) - 1;
+          const uint32_t v = __shfl_sync(0xFFFFFFFFu, target[i], from), c = from + 32 * i;
+          float x = 0.f;
+          for (uint32_t g = 0; g < p.segments; ++g)
+            x += tmem_ld1(acc + ((v / 128) * p.segments + g) * p.n + c);
+          if (lane == (v & 31u)) s_dot[c] = x;
+        }
+      fence_before();
+      together();
+      join_quads();
+      if (e < p.rows) dot = s_dot[e];
+    } else {
+      for (uint32_t from = 0;;) {
+        const uint32_t n = min(kFewEntries, listed - from);
+        for (uint32_t i = 0; i < n; i += 32) {
+          const uint32_t key = i + lane < n ? list[i + lane] : kInvalid;
+          uint32_t todo = __ballot_sync(0xFFFFFFFFu, key != kInvalid && ((key >> 5) & 3u) == quad);
+          while (todo) {  // four in flight
+            uint32_t at[4], v[4], x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              at[j] = todo ? __ffs(todo) - 1 : 32u;
+              todo &= todo - 1;
+              const uint32_t one = __shfl_sync(0xFFFFFFFFu, key, at[j] & 31u);
+              v[j] = at[j] < 32u ? one & 0xFFFFu : 0u;
+              x[j] = tmem_ld1_begin(acc + (v[j] / 128) * p.n + (at[j] < 32u ? one >> 16 : 0u));
+            }
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (at[j] < 32u && lane == (v[j] & 31u)) list_s[i + at[j]] = __uint_as_float(x[j]);
+            __syncwarp();
+          }
+        }
+        fence_before();
+        together();
+        if (from == 0) join_quads();
+        if (e < p.rows) {
+          const uint32_t end = min(s_first[e + 1], from + n);
+          for (uint32_t i = max(s_first[e], from); i < end; ++i) {
+            const float q = list_t[i - from];
+            if (q > 0.f) dot = fmaf(q, fmaf(list_s[i - from], p.c2, -base_of(m)), dot);
+          }
+        }
+        if (listed - from <= kFewEntries) break;
+        from += kFewEntries;
+        together();
+        fill(from);
+        together();
+        weigh(from);
       }
-    fence_before();
-    asm volatile("bar.sync 1, 128;" ::: "memory");  // the epilogue warps
-    const uint32_t r = threadIdx.x - 64;
-    if (r < p.rows) {
-      float m = -INFINITY, l = 0.f;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) join(m, l, Partial{part[q][r].x, part[q][r].y, 0.f, 0.f});
-      p.partial[(uint64_t)r * gridDim.x + blockIdx.x] = Partial{m, l, s_dot[r], 0.f};
+    }
+    if (e < p.rows) {
+      const uint64_t at = (uint64_t)e * gridDim.x + blockIdx.x;
+      p.partial[at] = Partial{m, l, dot, sum_q};
+      if (kDistill) p.local[at] = top;
     }
   }
   __syncthreads();
@@ -1511,7 +1691,8 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
   // table chunks full, table free, scores full, d full, dE full / empty [2], dH done
   __shared__ uint64_t bars[kFewGradChunks + 8];
   __shared__ uint32_t tmem_at, abort_word, loads;
-  __shared__ float s_coef[kFewGradRows], s_z2[kFewGradRows];
+  __shared__ float s_coef[kFewGradRows];
+  __shared__ float2 s_z2[kFewGradRows];
   __shared__ float s_top[kFewGradRows], s_share[kFewGradRows];
   __shared__ uint32_t s_target[kFewGradRows];
   __shared__ float s_short[kFewGradRows];  // p - 1 of the targets in the CTA's range
@@ -1570,7 +1751,7 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
     const float g = warp_max(a < INFINITY ? a : 0.f);
     const float coef = wr != 0.f ? wr / g * Type<T>::kScale : 0.f;
     s_coef[lane] = coef;
-    s_z2[lane] = lane < p.rows ? p.lse[lane] * kLog2e : 0.f;
+    s_z2[lane] = lse_units(lane < p.rows ? p.lse[lane] : 0.f);
     s_target[lane] = w.targets && lane < p.rows && coef != 0.f ? w.targets[lane] : kInvalid;
     if (lane == 0) s_gmax = g;
     if (blockIdx.x == 0 && lane < p.rows) p.rg[lane] = RowGrad{coef, g / Type<T>::kScale, 0.f};
@@ -1733,7 +1914,8 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
           for (int e = 0; e < 2; ++e) {
             const uint32_t n = c + j + e;
             const float coef = s_coef[n];
-            float d = min_nan(exp2_approx(fmaf(__uint_as_float(r[j + e]), c2, -s_z2[n])), 1.f);
+            const float2 z2 = s_z2[n];
+            float d = min_nan(exp2_approx(fmaf(__uint_as_float(r[j + e]), c2, -z2.x) - z2.y), 1.f);
             if (kDistill) d -= s_q[n * 128 + row];
             else if (s_target[n] == v) d = s_short[n];
             x[e] = coef == 0.f || !in ? 0.f : (dead ? nan : d * coef);
@@ -1818,76 +2000,33 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
                  : "memory");
 }
 
-// One block per row: the CTAs' sums, the wanted scores, the teacher's
-// distribution.
-constexpr uint32_t kJoinThreads = 256;
+// One warp per row, a block each: the CTAs' sums, the target's score, the
+// teacher's distribution.
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads)
+__global__ void __launch_bounds__(32)
 few_rows_join_kernel(Wanted w, const T* hidden, const T* table, uint32_t width, const Partial* part,
-                     uint32_t slots, uint32_t rows, uint32_t entries, uint32_t vocab,
-                     float c2, float* losses, float* lse) {
-  __shared__ float dots[kJoinThreads / 32];
-  const uint32_t r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const T* row = hidden + (uint64_t)r * width;
+                     const float* local, uint32_t slots, uint32_t entries, uint32_t vocab, float c2,
+                     float* losses, float* lse) {
+  const uint32_t r = blockIdx.x;
   const uint32_t target = w.targets ? w.targets[r] : kInvalid;
-  Teacher st{-INFINITY, 0.f, 0.f};
-  float dot = 0.f;  // of the row's wanted scores, as weighted
-  if (target < vocab) {
-    if (warp == 0) dot = warp_score(row, table + (uint64_t)target * width, width);
-  } else if (w.offsets) {
-    st = teacher_stat(w, r, entries, vocab);
-    if (!stat_empty(st) && !stat_invalid(st)) {
-      const int32_t end = w.offsets[r + 1];
-      constexpr int32_t kWarps = kJoinThreads / 32;
-      for (int32_t k = w.offsets[r] + (int32_t)warp; k < end; k += 4 * kWarps) {
-        const T* at[4];
-        float q[4], s[4] = {};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int32_t i = k + j * kWarps < end ? k + j * kWarps : k;
-          q[j] = k + j * kWarps < end ? expf((w.logits[i] - st.top) * w.inv_t) * st.share : 0.f;
-          at[j] = table + (uint64_t)w.ids[i] * width;
-        }
-        for (uint32_t c = lane * 8; c < width; c += 256) {  // four rows in flight
-          const uint4 x = ld_v4(row + c);
-          uint4 y[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) y[j] = ld_v4(at[j] + c);
-          const T* xs = reinterpret_cast<const T*>(&x);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const T* ys = reinterpret_cast<const T*>(&y[j]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s[j] = fmaf(Type<T>::to(xs[e]), Type<T>::to(ys[e]), s[j]);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-#pragma unroll
-          for (int o = 16; o; o >>= 1) s[j] += __shfl_xor_sync(0xFFFFFFFFu, s[j], o);
-          if (q[j] > 0.f) dot = fmaf(q[j], s[j] * w.inv_t, dot);
-        }
-      }
-    }
-  }
-  if (lane == 0) dots[warp] = dot;
-  __syncthreads();
-  if (warp) return;
+  Teacher st{};
+  float score = 0.f;
   // The inputs were complete before this kernel could start: every kernel here
   // lets the next one start only after its own wait for the one before.
-  dot = lane < kJoinThreads / 32 ? dots[lane] : 0.f;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
+  if (target < vocab)
+    score = warp_score(hidden + (uint64_t)r * width, table + (uint64_t)target * width, width);
+  else if (w.offsets)
+    st = teacher_stat(w, r, entries, vocab);
   pdl_wait();
   pdl_trigger();
-  float m, l, tensor;
-  join_slots(part + (uint64_t)r * slots, slots, m, l, tensor);
-  if (lane) return;
+  float m, l, dot;
+  join_slots(part + (uint64_t)r * slots, w.offsets ? local + (uint64_t)r * slots : nullptr, slots, st,
+             w.inv_t, m, l, dot);
+  if (threadIdx.x) return;
   float loss = no_target_loss(target);
-  if (target < vocab) loss = put_target(m, l, tensor, c2, dot);
-  const float z = target < vocab ? row_lse(m, l, dot, loss) : (m + log2f(l)) * kLn2;
-  lse[r] = z;
-  losses[r] = w.targets ? loss : set_loss(w, st, z, dot);
+  if (target < vocab) loss = put_target(m, l, dot, c2, score);
+  lse[r] = target < vocab ? row_lse(m, l, score, loss) : lse_of(m, l);
+  losses[r] = w.targets ? loss : set_loss(w, st, l, dot);
 }
 
 // d_hidden: the splits' sums in a fixed order, scaled and rounded; four columns
@@ -1965,7 +2104,7 @@ bool sizes_ok(uint64_t rows, uint64_t width, uint64_t vocab) {
 }
 
 struct ForwardPlan {
-  uint64_t m_tiles, n_tiles, slots, stat, partial, bytes;
+  uint64_t m_tiles, n_tiles, slots, stat, partial, local, bytes;
   ForwardPlan(uint64_t rows, uint64_t vocab) {
     m_tiles = (rows + 2 * kBM - 1) / (2 * kBM);
     n_tiles = (vocab + kBN - 1) / kBN;
@@ -1979,7 +2118,8 @@ struct ForwardPlan {
     if (rows <= kFewRows && slots < kMaxPairs) slots = kMaxPairs;
     stat = 0;
     partial = round_up(rows * sizeof(Teacher), 256);
-    bytes = round_up(partial + 2 * slots * rows * sizeof(Partial), 256);
+    local = partial + 2 * slots * rows * sizeof(Partial);
+    bytes = round_up(local + (rows <= kFewRows ? 2 * kMaxPairs * rows * sizeof(float) : 0), 256);
   }
 };
 
@@ -2246,7 +2386,7 @@ cudaError_t teacher_launch(const Wanted& w, uint64_t rows, uint64_t entries, uin
 struct FewPlan {
   uint32_t n, range, ctas, segments, seg_chunks, stages = 0;
   uint64_t smem;
-  FewPlan(uint64_t rows, uint64_t width, uint64_t vocab, uint64_t sms) {
+  FewPlan(uint64_t rows, uint64_t width, uint64_t vocab, uint64_t sms, bool distill) {
     if (rows > kFewRows) return;
     n = (uint32_t)round_up(rows, 16);
     range = (uint32_t)round_up((vocab + sms - 1) / sms, 32);
@@ -2254,14 +2394,16 @@ struct FewPlan {
     const uint32_t columns = (range + 127) / 128 * n;
     if (columns > kTmemCols) return;  // scores beyond TMEM
     const uint32_t chunks = (uint32_t)((width + kBK - 1) / kBK);
-    segments = kTmemCols / columns < 3 ? kTmemCols / columns : 3;
+    // distillation: the scores that the gradients will have, so one segment
+    segments = distill ? 1 : (kTmemCols / columns < 3 ? kTmemCols / columns : 3);
     seg_chunks = (chunks + segments - 1) / segments;
     segments = (chunks + seg_chunks - 1) / seg_chunks;
     const uint64_t hid = round_up((width + kBK - 1) / kBK * n * 128, 1024);
-    if (hid + 4 * kChunkBytes + 1024 > kFewSmem) return;  // no room for a ring
-    const uint64_t room = (kFewSmem - 1024 - hid) / kChunkBytes;
+    const uint64_t rest = hid + 1024 + (distill ? kFewListBytes : 0);
+    if (rest + 4 * kChunkBytes > kFewSmem) return;  // no room for a ring
+    const uint64_t room = (kFewSmem - rest) / kChunkBytes;
     stages = (uint32_t)(room < kFewMaxStages ? room : kFewMaxStages);
-    smem = hid + stages * kChunkBytes + 1024;
+    smem = rest + stages * kChunkBytes;
   }
 };
 
@@ -2276,8 +2418,10 @@ cudaError_t device_sms(uint32_t* sms) {
   uint32_t& c = cached[dev & 63];
   if (c == 0) {
     e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    for (const void* k : {(const void*)few_rows_kernel<__half>,
-                          (const void*)few_rows_kernel<__nv_bfloat16>,
+    for (const void* k : {(const void*)few_rows_kernel<__half, false>,
+                          (const void*)few_rows_kernel<__half, true>,
+                          (const void*)few_rows_kernel<__nv_bfloat16, false>,
+                          (const void*)few_rows_kernel<__nv_bfloat16, true>,
                           (const void*)few_rows_grad_kernel<__half, false>,
                           (const void*)few_rows_grad_kernel<__half, true>,
                           (const void*)few_rows_grad_kernel<__nv_bfloat16, false>,
@@ -2307,10 +2451,10 @@ struct FewGradPlan {
   }
 };
 
-template <typename T>
+template <typename T, bool kDistill>
 mf_status forward_few(const FewPlan& few, Wanted w, const T* hidden, const T* table, uint64_t entries,
-                      void* partial, float* losses, float* lse, uint64_t rows, uint64_t width,
-                      uint64_t vocab, cudaStream_t s) {
+                      void* partial, void* local, float* losses, float* lse, uint64_t rows,
+                      uint64_t width, uint64_t vocab, cudaStream_t s) {
   CUtensorMap tm_h, tm_t;
   if (!make_map<T>(&tm_h, hidden, rows, width, width, kBK, few.n) ||
       !make_map<T>(&tm_t, table, vocab, width, width, kBK, 32))
@@ -2324,15 +2468,18 @@ mf_status forward_few(const FewPlan& few, Wanted w, const T* hidden, const T* ta
   p.stages = few.stages;
   p.segments = few.segments;
   p.seg_chunks = few.seg_chunks;
-  p.c2 = w.inv_t * (1.f + (float)(few.seg_chunks * kBK) * kLostPerProduct) * kLog2e;
-  p.targets = w.targets;
+  // one segment: as the gradients' scores
+  const uint64_t products = few.segments == 1 ? width : few.seg_chunks * kBK;
+  p.c2 = w.inv_t * (1.f + (float)products * kLostPerProduct) * kLog2e;
+  p.entries = (uint32_t)entries;
   p.partial = static_cast<Partial*>(partial);
-  cudaError_t e = launch_after(few_rows_kernel<T>, few.ctas, kFewThreads, few.smem, s, tm_h,
-                               tm_t, p);
+  p.local = static_cast<float*>(local);
+  cudaError_t e = launch_after(few_rows_kernel<T, kDistill>, few.ctas, kFewThreads, few.smem, s, tm_h,
+                               tm_t, p, w);
   if (e == cudaSuccess)
-    e = launch_after(few_rows_join_kernel<T>, rows, kJoinThreads, 0, s, w, hidden, table,
-                     (uint32_t)width, static_cast<const Partial*>(p.partial), few.ctas, p.rows,
-                     (uint32_t)entries, p.vocab, p.c2, losses, lse);
+    e = launch_after(few_rows_join_kernel<T>, rows, 32, 0, s, w, hidden, table, (uint32_t)width,
+                     static_cast<const Partial*>(p.partial), static_cast<const float*>(p.local),
+                     few.ctas, p.entries, p.vocab, p.c2, losses, lse);
   return launched(e);
 }
 
@@ -2362,10 +2509,11 @@ mf_status forward(Span hidden, Span embedding, Span targets, Span ids, Span logi
   uint32_t sms = 0;
   cudaError_t e = device_sms(&sms);
   if (e != cudaSuccess) return fail(MF_CUDA_RUNTIME_FAILURE, (uint32_t)e);
-  const FewPlan few(rows, width, vocab, sms);
+  const FewPlan few(rows, width, vocab, sms, kDistill);
   if (few.stages > 0)
-    return forward_few<T>(few, w, static_cast<const T*>(hidden.p),
+    return forward_few<T, kDistill>(few, w, static_cast<const T*>(hidden.p),
                           static_cast<const T*>(embedding.p), ids.bytes / 4, ws + plan.partial,
+                          ws + plan.local,
                           static_cast<float*>(const_cast<void*>(losses.p)),
                           static_cast<float*>(const_cast<void*>(lse.p)), rows, width, vocab, s);
   uint32_t pairs = 0;
