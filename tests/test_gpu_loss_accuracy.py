@@ -1,0 +1,91 @@
+"""GPU tests of accuracies that the losses state beyond the formulas' bounds: up to
+32 rows carry d as two 16-bit numbers, and scores are corrected for what the
+tensor core's sums drop."""
+from __future__ import annotations
+
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def mf(cuda):
+    from market_sim_b200 import head
+
+    return head
+
+
+def _dtype(kind):
+    import torch
+
+    return {"f16": torch.float16, "bf16": torch.bfloat16}[kind]
+
+
+@pytest.mark.parametrize("kind", ("f16", "bf16"))
+@pytest.mark.parametrize("distill", (False, True))
+@pytest.mark.parametrize("rows", (1, 5, 32))
+def test_few_rows_round_the_result_alone(mf, rows, distill, kind):
+    """A sum of two 16-bit numbers holds d to u^2 (fp16 to half the step of its
+    smallest numbers, 2^-25 of 2^15 over the largest weight).  With scores of a few
+    units (error (64 + 4) 2^-23 sum |h e|), what a gradient element is off by is its
+    own rounding, u of it, and little more."""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    vocab, width = 900, 64
+    h = torch.randn(rows, width, generator=gen, device="cuda").to(_dtype(kind))
+    e = (0.5 / math.sqrt(width) * torch.randn(vocab, width, generator=gen, device="cuda")).to(
+        _dtype(kind))
+    targets = torch.randint(0, vocab, (rows,), generator=gen, device="cuda", dtype=torch.int32)
+    grad = 256 * (0.5 + torch.rand(rows, generator=gen, device="cuda"))
+    offsets = torch.arange(rows + 1, dtype=torch.int32, device="cuda")
+    sets = (offsets, targets, torch.zeros(rows, device="cuda"))
+    loss = mf.DenseLoss(e, rows, stream=torch.cuda.Stream())
+    torch.cuda.synchronize()
+    if distill:
+        _, lse = loss.distill(h, *sets)
+        dh, de = loss.distill_backward(h, *sets, 1.0, lse, grad)
+    else:
+        _, lse = loss.cross_entropy(h, targets)
+        dh, de = loss.cross_entropy_backward(h, targets, lse, grad)
+    torch.cuda.synchronize()
+    hd, ed, w = h.double(), e.double(), grad.double()[:, None]
+    scores = hd @ ed.T
+    p = torch.softmax(scores, 1)
+    q = torch.nn.functional.one_hot(targets.long(), vocab).double()
+    d, u = w * (p - q), torch.finfo(h.dtype).eps / 2
+    s_off = ((width + 4) * 2.0 ** -23 * (hd.abs() @ ed.abs().T)).amax(1, keepdim=True)
+    lse_off = s_off + vocab * 2.0 ** -24 + 2.0 ** -20 * (1 + torch.logsumexp(scores, 1, True).abs())
+    tiny = float(grad.max()) * (2.0 ** -40 if kind == "f16" else 2.0 ** -126)
+    d_off = w * ((s_off + lse_off) * p + q * 2.0 ** -19) + u * u * d.abs() + tiny
+    small = 2.0 ** -25 if kind == "f16" else 2.0 ** -134
+    for got, want, off, terms in (
+            (dh, d @ ed, d_off @ ed.abs(), (vocab + 4) * 2.0 ** -23 * (d.abs() @ ed.abs())),
+            (de, d.T @ hd, d_off.T @ hd.abs(), (rows + 4) * 2.0 ** -23 * (d.abs().T @ hd.abs()))):
+        off = (off + terms) * (1 + u) + u * want.abs() + small
+        assert bool(((got.double() - want).abs() <= off).all())
+
+
+@pytest.mark.parametrize("kind", ("f16", "bf16"))
+@pytest.mark.parametrize("rows", (40, 300))
+def test_scores_of_parallel_rows(mf, rows, kind):
+    """Products of one sign lose the most (4.2e-9 to 5e-9 of the score a product);
+    about 3e-9 a product is what the header leaves, on average over the rows (one
+    row's lies within a few 4.5e-7 of that)."""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    vocab, width = 500, 2048
+    e = torch.randn(vocab, width, generator=gen, device="cuda").to(_dtype(kind))
+    h = (e[torch.arange(rows, device="cuda") % vocab].float() / 8).to(_dtype(kind))
+    none = torch.full((rows,), -1, dtype=torch.int32, device="cuda")
+    loss = mf.DenseLoss(e, rows, stream=torch.cuda.Stream())
+    torch.cuda.synchronize()
+    _, lse = loss.cross_entropy(h, none)
+    torch.cuda.synchronize()
+    want = torch.logsumexp(h.double() @ e.double().T, 1)
+    assert float(want.min()) > 200  # the parallel row's score alone
+    off = float(((lse.double() - want) / want).mean().abs())
+    assert off <= 3.3e-9 * width + 4 * 4.5e-7 / math.sqrt(rows), off / width
