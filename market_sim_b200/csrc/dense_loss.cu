@@ -220,6 +220,24 @@ __device__ __forceinline__ int32_t first_entry(const Wanted& w, uint32_t r, uint
   return lo;
 }
 
+// The same with seven probes in flight at a time, in entries [lo, hi): three waits
+// for memory in place of nine for 300 entries.
+__device__ __forceinline__ int32_t first_entry_of_8(const int32_t* ids, int32_t lo, int32_t hi,
+                                                    uint32_t v) {
+  while (lo < hi) {
+    const int32_t step = (hi - lo + 7) / 8;
+    int32_t below = 0;
+#pragma unroll
+    for (int32_t j = 1; j < 8; ++j) {
+      const int64_t k = (int64_t)lo + (int64_t)step * j - 1;
+      below += k < hi && (uint32_t)ids[k] < v;
+    }
+    lo += below * step;
+    if (below < 7) hi = (int32_t)min((int64_t)hi, (int64_t)lo + step - 1);
+  }
+  return lo;
+}
+
 struct RowGrad {  // one row's factors of d
   float coef;     // d16 = (p - q) * coef
   float scale;    // d_hidden = (d16 . E) * scale
@@ -1263,19 +1281,21 @@ __global__ void merge_kernel(Wanted w, const T* hidden, const T* table, uint32_t
 // even to 32 rows), against the hidden rows, which stay in shared memory (N =
 // rows rounded up to 16).  All its scores fit in TMEM, so the softmax needs no
 // running maximum: one pass for each row's maximum over the CTA's range, one
-// for the sum.  Cross entropy: TMEM that is left holds each score in up to three
-// segments of its products, added in FP32, and the target's score comes from the
-// FP32 pipes in the join, in place of the tensor core's.  Distillation: the
-// entries in the CTA's range are listed while the table streams, and their scores
-// read out of TMEM, the same numbers that lse and the gradients are made of.  Measured (49,152 x 576, fp16, table from DRAM): 13.9 us for 1 row
+// for the sum.  TMEM that is left holds each score in up to three segments of its
+// products, added in FP32 (distillation: as many as the gradients' kernel will
+// make; above its 32 rows one, as the tile engine's).  Cross entropy: the target's
+// score comes from the FP32 pipes in the join, in place of the tensor core's.
+// Distillation: the entries in the CTA's range are listed and weighed while the
+// table streams; their scores are those of TMEM, the same numbers that lse and the
+// gradients are made of, laid out in shared memory for any thread to read.  Measured (49,152 x 576, fp16, table from DRAM): 13.9 us for 1 row
 // (4.1 TB/s; a read of the table alone takes 8.6 us at 6.55 TB/s), against 24.6
 // us with the tile engine; the join adds 1.4 us.
 constexpr uint32_t kFewRows = 64;
 constexpr uint32_t kFewMaxStages = 12;
 constexpr uint32_t kFewThreads = 192;  // producer, MMA issuer, 4 epilogue warps
 constexpr uint32_t kFewSmem = 222 * 1024;
-constexpr uint32_t kFewEntries = 256;        // of a teacher's sets, listed at a time
-constexpr uint32_t kFewListBytes = kFewEntries * 12;
+constexpr uint32_t kFewEntries = 2048;       // of a teacher's sets, listed at a time
+constexpr uint32_t kFewListBytes = kFewEntries * 8;
 
 struct FewParams {
   uint32_t rows, n;         // n: rows rounded up to 16
@@ -1296,13 +1316,9 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   tmem_wait_ld();
 }
 
-__device__ __forceinline__ uint32_t tmem_ld1_begin(uint32_t taddr) {  // valid after tmem_wait_ld
+__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
   uint32_t r;
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
-  return r;
-}
-__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
-  const uint32_t r = tmem_ld1_begin(taddr);
   tmem_wait_ld();
   return __uint_as_float(r);
 }
@@ -1415,12 +1431,13 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
     auto together = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };  // the epilogue warps
     uint32_t target[2];  // of rows lane and lane + 32, from v0 on; the warp's own, if any
     uint32_t listed = 0;  // entries in the range, row after row
-    // list: row and place in the range, or none; logit, then weight; score
+    // list of the entries in the range, row after row: place in the range, or
+    // none; logit, then weight
     uint32_t* list = reinterpret_cast<uint32_t*>(smem_raw + (ring - smem_u32(smem_raw)) +
                                                  p.stages * kChunkBytes);
     float* list_t = reinterpret_cast<float*>(list + kFewEntries);
-    float* list_s = list_t + kFewEntries;
     auto fill = [&](uint32_t from) {
+#pragma unroll 4
       for (uint32_t i = e; i < kFewEntries && from + i < listed; i += 128) {
         uint32_t r = 0;  // the last row that begins at or before the entry
 #pragma unroll
@@ -1428,25 +1445,34 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
           if (s_first[r + step] <= from + i) r += step;
         const int32_t k = s_at[r] + (int32_t)(from + i - s_first[r]);
         const uint32_t v = (uint32_t)w.ids[k] - v0;
-        list[i] = v < count ? r << 16 | v : kInvalid;  // ids of an invalid set lie anywhere
+        list[i] = v < count ? v : kInvalid;  // ids of an invalid set lie anywhere
         list_t[i] = v < count ? w.logits[k] : -INFINITY;
       }
     };
-    float dot = 0.f, sum_q = 0.f, top = -INFINITY;  // of row e: weights relative to `top`
-    // The listed logits of row e become weights.
+    // Distillation: 2 to 8 neighbouring threads share a row's entries.
+    const uint32_t share = p.n <= 16 ? 8u : (p.n <= 32 ? 4u : 2u);
+    const uint32_t r_mine = kDistill ? e / share : e, sub = kDistill ? e % share : 0u;
+    const bool mine = r_mine < p.rows;
+    float dot = 0.f, sum_q = 0.f, top = -INFINITY;  // weights relative to `top`
+    uint32_t begin = 0, end = 0;                    // of the row, in the list
+    // The listed logits of a row become weights.
     auto weigh = [&](uint32_t from) {
-      if (e >= p.rows) return;
-      const uint32_t begin = max(s_first[e], from) - from;
-      const uint32_t end = min(s_first[e + 1] - min(s_first[e + 1], from), kFewEntries);
-      float m = top;
-      for (uint32_t i = begin; i < end; ++i) m = fmaxf(m, list_t[i]);
-      if (m > top) {
-        const float by = expf((top - m) * w.inv_t);
+      begin = end = 0;
+      if (mine) {
+        begin = max(s_first[r_mine], from) - from + sub;
+        end = min(max(s_first[r_mine + 1], from) - from, kFewEntries);
+      }
+      float most = top;
+      for (uint32_t i = begin; i < end; i += share) most = fmaxf(most, list_t[i]);
+      for (uint32_t o = 1; o < share; o <<= 1)
+        most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+      if (most > top) {
+        const float by = expf((top - most) * w.inv_t);
         sum_q *= by;
         dot = by > 0.f ? dot * by : 0.f;  // an infinite score that no longer counts
-        top = m;
+        top = most;
       }
-      for (uint32_t i = begin; i < end; ++i) {
+      for (uint32_t i = begin; i < end; i += share) {
         const float t = list_t[i], q = t > -INFINITY ? expf((t - top) * w.inv_t) : 0.f;
         list_t[i] = q;
         sum_q += q;
@@ -1458,7 +1484,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
       if (r < p.rows) {
         const int32_t a = w.offsets[r], b = w.offsets[r + 1];
         if (a >= 0 && b >= a && (uint32_t)b <= p.entries)
-          at = first_entry(w, r, e < kFewRows ? v0 : v0 + count);
+          at = first_entry_of_8(w.ids, a, b, e < kFewRows ? v0 : v0 + count);
       }
       s_at[e] = at;
       together();
@@ -1507,6 +1533,16 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
           r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(x[j]));
       }
     };
+    // Distillation: the ring, which nothing uses any more, takes the scores of as
+    // many tiles as it holds, on the way of the sums; rows padded by one for the banks.
+    float* dense = reinterpret_cast<float*>(smem_raw + (ring - smem_u32(smem_raw)));
+    const uint32_t pitch = p.n + 1, held = p.stages * kChunkBytes / (512u * pitch);
+    auto keep = [&](uint32_t t, uint32_t c, const uint32_t (&r)[16]) {
+      float* at = dense + (t * 128 + quad * 32 + lane) * pitch + c;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) at[j] = __uint_as_float(r[j]);
+    };
+    const uint32_t kept = listed > 0 ? held : 0;
     for (uint32_t c = 0; c < p.n; c += 16) {
       float mx[16], l[16];
 #pragma unroll
@@ -1527,6 +1563,8 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
       for (uint32_t t = 0; t < tiles; ++t) {
         uint32_t r[16];
         scores(t, c, r);
+        if constexpr (kDistill)
+          if (t < kept) keep(t, c, r);
         const bool in = t * 128 + quad * 32 + lane < count;
 #pragma unroll
         for (int j = 0; j < 16; ++j)
@@ -1549,12 +1587,6 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
       if ((lane & 1u) == 0)
         part[quad][c + lane / 2] = make_float2(mx[0], ok ? sum[0] : __uint_as_float(0x7FC00000u));
     }
-    float m = -INFINITY, l = 0.f;  // of row e
-    auto join_quads = [&]() {
-      if (e < p.rows)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) join(m, l, part[q][e]);
-    };
     if constexpr (!kDistill) {
       // the targets' scores: of all rows' targets, few lie in one CTA's range
 #pragma unroll
@@ -1567,41 +1599,37 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
             x += tmem_ld1(acc + ((v / 128) * p.segments + g) * p.n + c);
           if (lane == (v & 31u)) s_dot[c] = x;
         }
-      fence_before();
-      together();
-      join_quads();
-      if (e < p.rows) dot = s_dot[e];
-    } else {
+    }
+    fence_before();
+    together();
+    float m = -INFINITY, l = 0.f;  // of the row
+    if (mine)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) join(m, l, part[q][r_mine]);
+    if constexpr (!kDistill) {
+      if (mine) dot = s_dot[r_mine];
+    } else if (listed > 0) {
+      const float base = base_of(m);
       for (uint32_t from = 0;;) {
-        const uint32_t n = min(kFewEntries, listed - from);
-        for (uint32_t i = 0; i < n; i += 32) {
-          const uint32_t key = i + lane < n ? list[i + lane] : kInvalid;
-          uint32_t todo = __ballot_sync(0xFFFFFFFFu, key != kInvalid && ((key >> 5) & 3u) == quad);
-          while (todo) {  // four in flight
-            uint32_t at[4], v[4], x[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              at[j] = todo ? __ffs(todo) - 1 : 32u;
-              todo &= todo - 1;
-              const uint32_t one = __shfl_sync(0xFFFFFFFFu, key, at[j] & 31u);
-              v[j] = at[j] < 32u ? one & 0xFFFFu : 0u;
-              x[j] = tmem_ld1_begin(acc + (v[j] / 128) * p.n + (at[j] < 32u ? one >> 16 : 0u));
-            }
-            tmem_wait_ld();
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (at[j] < 32u && lane == (v[j] & 31u)) list_s[i + at[j]] = __uint_as_float(x[j]);
-            __syncwarp();
+        uint32_t i = begin;
+        for (uint32_t t0 = 0; t0 < tiles; t0 += held) {
+          if (held < tiles && (t0 > 0 || from > 0)) {
+            together();
+            for (uint32_t t = t0; t < min(tiles, t0 + held); ++t)
+              for (uint32_t c = 0; c < p.n; c += 16) {
+                uint32_t r[16];
+                scores(t, c, r);
+                keep(t - t0, c, r);
+              }
+            together();
           }
-        }
-        fence_before();
-        together();
-        if (from == 0) join_quads();
-        if (e < p.rows) {
-          const uint32_t end = min(s_first[e + 1], from + n);
-          for (uint32_t i = max(s_first[e], from); i < end; ++i) {
-            const float q = list_t[i - from];
-            if (q > 0.f) dot = fmaf(q, fmaf(list_s[i - from], p.c2, -base_of(m)), dot);
+          // a valid set ascends; of an invalid one what lies elsewhere is left out
+          for (; i < end; i += share) {
+            const uint32_t v = list[i];
+            if (v != kInvalid && v >= (t0 + held) * 128) break;
+            const float q = list_t[i];
+            if (q > 0.f && v >= t0 * 128)
+              dot = fmaf(q, fmaf(dense[(v - t0 * 128) * pitch + r_mine], p.c2, -base), dot);
           }
         }
         if (listed - from <= kFewEntries) break;
@@ -1611,9 +1639,13 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
         together();
         weigh(from);
       }
+      for (uint32_t o = 1; o < share; o <<= 1) {
+        dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
+        sum_q += __shfl_xor_sync(0xFFFFFFFFu, sum_q, o);
+      }
     }
-    if (e < p.rows) {
-      const uint64_t at = (uint64_t)e * gridDim.x + blockIdx.x;
+    if (mine && sub == 0) {
+      const uint64_t at = (uint64_t)r_mine * gridDim.x + blockIdx.x;
       p.partial[at] = Partial{m, l, dot, sum_q};
       if (kDistill) p.local[at] = top;
     }
@@ -1653,7 +1685,8 @@ struct FewGradParams {
   uint32_t rows, n;         // n: rows rounded up to 16
   uint32_t width, w_chunks;
   uint32_t vocab, range;    // table rows per CTA, a multiple of 32
-  float score_scale;
+  uint32_t segments, seg_chunks;  // as forward
+  float c2;
   const void *hidden, *table;
   const float* grad;
   const float* lse;
@@ -1788,7 +1821,7 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
   __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_at;
-  // TMEM columns: d H^T [blocks x n], scores [n], dE [2 x 128]
+  // TMEM columns: d H^T [blocks x n], scores [segments x n], dE [2 x 128]
   const uint32_t acc_h = tmem, acc_s = tmem + blocks * p.n, acc_e = tmem + 256;
 
   if (warp == 0) {
@@ -1811,13 +1844,16 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
       bool ok = true;
       uint32_t pass = 0;  // dE buffers used so far
       for (uint32_t t = 0; ok && t < tiles && !*abort_flag; ++t) {
+        uint32_t acc = acc_s, seg_end = p.seg_chunks;
         for (uint32_t kc = 0; ok && kc < p.w_chunks; ++kc) {
           ok = bar_wait(e_full(kc), t & 1u);
           if (!ok) break;
           const uint64_t a = sw128_desc(tab + kc * kChunkBytes), b = sw128_desc(hid + kc * hid_chunk);
+          if (kc == seg_end) acc += p.n, seg_end += p.seg_chunks;
+          const bool add = kc + p.seg_chunks != seg_end;
 #pragma unroll
           for (int k4 = 0; k4 < kBK / 16; ++k4)
-            mma_one(acc_s, a + 2 * k4, b + 2 * k4, idesc_s, (kc | (uint32_t)k4) != 0u);
+            mma_one(acc, a + 2 * k4, b + 2 * k4, idesc_s, add || k4 != 0);
         }
         if (!ok) break;
         mma_commit_one(s_full);
@@ -1864,7 +1900,7 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
     const uint32_t quad = warp & 3u, half = (warp - 2) >> 2;
     const uint32_t lanes = (quad * 32u) << 16;
     const uint32_t row = quad * 32 + lane;  // of the tile
-    const float c2 = w.inv_t * p.score_scale * kLog2e, t2 = w.inv_t * kLog2e;
+    const float c2 = p.c2, t2 = w.inv_t * kLog2e;
     const float scale = s_gmax / Type<T>::kScale;
     const float nan = __uint_as_float(0x7FC00000u);
     bool dead = false;
@@ -1906,6 +1942,13 @@ few_rows_grad_kernel(const __grid_constant__ CUtensorMap tm_table, const FewGrad
       for (uint32_t c = half * (p.n / 2); c < (half + 1) * (p.n / 2); c += 8) {
         uint32_t r[8];
         tmem_ld8(acc_s + lanes + c, r);
+        for (uint32_t g = 1; g < p.segments; ++g) {
+          uint32_t x[8];
+          tmem_ld8(acc_s + lanes + g * p.n + c, x);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(x[j]));
+        }
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
@@ -2382,31 +2425,6 @@ cudaError_t teacher_launch(const Wanted& w, uint64_t rows, uint64_t entries, uin
                       (uint32_t)rows, (uint32_t)entries, (uint32_t)vocab);
 }
 
-// How the few-rows kernel takes a call; stages 0: it does not.
-struct FewPlan {
-  uint32_t n, range, ctas, segments, seg_chunks, stages = 0;
-  uint64_t smem;
-  FewPlan(uint64_t rows, uint64_t width, uint64_t vocab, uint64_t sms, bool distill) {
-    if (rows > kFewRows) return;
-    n = (uint32_t)round_up(rows, 16);
-    range = (uint32_t)round_up((vocab + sms - 1) / sms, 32);
-    ctas = (uint32_t)((vocab + range - 1) / range);
-    const uint32_t columns = (range + 127) / 128 * n;
-    if (columns > kTmemCols) return;  // scores beyond TMEM
-    const uint32_t chunks = (uint32_t)((width + kBK - 1) / kBK);
-    // distillation: the scores that the gradients will have, so one segment
-    segments = distill ? 1 : (kTmemCols / columns < 3 ? kTmemCols / columns : 3);
-    seg_chunks = (chunks + segments - 1) / segments;
-    segments = (chunks + seg_chunks - 1) / seg_chunks;
-    const uint64_t hid = round_up((width + kBK - 1) / kBK * n * 128, 1024);
-    const uint64_t rest = hid + 1024 + (distill ? kFewListBytes : 0);
-    if (rest + 4 * kChunkBytes > kFewSmem) return;  // no room for a ring
-    const uint64_t room = (kFewSmem - rest) / kChunkBytes;
-    stages = (uint32_t)(room < kFewMaxStages ? room : kFewMaxStages);
-    smem = rest + stages * kChunkBytes;
-  }
-};
-
 // SMs of the current device, at most twice kMaxPairs (the workspace's slots).
 cudaError_t device_sms(uint32_t* sms) {
   static std::mutex mu;
@@ -2435,21 +2453,62 @@ cudaError_t device_sms(uint32_t* sms) {
   return cudaSuccess;
 }
 
-// The same for the gradients; smem 0: the kernel does not take the call.
+// How the few-rows gradients take a call; smem 0: they do not.
 struct FewGradPlan {
-  uint32_t n, range, ctas;
+  uint32_t n, range, ctas, segments, seg_chunks;
   uint64_t smem = 0;
   FewGradPlan(uint64_t rows, uint64_t width, uint64_t vocab, uint64_t sms, bool distill) {
-    const uint64_t chunks = (width + kBK - 1) / kBK;
+    const uint32_t chunks = (uint32_t)((width + kBK - 1) / kBK);
     if (rows > kFewGradRows || chunks > kFewGradChunks) return;
     n = (uint32_t)round_up(rows, 16);
     range = (uint32_t)round_up((vocab + sms - 1) / sms, 32);
     ctas = (uint32_t)((vocab + range - 1) / range);
+    // as many segments of a score's products as TMEM holds here (beside d H^T, below
+    // the 256 columns of dE) and in the forward kernel
+    segments = (256 - (chunks + 1) / 2 * n) / n;
+    const uint32_t forward = kTmemCols / ((range + 127) / 128 * n);
+    if (segments > forward) segments = forward < 1 ? 1 : forward;
+    if (segments > 3) segments = 3;
+    seg_chunks = (chunks + segments - 1) / segments;
+    segments = (chunks + seg_chunks - 1) / seg_chunks;
     const uint64_t bytes =
         chunks * (kChunkBytes + n * 128) + kDBytes + (distill ? n * 512 : 0) + 1024;
     if (bytes <= kFewSmem) smem = bytes;
   }
 };
+
+// How the few-rows forward kernel takes a call; stages 0: it does not.
+struct FewPlan {
+  uint32_t n, range, ctas, segments, seg_chunks, stages = 0;
+  uint64_t smem;
+  FewPlan(uint64_t rows, uint64_t width, uint64_t vocab, uint64_t sms, bool distill) {
+    if (rows > kFewRows) return;
+    n = (uint32_t)round_up(rows, 16);
+    range = (uint32_t)round_up((vocab + sms - 1) / sms, 32);
+    ctas = (uint32_t)((vocab + range - 1) / range);
+    const uint32_t columns = (range + 127) / 128 * n;
+    if (columns > kTmemCols) return;  // scores beyond TMEM
+    const uint32_t chunks = (uint32_t)((width + kBK - 1) / kBK);
+    // distillation: the scores that the gradients will have
+    const FewGradPlan grad(rows, width, vocab, sms, distill);
+    segments = kTmemCols / columns < 3 ? kTmemCols / columns : 3;
+    if (distill) segments = grad.smem > 0 ? grad.segments : 1;
+    seg_chunks = (chunks + segments - 1) / segments;
+    segments = (chunks + seg_chunks - 1) / seg_chunks;
+    const uint64_t hid = round_up((width + kBK - 1) / kBK * n * 128, 1024);
+    const uint64_t rest = hid + 1024 + (distill ? kFewListBytes : 0);
+    if (rest + 4 * kChunkBytes > kFewSmem) return;  // no room for a ring
+    const uint64_t room = (kFewSmem - rest) / kChunkBytes;
+    stages = (uint32_t)(room < kFewMaxStages ? room : kFewMaxStages);
+    smem = rest + stages * kChunkBytes;
+  }
+};
+
+// 1 / T and the correction of scores summed in segments, in units of ln 2.
+float few_scale(float inv_t, uint32_t segments, uint32_t seg_chunks, uint64_t width) {
+  const uint64_t products = segments == 1 ? width : seg_chunks * kBK;
+  return inv_t * (1.f + (float)products * kLostPerProduct) * kLog2e;
+}
 
 template <typename T, bool kDistill>
 mf_status forward_few(const FewPlan& few, Wanted w, const T* hidden, const T* table, uint64_t entries,
@@ -2468,9 +2527,7 @@ mf_status forward_few(const FewPlan& few, Wanted w, const T* hidden, const T* ta
   p.stages = few.stages;
   p.segments = few.segments;
   p.seg_chunks = few.seg_chunks;
-  // one segment: as the gradients' scores
-  const uint64_t products = few.segments == 1 ? width : few.seg_chunks * kBK;
-  p.c2 = w.inv_t * (1.f + (float)products * kLostPerProduct) * kLog2e;
+  p.c2 = few_scale(w.inv_t, few.segments, few.seg_chunks, width);
   p.entries = (uint32_t)entries;
   p.partial = static_cast<Partial*>(partial);
   p.local = static_cast<float*>(local);
@@ -2609,7 +2666,9 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
     f.w_chunks = (uint32_t)((width + kBK - 1) / kBK);
     f.vocab = (uint32_t)vocab;
     f.range = few.range;
-    f.score_scale = 1.f + (float)width * kLostPerProduct;
+    f.segments = few.segments;
+    f.seg_chunks = few.seg_chunks;
+    f.c2 = few_scale(w.inv_t, few.segments, few.seg_chunks, width);
     f.hidden = hidden.p;
     f.table = embedding.p;
     f.grad = static_cast<const float*>(grad.p);
