@@ -1287,9 +1287,11 @@ __global__ void merge_kernel(Wanted w, const T* hidden, const T* table, uint32_t
 // score comes from the FP32 pipes in the join, in place of the tensor core's.
 // Distillation: the entries in the CTA's range are listed and weighed while the
 // table streams; their scores are those of TMEM, the same numbers that lse and the
-// gradients are made of, laid out in shared memory for any thread to read.  Measured (49,152 x 576, fp16, table from DRAM): 13.9 us for 1 row
-// (4.1 TB/s; a read of the table alone takes 8.6 us at 6.55 TB/s), against 24.6
-// us with the tile engine; the join adds 1.4 us.
+// gradients are made of, laid out in shared memory for any thread to read.
+// Measured (49,152 x 576, fp16, table from DRAM): 13.9 us for 1 row (4.1 TB/s; a
+// read of the table alone takes 8.6 us at 6.55 TB/s), against 24.6 us with the tile
+// engine; the join adds 1.4 us.  Sets of 32 and 300 entries add 0.8 us for 1 row; at
+// 64 rows (18.7 and 21 us) they take less and 1 us more than the targets (19.8).
 constexpr uint32_t kFewRows = 64;
 constexpr uint32_t kFewMaxStages = 12;
 constexpr uint32_t kFewThreads = 192;  // producer, MMA issuer, 4 epilogue warps
@@ -1428,7 +1430,10 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
     }
   } else {
     const uint32_t quad = warp & 3, e = threadIdx.x - 64;
-    auto together = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };  // the epilogue warps
+    auto together = [] {  // the epilogue warps
+      __syncwarp();
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+    };
     uint32_t target[2];  // of rows lane and lane + 32, from v0 on; the warp's own, if any
     uint32_t listed = 0;  // entries in the range, row after row
     // list of the entries in the range, row after row: place in the range, or

@@ -94,9 +94,12 @@ def test_agreed_rows(mf, rows, vocab, width, common, T, kind):
 
 
 @pytest.mark.parametrize("kind", ("f16", "bf16"))
-@pytest.mark.parametrize("rows,vocab,width", [(1, 20_000, 64), (8, 20_000, 64), (64, 9000, 72)])
+@pytest.mark.parametrize("rows,vocab,width", [(1, 20_000, 64), (8, 20_000, 64), (64, 9000, 72),
+                                              (16, 100_000, 64), (48, 40_000, 1024),
+                                              (64, 40_000, 1024)])
 def test_a_teacher_of_the_whole_vocabulary(mf, rows, vocab, width, kind):
-    """More entries in a CTA's range than are listed at a time; some rows have few."""
+    """More entries in a CTA's range than are listed at a time, more scores than its
+    memory takes at once (width 1,024); some rows have few."""
     import torch
 
     gen = torch.Generator(device="cuda").manual_seed(rows)
