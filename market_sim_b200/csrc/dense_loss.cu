@@ -62,6 +62,7 @@ constexpr uint32_t kTmemCols = 512;
 constexpr int kSetupThreads = 1024;
 constexpr uint32_t kMaxPairs = 74;             // pairs of the persistent grid
 constexpr uint64_t kPieceBytes = 128ull << 20; // one piece of d
+constexpr uint32_t kHalvesRows = 64;           // up to these, d in two halves
 constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = (float)(1.4426950408889634 - (double)kLog2e);
 constexpr float kLn2 = 0.6931471805599453f, kLn2Low = (float)(0.6931471805599453 - (double)kLn2);
 // The tensor core's additions drop the bits that fall below the sum's last
@@ -294,7 +295,8 @@ __device__ __forceinline__ float target_short(const T* hidden, const T* table, u
 template <typename T>
 __global__ void __launch_bounds__(kSetupThreads, 1)
 setup_kernel(Wanted w, const float* grad, const T* hidden, const T* table, const float* lse, T* scaled,
-             RowGrad* rg, float* gmax_out, uint32_t rows, uint32_t width, uint32_t vocab) {
+             RowGrad* rg, float* gmax_out, uint32_t rows, uint32_t width, uint32_t vocab,
+             uint32_t halves) {
   __shared__ float s_max[kSetupThreads / 32];
   pdl_wait();
   pdl_trigger();
@@ -337,7 +339,8 @@ setup_kernel(Wanted w, const float* grad, const T* hidden, const T* table, const
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = Type<T>::from(Type<T>::to(v[j]) * two_e);
       }
-      *reinterpret_cast<uint4*>(scaled + (uint64_t)r * width + c) = x;
+      for (uint32_t i = 0; i < halves; ++i)
+        *reinterpret_cast<uint4*>(scaled + (uint64_t)(r + i * rows) * width + c) = x;
     }
   }
 }
@@ -465,6 +468,7 @@ struct Params {
   Partial* partial;             // forward: [rows][slots]
   uint32_t slots;
   void* d;                      // backward: the piece being made
+  uint32_t d_rows;              // its rows: the batch's, or twice them (high and low halves)
   uint32_t pitch;
   const float* lse;
   const RowGrad* rg;
@@ -474,9 +478,9 @@ struct Params {
   uint32_t t_tiles;              // 256-row tiles of the piece
   uint32_t p_stages, p_stage_bytes;
   uint32_t p_chunks, per_split;  // d E: K chunks of the piece, and of one split
-  float* planes;                 // this piece's: [splits][rows][width]
+  float* planes;                 // this piece's: [splits][d_rows][width]
   uint32_t add;                  // they hold an earlier piece's sums
-  uint32_t r_chunks;             // d^T H: K chunks of the batch
+  uint32_t r_chunks;             // d^T H: K chunks of d_rows
   void* table_out;               // d_embedding + pv0 rows
   uint32_t wide_rows;            // its rows start on 32 bytes
   const float* gmax;
@@ -656,7 +660,9 @@ __device__ __forceinline__ float pick64(const uint32_t (&r)[64], uint32_t i) {
   return __uint_as_float(a[0]);
 }
 
-template <typename T, bool kForward, bool kDistill>
+// kHalves (backward, up to 64 rows): d as the sum of two 16-bit numbers.  Both
+// CTAs of a pair then hold the same rows' scores, and each takes half the columns.
+template <typename T, bool kForward, bool kDistill, bool kHalves>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p, Wanted w) {
   extern __shared__ unsigned char smem_raw[];
@@ -718,6 +724,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
       for (bool scores = false; ok && !t.done() && !*abort_flag; t.next(p)) {
         const int arow = (int)(t.m * 2 * kBM + rank * kBM);
         if (t.kind == kScore) {
+          const int hrow = kHalves ? 0 : arow;
           if (!scores) {  // every product stage read by its MMAs
             scores = true;
             for (uint32_t st = 0; ok && st < pr.n; ++st) {
@@ -744,7 +751,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
             const uint32_t at = sbase + p.s_ring + sr.at * p.s_stage_bytes;
             if (leader) bar_expect_tx(s_full(sr.at), bytes);
             tma_load_2d(at, &maps.table, k, brow, bar);
-            if (load_a) tma_load_2d(p.keep_hidden ? a_at : at + kChunkBytes, &maps.hidden, k, arow, bar);
+            if (load_a) tma_load_2d(p.keep_hidden ? a_at : at + kChunkBytes, &maps.hidden, k, hrow, bar);
             sr.next();
           }
         } else if constexpr (!kForward) {
@@ -865,6 +872,9 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
     const uint32_t quad = (uint32_t)(warp & 3);
     const uint32_t half = (uint32_t)(warp - 2) >> 2;
     const uint32_t tile_row = rank * kBM + quad * 32 + (uint32_t)lane;
+    // this warp's columns of a score tile
+    constexpr uint32_t kMine = kHalves ? kBN / 4 : kBN / 2;
+    const uint32_t c_begin = (kHalves ? 2 * rank + half : half) * kMine;
     const uint32_t leader_acc_empty0 = mapa(acc_empty(0), 0);
     const uint32_t leader_acc_empty1 = mapa(acc_empty(1), 0);
     const float nan = __uint_as_float(0x7FC00000u);
@@ -900,11 +910,11 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
     for (uint32_t block = 0; !t.done(); ++sub) {
       const uint32_t buf = sub & 1u;
       if (t.kind == kScore) {
-        const uint32_t v = p.v0 + t.n * kBN + half * (kBN / 2);
+        const uint32_t v = p.v0 + t.n * kBN + c_begin;
         if (t.m != cur_m) {  // (a score tile has one block)
           flush();
           cur_m = t.m;
-          row = t.m * 2 * kBM + tile_row;
+          row = t.m * 2 * kBM + (kHalves ? tile_row - rank * kBM : tile_row);
           live = row < p.rows;
           if (kForward) {
             // slot: this pair's place among the pairs that walk row tile m
@@ -944,10 +954,10 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
       fence_after();
       const uint32_t acc = tmem + ((quad * 32u) << 16) + buf * kBN;
       if (t.kind == kScore) {
-        cur.skip_to(w, p.v0 + t.n * kBN + half * (kBN / 2));
+        cur.skip_to(w, p.v0 + t.n * kBN + c_begin);
         const uint32_t c_end = p.cols - min(p.cols, t.n * kBN);  // columns of the tile that exist
 #pragma unroll 1
-        for (uint32_t c = half * (kBN / 2); c < (half + 1) * (kBN / 2); c += 64) {
+        for (uint32_t c = c_begin; c < c_begin + kMine; c += 64) {
           if (c >= c_end) break;
           uint32_t r[64];
           if (!dead) {
@@ -1008,7 +1018,37 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
             // |coef| goes into the exponent
             T* out = static_cast<T*>(p.d) + (uint64_t)row * p.pitch + t.n * kBN + c;
             const float2 cc = make_float2(c2, c2), ee = make_float2(e2, e2);
-            if (row < p.rows) {
+            T* out_low = out + (uint64_t)p.rows * p.pitch;
+            // element i of both halves
+            auto put = [&](uint32_t i, float x) {
+              const T high = Type<T>::from(x);
+              out[i] = high;
+              if constexpr (kHalves) {
+                out_low[i] = Type<T>::from(x - Type<T>::to(high));
+              }
+            };
+            if constexpr (kHalves) {
+              const float cap = fabsf(coef);
+              if (row < p.rows) {
+#pragma unroll
+                for (int j = 0; j < 64; j += 16) {
+                  uint32_t v[8], lo[8];
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) {
+                    const float2 x = fma2(make_float2(__uint_as_float(r[j + 2 * e]),
+                                                      __uint_as_float(r[j + 2 * e + 1])), cc, ee);
+                    const float a = min_nan(exp2_approx(x.x), cap), b = min_nan(exp2_approx(x.y), cap);
+                    v[e] = Type<T>::pack(a, b);
+                    const T* h = reinterpret_cast<const T*>(&v[e]);
+                    // (the high half of a finite weight is finite)
+                    lo[e] = (Type<T>::pack(a - Type<T>::to(h[0]), b - Type<T>::to(h[1])) & keep) ^ sign;
+                    v[e] = (v[e] & keep) ^ sign;
+                  }
+                  store_v8(out + j, v);
+                  store_v8(out_low + j, lo);
+                }
+              }
+            } else if (row < p.rows) {
 #pragma unroll
               for (int j = 0; j < 64; j += 16) {
                 uint32_t v[8];
@@ -1025,7 +1065,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
             if constexpr (!kDistill) {  // over the element just stored
               const bool mine = cur.id[0] - col < 64u;
               if (__any_sync(0xFFFFFFFFu, mine)) {
-                if (mine) out[cur.id[0] - col] = Type<T>::from(dead ? nan : at_target);
+                if (mine) put(cur.id[0] - col, dead ? nan : at_target);
                 __syncwarp();
               }
             } else {
@@ -1034,7 +1074,7 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
                 const bool mine = cur.id[0] - col < 64u;
                 if (mine) {  // p - q in FP32
                   const float x = min_nan(exp2_approx(fmaf(s, c2, -z2.x) - z2.y), 1.f) - cur.weight(t2, top, share);
-                  out[cur.id[0] - col] = Type<T>::from(x * coef);
+                  put(cur.id[0] - col, x * coef);
                 }
                 cur.drop(w, mine);
               }
@@ -1044,8 +1084,8 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
       } else if constexpr (!kForward) {
         const uint32_t c_half = p.bn / 2;
         const uint32_t m_row = (t.m + block) * 2 * kBM + tile_row;
-        const bool mine = m_row < (t.kind == kHidden ? p.rows : p.pcols);
-        const uint64_t at = ((uint64_t)(t.kind == kHidden ? t.split : 0u) * p.rows + m_row) * p.width;
+        const bool mine = m_row < (t.kind == kHidden ? p.d_rows : p.pcols);
+        const uint64_t at = ((uint64_t)(t.kind == kHidden ? t.split : 0u) * p.d_rows + m_row) * p.width;
 #pragma unroll 1
         for (uint32_t c = 0; c < c_half; c += 64) {
           uint32_t r[2][32];
@@ -2173,6 +2213,7 @@ struct ForwardPlan {
 
 struct BackwardPlan {
   uint64_t m_tiles, stat, rg, gmax, scaled, planes, piece[2], bytes;
+  uint32_t halves;        // of d: 2 where both fit the one row tile
   uint32_t cols, pieces;  // vocabulary rows of one piece
   uint32_t bn, bn_tiles;  // product tiles along the hidden width
   uint32_t blocks;        // row blocks that share a product tile's B
@@ -2183,6 +2224,15 @@ struct BackwardPlan {
     // with the rows
     m_tiles = (rows + 2 * kBM - 1) / (2 * kBM);
     const uint64_t all_rows = m_tiles * 2 * kBM;
+    // Up to 64 rows d is carried as the sum of two 16-bit numbers, the low halves in
+    // rows of their own of the one row tile (with the same hidden rows beside them,
+    // and sums that the last kernel adds): gradients keep what their type holds. With
+    // one 16-bit number a gradient is 1.4 times as far off as its own rounding makes
+    // it, and with few rows, whose errors do not average, up to 2.3 times. 49,152 x
+    // 576: 33 rows 57 and 63 us, 64 rows 58 and 65; 128 rows, where it is not done,
+    // would take 73 in place of 62.
+    halves = rows <= kHalvesRows ? 2 : 1;
+    const uint64_t d_rows = rows * halves;
     uint64_t c = kPieceBytes / (2 * all_rows) / kBN * kBN;
     if (c < kBN) c = kBN;
     pieces = (uint32_t)((vocab + c - 1) / c);
@@ -2211,7 +2261,7 @@ struct BackwardPlan {
     splits = (uint32_t)((chunks + per_split - 1) / per_split);
     // Sums kept apart cost a store a piece and are joined at the end; adding at
     // L2 from this layout (a row a thread) made a launch 25 us longer at 8,192 rows
-    const uint64_t set = (uint64_t)splits * rows * width * 4;
+    const uint64_t set = (uint64_t)splits * d_rows * width * 4;
     sets = (uint32_t)(kPieceBytes / ((uint64_t)splits * all_rows * width * 4));
     if (sets > pieces) sets = pieces;
     if (sets < 1) sets = 1;
@@ -2219,26 +2269,26 @@ struct BackwardPlan {
     rg = round_up(stat + rows * sizeof(Teacher), 256);
     gmax = round_up(rg + rows * sizeof(RowGrad), 256);
     scaled = gmax + 256;
-    planes = round_up(scaled + rows * width * 2, 256);
+    planes = round_up(scaled + d_rows * width * 2, 256);
     uint64_t sums = sets * set;
     const uint64_t few = 2 * kMaxPairs * rows * width * 4;  // few_rows_grad_kernel's planes
     if (rows <= kFewGradRows && width <= kFewGradChunks * kBK && sums < few) sums = few;
     piece[0] = round_up(planes + sums, 256);
-    const uint64_t one = round_up(rows * cols * 2, 256);
+    const uint64_t one = round_up(d_rows * cols * 2, 256);
     piece[1] = piece[0] + (pieces > 1 ? one : 0);
     bytes = piece[1] + one;
   }
 };
 
 // What a batch of at most `rows` rows needs: the most that any needs.  Within a
-// row tile, and up to `few` rows, a plan's bytes grow with the rows.
+// row tile, and up to each of `few` rows, a plan's bytes grow with the rows.
 template <typename F>
-uint64_t most_bytes(uint64_t rows, uint64_t few, F bytes) {
+uint64_t most_bytes(uint64_t rows, std::initializer_list<uint64_t> few, F bytes) {
   uint64_t most = bytes(rows);
   auto at = [&](uint64_t r) {
     if (r < rows && bytes(r) > most) most = bytes(r);
   };
-  at(few);
+  for (uint64_t r : few) at(r);
   for (uint64_t r = 2 * kBM; r < rows; r += 2 * kBM) at(r);
   return most;
 }
@@ -2310,7 +2360,7 @@ bool make_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, 
 
 // Sets the kernel's shared-memory limit (once per device) and returns how
 // many CTA pairs can be resident at once, at most kMaxPairs.
-template <typename T, bool kForward, bool kDistill>
+template <typename T, bool kForward, bool kDistill, bool kHalves>
 cudaError_t resident_pairs(uint32_t* pairs) {
   static std::mutex mu;
   static uint32_t cached[64] = {};
@@ -2321,7 +2371,7 @@ cudaError_t resident_pairs(uint32_t* pairs) {
   std::lock_guard<std::mutex> lock(mu);
   uint32_t& c = cached[dev & 63];
   if (c == 0) {
-    auto kernel = engine_kernel<T, kForward, kDistill>;
+    auto kernel = engine_kernel<T, kForward, kDistill, kHalves>;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
@@ -2579,7 +2629,7 @@ mf_status forward(Span hidden, Span embedding, Span targets, Span ids, Span logi
                           static_cast<float*>(const_cast<void*>(losses.p)),
                           static_cast<float*>(const_cast<void*>(lse.p)), rows, width, vocab, s);
   uint32_t pairs = 0;
-  e = resident_pairs<T, true, kDistill>(&pairs);
+  e = resident_pairs<T, true, kDistill, false>(&pairs);
   if (e != cudaSuccess) return fail(MF_CUDA_RUNTIME_FAILURE, (uint32_t)e);
   Maps maps = {};
   if (!make_map<T>(&maps.hidden, hidden.p, rows, width, width, kBK, kBM) ||
@@ -2597,7 +2647,7 @@ mf_status forward(Span hidden, Span embedding, Span targets, Span ids, Span logi
   p.partial = reinterpret_cast<Partial*>(ws + plan.partial);
   p.slots = (uint32_t)(2 * plan.slots);
   for (uint32_t i = 0; i <= pairs; ++i) p.score_at[i] = (uint32_t)(total * i / pairs);
-  e = launch_after(engine_kernel<T, true, kDistill>, 2 * pairs, kThreads, kSmemBytes, s,
+  e = launch_after(engine_kernel<T, true, kDistill, false>, 2 * pairs, kThreads, kSmemBytes, s,
                    maps, p, w);
   if (e != cudaSuccess) return launched(e);
   e = launch_after(merge_kernel<T>, (rows + 7) / 8, 256, 0, s, w,
@@ -2639,7 +2689,10 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint32_t pairs = 0, sms = 0;
   cudaError_t err = device_sms(&sms);
-  if (err == cudaSuccess) err = resident_pairs<T, false, kDistill>(&pairs);
+  if (err == cudaSuccess) err = resident_pairs<T, false, false, false>(&pairs);
+  if (err == cudaSuccess)
+    err = plan.halves > 1 ? resident_pairs<T, false, kDistill, true>(&pairs)
+                          : resident_pairs<T, false, kDistill, false>(&pairs);
   if (err != cudaSuccess) return fail(MF_CUDA_RUNTIME_FAILURE, (uint32_t)err);
   RowGrad* rg = reinterpret_cast<RowGrad*>(ws + plan.rg);
   float* gmax = reinterpret_cast<float*>(ws + plan.gmax);
@@ -2688,15 +2741,16 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
     return launched(err);
   }
   Maps maps = {};
+  const uint64_t d_rows = rows * plan.halves;
   if (!make_map<T>(&maps.hidden, hidden.p, rows, width, width, kBK, kBM) ||
       !make_map<T>(&maps.table, embedding.p, vocab, width, width, kBK, kBN / 2) ||
       !make_map<T>(&maps.table_n, embedding.p, vocab, width, width, 32, kBK) ||
-      !make_map<T>(&maps.scaled_n, scaled, rows, width, width, 32, kBK))
+      !make_map<T>(&maps.scaled_n, scaled, d_rows, width, width, 32, kBK))
     return fail(MF_CUDA_RUNTIME_FAILURE);
   err = launch_after(setup_kernel<T>, rows < 32 * 148 ? (rows + 31) / 32 : 148, kSetupThreads, 0, s, w,
                      static_cast<const float*>(grad.p), static_cast<const T*>(hidden.p),
                      static_cast<const T*>(embedding.p), static_cast<const float*>(lse.p), scaled, rg,
-                     gmax, (uint32_t)rows, (uint32_t)width, (uint32_t)vocab);
+                     gmax, (uint32_t)rows, (uint32_t)width, (uint32_t)vocab, plan.halves);
   if (err != cudaSuccess) return launched(err);
 
   Params p = base_params(rows, width, vocab);
@@ -2709,7 +2763,8 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
   p.p_stage_bytes = p.blocks * kChunkBytes + p.bn * kBK;
   p.p_stages = kRingBytes / p.p_stage_bytes < kMaxStages ? kRingBytes / p.p_stage_bytes : kMaxStages;
   p.per_split = plan.per_split;
-  p.r_chunks = (uint32_t)((rows + kBK - 1) / kBK);
+  p.d_rows = (uint32_t)d_rows;
+  p.r_chunks = (uint32_t)((d_rows + kBK - 1) / kBK);
   p.gmax = gmax;
   p.wide_rows = width % 16 == 0 && (uintptr_t)de % 32 == 0;
   auto piece_cols = [&](uint32_t i) {
@@ -2726,11 +2781,11 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
       p.pcols = piece_cols(i - 1);
       p.p_chunks = (p.pcols + kBK - 1) / kBK;
       p.add = i > plan.sets;
-      p.planes = planes + (uint64_t)((i - 1) % plan.sets) * plan.splits * rows * width;
+      p.planes = planes + (uint64_t)((i - 1) % plan.sets) * plan.splits * d_rows * width;
       p.table_out = de ? de + (uint64_t)p.pv0 * width : nullptr;
       const void* d = ws + plan.piece[(i - 1) & 1];
-      if (!make_map<T>(&maps.d_k, d, rows, p.pcols, plan.cols, kBK, kBM) ||
-          !make_map<T>(&maps.d_m, d, rows, p.pcols, plan.cols, kBK, kBK))
+      if (!make_map<T>(&maps.d_k, d, d_rows, p.pcols, plan.cols, kBK, kBM) ||
+          !make_map<T>(&maps.d_m, d, d_rows, p.pcols, plan.cols, kBK, kBK))
         return fail(MF_CUDA_RUNTIME_FAILURE);
       const uint32_t splits = (p.p_chunks + p.per_split - 1) / p.per_split;
       // a short last piece fills the first splits of its set; a set that is
@@ -2753,11 +2808,15 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
     deal(n_table, cost(p.blocks * p.bn, p.r_chunks), pairs, load, p.table_at);
     // a score tile takes a tenth longer than its columns x chunks
     deal(n_score, 1.1 * cost(kBN, p.w_chunks), pairs, load, p.score_at);
-    err = launch_after(engine_kernel<T, false, kDistill>, 2 * pairs, kThreads, kSmemBytes, s,
-                       maps, p, w);
+    // products alone: the variant that needs the fewest registers
+    auto kernel = i == plan.pieces ? engine_kernel<T, false, false, false>
+                                   : (plan.halves > 1 ? engine_kernel<T, false, kDistill, true>
+                                                      : engine_kernel<T, false, kDistill, false>);
+    err = launch_after(kernel, 2 * pairs, kThreads, kSmemBytes, s, maps, p, w);
     if (err != cudaSuccess) return launched(err);
   }
-  if (dh) err = finish_launch(planes, n_planes, rg, dh, rows, width, s);
+  // a plane of two halves is two planes
+  if (dh) err = finish_launch(planes, n_planes * plan.halves, rg, dh, rows, width, s);
   return launched(err);
 }
 
@@ -2770,14 +2829,14 @@ using mfb::loss::Span;
 extern "C" uint64_t mf_dense_loss_workspace_bytes(uint64_t rows, uint64_t hidden_size,
                                                   uint64_t vocab) {
   if (!loss::sizes_ok(rows, hidden_size, vocab)) return 0;
-  return loss::most_bytes(rows, loss::kFewRows,
+  return loss::most_bytes(rows, {loss::kFewRows},
                           [&](uint64_t r) { return loss::ForwardPlan(r, vocab).bytes; });
 }
 
 extern "C" uint64_t mf_dense_loss_backward_workspace_bytes(uint64_t rows, uint64_t hidden_size,
                                                            uint64_t vocab) {
   if (!loss::sizes_ok(rows, hidden_size, vocab)) return 0;
-  return loss::most_bytes(rows, loss::kFewGradRows, [&](uint64_t r) {
+  return loss::most_bytes(rows, {loss::kFewGradRows, loss::kHalvesRows}, [&](uint64_t r) {
     return loss::BackwardPlan(r, hidden_size, vocab).bytes;
   });
 }

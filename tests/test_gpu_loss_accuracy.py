@@ -1,5 +1,5 @@
 """GPU tests of accuracies that the losses state beyond the formulas' bounds: up to
-32 rows carry d as two 16-bit numbers, and scores are corrected for what the
+64 rows carry d as two 16-bit numbers, and scores are corrected for what the
 tensor core's sums drop."""
 from __future__ import annotations
 
@@ -25,19 +25,20 @@ def _dtype(kind):
 
 @pytest.mark.parametrize("kind", ("f16", "bf16"))
 @pytest.mark.parametrize("distill", (False, True))
-@pytest.mark.parametrize("rows", (1, 5, 32))
-def test_few_rows_round_the_result_alone(mf, rows, distill, kind):
+@pytest.mark.parametrize("rows,width", [(1, 64), (5, 64), (32, 64), (33, 64), (64, 64), (1, 648),
+                                        (7, 1024), (64, 648)])
+def test_few_rows_round_the_result_alone(mf, rows, width, distill, kind):
     """A sum of two 16-bit numbers holds d to u^2 (fp16 to half the step of its
     smallest numbers, 2^-25 of 2^15 over the largest weight).  With scores of a few
-    units (error (64 + 4) 2^-23 sum |h e|), what a gradient element is off by is its
-    own rounding, u of it, and little more."""
+    units (error (64 + 4) 2^-23 sum |h e|; wider rows hold zeros), what a gradient
+    element is off by is its own rounding, u of it, and little more."""
     import torch
 
     gen = torch.Generator(device="cuda").manual_seed(rows)
-    vocab, width = 900, 64
+    vocab = 900
     h = torch.randn(rows, width, generator=gen, device="cuda").to(_dtype(kind))
-    e = (0.5 / math.sqrt(width) * torch.randn(vocab, width, generator=gen, device="cuda")).to(
-        _dtype(kind))
+    h[:, 64:] = 0  # products of the others add nothing and drop nothing
+    e = (0.5 / 8 * torch.randn(vocab, width, generator=gen, device="cuda")).to(_dtype(kind))
     targets = torch.randint(0, vocab, (rows,), generator=gen, device="cuda", dtype=torch.int32)
     grad = 256 * (0.5 + torch.rand(rows, generator=gen, device="cuda"))
     offsets = torch.arange(rows + 1, dtype=torch.int32, device="cuda")
@@ -56,7 +57,9 @@ def test_few_rows_round_the_result_alone(mf, rows, distill, kind):
     p = torch.softmax(scores, 1)
     q = torch.nn.functional.one_hot(targets.long(), vocab).double()
     d, u = w * (p - q), torch.finfo(h.dtype).eps / 2
-    s_off = ((width + 4) * 2.0 ** -23 * (hd.abs() @ ed.abs().T)).amax(1, keepdim=True)
+    # 64 products, and the score correction of the width: 2^-29 a product of |s|
+    s_off = ((64 + 4) * 2.0 ** -23 * (hd.abs() @ ed.abs().T)
+             + width * 2.0 ** -29 * scores.abs()).amax(1, keepdim=True)
     lse_off = s_off + vocab * 2.0 ** -24 + 2.0 ** -20 * (1 + torch.logsumexp(scores, 1, True).abs())
     tiny = float(grad.max()) * (2.0 ** -40 if kind == "f16" else 2.0 ** -126)
     d_off = w * ((s_off + lse_off) * p + q * 2.0 ** -19) + u * u * d.abs() + tiny

@@ -215,7 +215,8 @@ def test_workspace_of_few_wide_rows(lib):
     for width in (8, 576, 640, 648, 1024, 4096, 8192):
         for rows in (1, 31, 32, 33, 64, 300):
             for vocab in (1, 1000, 49152, 1 << 24):
-                whole = 2 * rows * ((vocab + 255) // 256 * 256)  # d of all the vocabulary
+                # d of all the vocabulary, up to 64 rows in two halves
+                whole = 2 * max(rows, 2 * min(rows, 64)) * ((vocab + 255) // 256 * 256)
                 pieces = min(whole, 2 * (128 << 20))
                 sums = max(128 << 20, rows * width * 4)
                 assert b(rows, width, vocab) <= pieces + sums + rows * width * 2 + 4096 + rows * 24, \
