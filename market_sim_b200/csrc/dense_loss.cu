@@ -465,6 +465,7 @@ struct Params {
   uint32_t keep_hidden;         // the hidden tile stays in shared memory
   uint32_t s_ring, s_stages, s_stage_bytes;
   float score_scale;            // 1 + what the tensor core's additions lose
+  uint32_t score_accs, seg_chunks;  // kHalves: accumulators of a score tile, chunks in the first
   Partial* partial;             // forward: [rows][slots]
   uint32_t slots;
   void* d;                      // backward: the piece being made
@@ -648,7 +649,17 @@ struct Cursor {
   }
 };
 
-// r[i] for an index that differs from lane to lane (63 selects).
+// r[i] for an index that differs from lane to lane (31 and 63 selects).
+__device__ __forceinline__ float pick32(const uint32_t (&r)[32], uint32_t i) {
+  uint32_t a[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) a[j] = (i & 16u) ? r[j + 16] : r[j];
+#pragma unroll
+  for (int s = 8; s > 0; s >>= 1)
+#pragma unroll
+    for (int j = 0; j < s; ++j) a[j] = (i & (uint32_t)s) ? a[j + s] : a[j];
+  return __uint_as_float(a[0]);
+}
 __device__ __forceinline__ float pick64(const uint32_t (&r)[64], uint32_t i) {
   uint32_t a[32];
 #pragma unroll
@@ -661,7 +672,9 @@ __device__ __forceinline__ float pick64(const uint32_t (&r)[64], uint32_t i) {
 }
 
 // kHalves (backward, up to 64 rows): d as the sum of two 16-bit numbers.  Both
-// CTAs of a pair then hold the same rows' scores, and each takes half the columns.
+// CTAs of a pair then hold the same rows' scores, and each takes half the columns;
+// a score may be summed in two segments of its products, one in each accumulator,
+// as the forward kernel of these rows sums it.
 template <typename T, bool kForward, bool kDistill, bool kHalves>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p, Wanted w) {
@@ -804,13 +817,15 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
       const uint64_t k_major = sw128_desc(sbase);  // + offset / 16: any place of the region
       const uint64_t m_major = mn_desc(sbase, 128), n_major = mn_desc(sbase, 64);
       for (; ok && !t.done() && !*abort_flag; t.next(p)) {
-        for (uint32_t j = 0; ok && j < t.blocks; ++j)
+        const uint32_t accs = kHalves && t.kind == kScore ? p.score_accs : t.blocks;
+        for (uint32_t j = 0; ok && j < accs; ++j)
           ok = bar_wait(acc_empty((sub + j) & 1u), (((sub + j) >> 1) & 1u) ^ 1u);
         if (!ok) break;
         fence_after();
         const uint32_t acc = tmem + (sub & 1u) * kBN;
         if (t.kind == kScore) {
           constexpr uint32_t idesc = kIdesc | ((uint32_t)(kBN >> 3) << 17);
+          uint32_t to = acc, fresh = 0;  // the segment's accumulator and first chunk
           bool ready = bar_test(s_full(sr.at), sr.fills & 1u);
           for (uint32_t kc = 0; kc < t.chunks; ++kc) {
             if (!ready && !bar_wait(s_full(sr.at), sr.fills & 1u)) {
@@ -824,9 +839,10 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
             sr.next();
             // asked before the MMAs, whose issue takes as long as they do
             ready = bar_test(s_full(sr.at), sr.fills & 1u);
+            if (kHalves && kc == p.seg_chunks) to = tmem + ((sub + 1) & 1u) * kBN, fresh = kc;
 #pragma unroll
             for (int k4 = 0; k4 < kBK / 16; ++k4)
-              mma_pair(acc, a + 2 * k4, b + 2 * k4, idesc, (kc | (uint32_t)k4) != 0u);
+              mma_pair(to, a + 2 * k4, b + 2 * k4, idesc, kc != fresh || k4 != 0);
             mma_commit_pair(s_empty(at));  // frees the stage (both CTAs) once read
           }
         } else if constexpr (!kForward) {
@@ -859,8 +875,8 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
           }
         }
         if (!ok) break;
-        for (uint32_t j = 0; j < t.blocks; ++j) mma_commit_pair(acc_full((sub + j) & 1u));
-        sub += t.blocks;
+        for (uint32_t j = 0; j < accs; ++j) mma_commit_pair(acc_full((sub + j) & 1u));
+        sub += accs;
       }
       if (!ok) *abort_flag = 1u;
       mma_commit_local(drain);
@@ -947,7 +963,9 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
           cur.fill(w);
         }
       }
-      if (!dead && (*abort_flag || !bar_wait(acc_full(buf), (sub >> 1) & 1u))) {
+      const bool two = kHalves && t.kind == kScore && p.score_accs == 2;
+      if (!dead && (*abort_flag || !bar_wait(acc_full(buf), (sub >> 1) & 1u) ||
+                    (two && !bar_wait(acc_full(buf ^ 1u), ((sub + 1) >> 1) & 1u)))) {
         *abort_flag = 1u;
         dead = true;
       }
@@ -956,127 +974,163 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
       if (t.kind == kScore) {
         cur.skip_to(w, p.v0 + t.n * kBN + c_begin);
         const uint32_t c_end = p.cols - min(p.cols, t.n * kBN);  // columns of the tile that exist
+        if constexpr (kHalves) {
 #pragma unroll 1
-        for (uint32_t c = c_begin; c < c_begin + kMine; c += 64) {
-          if (c >= c_end) break;
-          uint32_t r[64];
-          if (!dead) {
-            tmem_ld64(acc + c, r);
-          } else {
+          for (uint32_t c = c_begin; c < c_begin + kMine && c < c_end; c += 32) {
+            uint32_t r[32];
+            if (!dead) {
+              tmem_ld32(acc + c, r);
+              if (two) {
+                uint32_t x[32];
+                tmem_ld32(tmem + ((quad * 32u) << 16) + (buf ^ 1u) * kBN + c, x);
+                tmem_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 64; ++j) r[j] = __float_as_uint(nan);
-          }
-          const uint32_t col = p.v0 + t.n * kBN + c;  // vocabulary id of r[0]
-          if constexpr (kForward) {
-            if (c + 64 > c_end) {
-#pragma unroll
-              for (int j = 0; j < 64; ++j)
-                if (c + j >= c_end) r[j] = 0xFF800000u;  // -inf
-            }
-            float mx[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) mx[j] = __uint_as_float(r[j]);
-#pragma unroll
-            for (int j = 4; j < 64; j += 8)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (j + 4 + e < 64)
-                  mx[e] = fmaxf(fmaxf(mx[e], __uint_as_float(r[j + e])),
-                                __uint_as_float(r[j + 4 + e]));
-                else
-                  mx[e] = fmaxf(mx[e], __uint_as_float(r[j + e]));
-            const float m =
-                fmaxf(run_m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c2);
-            const float from = base_of(m);
-            if (kDistill) dot = fmaf(run_q, base_of(run_m) - from, dot);
-            float2 l[2] = {make_float2(run_l * exp2_approx(run_m - from), 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-            for (int j = 0; j < 64; j += 2) {
-              const float2 x = fma2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])),
-                                    make_float2(c2, c2), make_float2(-from, -from));
-              l[(j >> 1) & 1] =
-                  add2(l[(j >> 1) & 1], make_float2(exp2_approx(x.x), exp2_approx(x.y)));
-            }
-            run_m = m;
-            l[0] = add2(l[0], l[1]);
-            run_l = l[0].x + l[0].y;
-            while (__any_sync(0xFFFFFFFFu, cur.id[0] - col < 64u)) {
-              const float s = pick64(r, cur.id[0] - col);
-              const bool mine = cur.id[0] - col < 64u;
-              if (mine) {
-                const float q = cur.weight(t2, top, share);
-                if (!kDistill) {
-                  dot = s;
-                } else if (q > 0.f) {
-                  dot = fmaf(q, fmaf(s, c2, -from), dot);
-                  run_q += q;
-                }
+                for (int j = 0; j < 32; ++j)
+                  r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(x[j]));
+              } else {
+                tmem_wait_ld();
               }
-              cur.drop(w, mine);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(nan);
             }
-          } else {
-            // |coef| goes into the exponent
+            const uint32_t col = p.v0 + t.n * kBN + c;
             T* out = static_cast<T*>(p.d) + (uint64_t)row * p.pitch + t.n * kBN + c;
-            const float2 cc = make_float2(c2, c2), ee = make_float2(e2, e2);
             T* out_low = out + (uint64_t)p.rows * p.pitch;
-            // element i of both halves
-            auto put = [&](uint32_t i, float x) {
-              const T high = Type<T>::from(x);
-              out[i] = high;
-              if constexpr (kHalves) {
-                out_low[i] = Type<T>::from(x - Type<T>::to(high));
-              }
-            };
-            if constexpr (kHalves) {
+            if (row < p.rows) {
+              const float2 cc = make_float2(c2, c2), ee = make_float2(e2, e2);
               const float cap = fabsf(coef);
-              if (row < p.rows) {
 #pragma unroll
-                for (int j = 0; j < 64; j += 16) {
-                  uint32_t v[8], lo[8];
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) {
-                    const float2 x = fma2(make_float2(__uint_as_float(r[j + 2 * e]),
-                                                      __uint_as_float(r[j + 2 * e + 1])), cc, ee);
-                    const float a = min_nan(exp2_approx(x.x), cap), b = min_nan(exp2_approx(x.y), cap);
-                    v[e] = Type<T>::pack(a, b);
-                    const T* h = reinterpret_cast<const T*>(&v[e]);
-                    // (the high half of a finite weight is finite)
-                    lo[e] = (Type<T>::pack(a - Type<T>::to(h[0]), b - Type<T>::to(h[1])) & keep) ^ sign;
-                    v[e] = (v[e] & keep) ^ sign;
-                  }
-                  store_v8(out + j, v);
-                  store_v8(out_low + j, lo);
-                }
-              }
-            } else if (row < p.rows) {
-#pragma unroll
-              for (int j = 0; j < 64; j += 16) {
-                uint32_t v[8];
+              for (int j = 0; j < 32; j += 16) {
+                uint32_t v[8], lo[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                   const float2 x = fma2(make_float2(__uint_as_float(r[j + 2 * e]),
                                                     __uint_as_float(r[j + 2 * e + 1])), cc, ee);
-                  v[e] = (Type<T>::least(Type<T>::pack(exp2_approx(x.x), exp2_approx(x.y)), most) &
-                          keep) ^ sign;
+                  const float a = min_nan(exp2_approx(x.x), cap), b = min_nan(exp2_approx(x.y), cap);
+                  v[e] = Type<T>::pack(a, b);
+                  const T* h = reinterpret_cast<const T*>(&v[e]);
+                  // (the high half of a finite weight is finite)
+                  lo[e] = (Type<T>::pack(a - Type<T>::to(h[0]), b - Type<T>::to(h[1])) & keep) ^ sign;
+                  v[e] = (v[e] & keep) ^ sign;
                 }
                 store_v8(out + j, v);
+                store_v8(out_low + j, lo);
               }
             }
-            if constexpr (!kDistill) {  // over the element just stored
-              const bool mine = cur.id[0] - col < 64u;
-              if (__any_sync(0xFFFFFFFFu, mine)) {
-                if (mine) put(cur.id[0] - col, dead ? nan : at_target);
-                __syncwarp();
+            // over the elements just stored
+            while (__any_sync(0xFFFFFFFFu, cur.id[0] - col < 32u)) {
+              const uint32_t i = cur.id[0] - col;
+              float x = at_target;
+              if constexpr (kDistill) {
+                const float s = pick32(r, i);
+                x = (min_nan(exp2_approx(fmaf(s, c2, -z2.x) - z2.y), 1.f) -
+                     cur.weight(t2, top, share)) * coef;
               }
+              if (dead) x = nan;
+              const bool mine = i < 32u;
+              if (mine) {
+                out[i] = Type<T>::from(x);
+                out_low[i] = Type<T>::from(x - Type<T>::to(Type<T>::from(x)));
+              }
+              cur.drop(w, mine);
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (uint32_t c = c_begin; c < c_begin + kMine; c += 64) {
+            if (c >= c_end) break;
+            uint32_t r[64];
+            if (!dead) {
+              tmem_ld64(acc + c, r);
             } else {
+#pragma unroll
+              for (int j = 0; j < 64; ++j) r[j] = __float_as_uint(nan);
+            }
+            const uint32_t col = p.v0 + t.n * kBN + c;  // vocabulary id of r[0]
+            if constexpr (kForward) {
+              if (c + 64 > c_end) {
+#pragma unroll
+                for (int j = 0; j < 64; ++j)
+                  if (c + j >= c_end) r[j] = 0xFF800000u;  // -inf
+              }
+              float mx[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) mx[j] = __uint_as_float(r[j]);
+#pragma unroll
+              for (int j = 4; j < 64; j += 8)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (j + 4 + e < 64)
+                    mx[e] = fmaxf(fmaxf(mx[e], __uint_as_float(r[j + e])),
+                                  __uint_as_float(r[j + 4 + e]));
+                  else
+                    mx[e] = fmaxf(mx[e], __uint_as_float(r[j + e]));
+              const float m =
+                  fmaxf(run_m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c2);
+              const float from = base_of(m);
+              if (kDistill) dot = fmaf(run_q, base_of(run_m) - from, dot);
+              float2 l[2] = {make_float2(run_l * exp2_approx(run_m - from), 0.f),
+                             make_float2(0.f, 0.f)};
+#pragma unroll
+              for (int j = 0; j < 64; j += 2) {
+                const float2 x = fma2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])),
+                                      make_float2(c2, c2), make_float2(-from, -from));
+                l[(j >> 1) & 1] =
+                    add2(l[(j >> 1) & 1], make_float2(exp2_approx(x.x), exp2_approx(x.y)));
+              }
+              run_m = m;
+              l[0] = add2(l[0], l[1]);
+              run_l = l[0].x + l[0].y;
               while (__any_sync(0xFFFFFFFFu, cur.id[0] - col < 64u)) {
                 const float s = pick64(r, cur.id[0] - col);
                 const bool mine = cur.id[0] - col < 64u;
-                if (mine) {  // p - q in FP32
-                  const float x = min_nan(exp2_approx(fmaf(s, c2, -z2.x) - z2.y), 1.f) - cur.weight(t2, top, share);
-                  put(cur.id[0] - col, x * coef);
+                if (mine) {
+                  const float q = cur.weight(t2, top, share);
+                  if (!kDistill) {
+                    dot = s;
+                  } else if (q > 0.f) {
+                    dot = fmaf(q, fmaf(s, c2, -from), dot);
+                    run_q += q;
+                  }
                 }
                 cur.drop(w, mine);
+              }
+            } else {
+              // |coef| goes into the exponent
+              T* out = static_cast<T*>(p.d) + (uint64_t)row * p.pitch + t.n * kBN + c;
+              const float2 cc = make_float2(c2, c2), ee = make_float2(e2, e2);
+              if (row < p.rows) {
+#pragma unroll
+                for (int j = 0; j < 64; j += 16) {
+                  uint32_t v[8];
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) {
+                    const float2 x = fma2(make_float2(__uint_as_float(r[j + 2 * e]),
+                                                      __uint_as_float(r[j + 2 * e + 1])), cc, ee);
+                    v[e] = (Type<T>::least(Type<T>::pack(exp2_approx(x.x), exp2_approx(x.y)), most) &
+                            keep) ^ sign;
+                  }
+                  store_v8(out + j, v);
+                }
+              }
+              if constexpr (!kDistill) {  // over the element just stored
+                const bool mine = cur.id[0] - col < 64u;
+                if (__any_sync(0xFFFFFFFFu, mine)) {
+                  if (mine) out[cur.id[0] - col] = Type<T>::from(dead ? nan : at_target);
+                  __syncwarp();
+                }
+              } else {
+                while (__any_sync(0xFFFFFFFFu, cur.id[0] - col < 64u)) {
+                  const float s = pick64(r, cur.id[0] - col);
+                  const bool mine = cur.id[0] - col < 64u;
+                  if (mine) {  // p - q in FP32
+                    const float x = min_nan(exp2_approx(fmaf(s, c2, -z2.x) - z2.y), 1.f) -
+                                    cur.weight(t2, top, share);
+                    out[cur.id[0] - col] = Type<T>::from(x * coef);
+                  }
+                  cur.drop(w, mine);
+                }
               }
             }
           }
@@ -1143,6 +1197,10 @@ engine_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params 
         continue;
       }
       release(buf);
+      if (two) {
+        release(buf ^ 1u);
+        ++sub;
+      }
       cur.fill(w);  // loads that the next tile waits for, not this one
       t.next(p);
     }
@@ -1322,16 +1380,16 @@ __global__ void merge_kernel(Wanted w, const T* hidden, const T* table, uint32_t
 // rows rounded up to 16).  All its scores fit in TMEM, so the softmax needs no
 // running maximum: one pass for each row's maximum over the CTA's range, one
 // for the sum.  TMEM that is left holds each score in up to three segments of its
-// products, added in FP32 (distillation: as many as the gradients' kernel will
-// make; above its 32 rows one, as the tile engine's).  Cross entropy: the target's
-// score comes from the FP32 pipes in the join, in place of the tensor core's.
-// Distillation: the entries in the CTA's range are listed and weighed while the
-// table streams; their scores are those of TMEM, the same numbers that lse and the
-// gradients are made of, laid out in shared memory for any thread to read.
+// products, added in FP32 (distillation: as many as the gradients' kernel makes).
+// Cross entropy: the target's score comes from the FP32 pipes in the join, in place
+// of the tensor core's.  Distillation: the entries in the CTA's range are listed and
+// weighed while the table streams; their scores are those of TMEM, the same numbers
+// that lse and the gradients are made of, laid out in shared memory for any thread
+// to read.
 // Measured (49,152 x 576, fp16, table from DRAM): 13.9 us for 1 row (4.1 TB/s; a
 // read of the table alone takes 8.6 us at 6.55 TB/s), against 24.6 us with the tile
-// engine; the join adds 1.4 us.  Sets of 32 and 300 entries add 0.8 us for 1 row; at
-// 64 rows (18.7 and 21 us) they take less and 1 us more than the targets (19.8).
+// engine; the join adds 1.4 us.  Sets of 32 and 300 entries add 0.8 us for 1 row and
+// 1 and 3 us for 64 (19.7).
 constexpr uint32_t kFewRows = 64;
 constexpr uint32_t kFewMaxStages = 12;
 constexpr uint32_t kFewThreads = 192;  // producer, MMA issuer, 4 epilogue warps
@@ -1380,7 +1438,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_hidden,
   __shared__ uint32_t tmem_at, abort_word, filled;
   __shared__ float2 part[4][kFewRows];
   __shared__ float s_dot[kFewRows];
-  __shared__ int32_t s_at[kDistill ? 2 * kFewRows : 1];       // first entries in the range, and behind it
+  __shared__ int32_t s_at[kDistill ? 2 * kFewRows : 1];  // first entries in the range and behind it
   __shared__ uint32_t s_first[kDistill ? kFewRows + 1 : 1];  // their places in the list
   const uint32_t hid = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t hid_chunk = p.n * 128;
@@ -2544,10 +2602,12 @@ struct FewPlan {
     const uint32_t columns = (range + 127) / 128 * n;
     if (columns > kTmemCols) return;  // scores beyond TMEM
     const uint32_t chunks = (uint32_t)((width + kBK - 1) / kBK);
-    // distillation: the scores that the gradients will have
+    // distillation: the scores that the gradients will have (two segments where the
+    // tile engine makes them)
     const FewGradPlan grad(rows, width, vocab, sms, distill);
     segments = kTmemCols / columns < 3 ? kTmemCols / columns : 3;
-    if (distill) segments = grad.smem > 0 ? grad.segments : 1;
+    if (distill && grad.smem > 0) segments = grad.segments;
+    else if (distill && segments > 2) segments = 2;
     seg_chunks = (chunks + segments - 1) / segments;
     segments = (chunks + seg_chunks - 1) / seg_chunks;
     const uint64_t hid = round_up((width + kBK - 1) / kBK * n * 128, 1024);
@@ -2764,6 +2824,17 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
   p.p_stages = kRingBytes / p.p_stage_bytes < kMaxStages ? kRingBytes / p.p_stage_bytes : kMaxStages;
   p.per_split = plan.per_split;
   p.d_rows = (uint32_t)d_rows;
+  p.score_accs = 1;
+  p.seg_chunks = p.w_chunks;
+  if (kDistill && plan.halves > 1) {  // the scores that the forward call's lse is made of
+    const FewPlan forward(rows, width, vocab, sms, true);
+    const uint32_t first = (p.w_chunks + 1) / 2;
+    if (forward.stages > 0 && forward.segments > 1 && p.w_chunks > 1) {
+      p.score_accs = 2;
+      p.seg_chunks = first;
+      p.score_scale = 1.f + (float)(first * kBK) * kLostPerProduct;
+    }
+  }
   p.r_chunks = (uint32_t)((d_rows + kBK - 1) / kBK);
   p.gmax = gmax;
   p.wide_rows = width % 16 == 0 && (uintptr_t)de % 32 == 0;

@@ -92,3 +92,39 @@ def test_scores_of_parallel_rows(mf, rows, kind):
     assert float(want.min()) > 200  # the parallel row's score alone
     off = float(((lse.double() - want) / want).mean().abs())
     assert off <= 3.3e-9 * width + 4 * 4.5e-7 / math.sqrt(rows), off / width
+
+
+@pytest.mark.parametrize("kind", ("f16", "bf16"))
+@pytest.mark.parametrize("rows,width,products", [(3, 2048, 1024), (20, 2048, 1024),
+                                                 (64, 1024, 512), (64, 2048, 2048),
+                                                 (65, 2048, 2048)])
+def test_few_rows_sum_scores_in_segments(mf, rows, width, products, kind):
+    """The same in distillation, where up to 64 rows sum a score in two segments (as
+    long as the hidden rows leave room beside the table's ring: not 64 of 2,048):
+    what is left is that of half the products.  The gradients agree with it: of a row
+    that is as sure as its teacher, the sum of d stays within lse's rounding and a
+    few of numbers near 1."""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    vocab = 500
+    e = torch.randn(vocab, width, generator=gen, device="cuda")
+    e[:, -64:] = 1.0  # shows the sum of d
+    e = e.to(_dtype(kind))
+    h = (e[:rows].float() / 8).to(_dtype(kind))
+    sets = (torch.arange(rows + 1, dtype=torch.int32, device="cuda"),
+            torch.arange(rows, dtype=torch.int32, device="cuda"), torch.zeros(rows, device="cuda"))
+    loss = mf.DenseLoss(e, rows, stream=torch.cuda.Stream())
+    torch.cuda.synchronize()
+    losses, lse = loss.distill(h, *sets)
+    dh, _ = loss.distill_backward(h, *sets, 1.0, lse, torch.ones(rows, device="cuda"),
+                                  embedding_grad=False)
+    torch.cuda.synchronize()
+    want = torch.logsumexp(h.double() @ e.double().T, 1)
+    assert float(want.min()) > 100  # the parallel row's score alone: p and the loss are 1 and 0
+    off = float(((lse.double() - want) / want).mean().abs())
+    assert off <= 3.3e-9 * products + 4 * 4.5e-7 / math.sqrt(rows), off / products
+    assert float(losses.abs().max()) <= 2.0 ** -20
+    # d is p - 1 at the parallel row, which a clamp keeps at or below 0
+    left = 1.5 * 2.0 ** -24 * want + 2.0 ** -20
+    assert bool((dh[:, -64:].double().abs().amax(1) <= left * (1 + 2.0 ** -7)).all())
