@@ -33,7 +33,7 @@
  * Types: _f16 takes fp16 and _bf16 bfloat16 hidden rows and table; gradients
  * have the type of what they are the gradient of.  Losses, lse, grad_losses
  * and teacher logits are f32, every sum is held in FP32, and d is rounded once
- * to the 16-bit type for the two gradient products (up to 32 rows: to the sum
+ * to the 16-bit type for the two gradient products (up to 64 rows: to the sum
  * of two such numbers).
  * fp16 gradients beyond 65504 become infinite; in d_embedding, what a row of a
  * small weight adds is good to 2^-25 of the call's largest weight, which fp16
@@ -88,9 +88,10 @@ extern "C" {
 #define MF_LOSS_MAX_ENTRIES ((1u << 31) - 1024u)
 
 /* Bytes of device memory that a forward call and a backward call of at most
- * `rows` rows need; 0 for sizes outside the limits.  A backward call's holds up to two pieces of d of at most
- * 128 MiB, a copy of the hidden rows, and FP32 sums of d_hidden of at most 128
- * MiB (4 bytes an element above 32 Mi elements). */
+ * `rows` rows need; 0 for sizes outside the limits.  A backward call's holds up
+ * to two pieces of d of at most 128 MiB, a copy of the hidden rows (two up to 64
+ * rows), and FP32 sums of d_hidden of at most 128 MiB (4 bytes an element above
+ * 32 Mi elements). */
 MF_API uint64_t mf_dense_loss_workspace_bytes(uint64_t rows, uint64_t hidden_size, uint64_t vocab);
 MF_API uint64_t mf_dense_loss_backward_workspace_bytes(uint64_t rows, uint64_t hidden_size,
                                                        uint64_t vocab);

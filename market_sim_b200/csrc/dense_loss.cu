@@ -8,7 +8,9 @@
 // out of the accumulator; a small kernel joins the walks.
 // Backward: the scores again, a piece of the vocabulary at a time, turned into
 // d = T g (p - q) in the epilogue and stored in 16 bits (a piece, never all of
-// it), then two products on the piece: d E into FP32 sums of d_hidden and
+// it; the tensor cores multiply 16-bit numbers, and a second 16 bits would double
+// both products and d's traffic, which only up to 64 rows cost little), then two
+// products on the piece: d E into FP32 sums of d_hidden and
 // d^T H into d_embedding.  One launch makes piece i + 1 of d and the products
 // of piece i, so the many small score tiles fill the SMs that the long product
 // tiles leave idle; a last kernel joins and rounds d_hidden.
@@ -28,9 +30,10 @@
 // a score tile's 64-K chunk take 668 clocks with neither copies nor an epilogue
 // running (1.63 PFLOP/s at the clock seen), 708 with both; the epilogue warps are
 // busy for half of a tile forward and two thirds of one backward.  Long runs
-// are held by the power limit.  Measured (fp16, 8,192 x 49,152 x 576): forward
-// 330 to 350 us (1.33 to 1.40 PFLOP/s), backward 1,127 to 1,160 us (1.20 to
-// 1.23 PFLOP/s over its three products).
+// are held by the power limit.  Measured (fp16, 8,192 x 49,152 x 576): a call alone
+// after idling forward 342 to 370 us (1.25 to 1.36 PFLOP/s), backward 1,165 to 1,224
+// us (1.14 to 1.19 PFLOP/s over its three products); in a run of two seconds, at
+// 1,370 to 1,560 MHz under the power cap, 375 and 1,305 us, a step of both 1,676 us.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
