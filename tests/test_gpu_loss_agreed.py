@@ -155,3 +155,38 @@ def test_sets_that_overlap_and_do_not_ascend(mf, rows):
     _near(losses, ref.losses, ref.losses_off, "losses")
     _near(dh, ref.d_hidden, ref.dh_off, "d_hidden")
     _near(de, ref.d_embedding, ref.de_off, "d_embedding")
+
+
+@pytest.mark.parametrize("kind", ("f16", "bf16"))
+@pytest.mark.parametrize("rows,width", [(7, 648), (33, 576), (48, 1024), (64, 576)])
+def test_same_bits_whatever_the_workspace_held(mf, rows, width, kind):
+    """Few rows of either loss, twice, over workspaces of NaN and of huge numbers."""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    vocab = 9001
+    h = torch.randn(rows, width, generator=gen, device="cuda").to(_dtype(kind))
+    e = (2.0 / math.sqrt(width) * torch.randn(vocab, width, generator=gen, device="cuda")).to(
+        _dtype(kind))
+    t = torch.randint(-1, vocab, (rows,), generator=gen, device="cuda", dtype=torch.int32)
+    keep = torch.rand(rows, vocab, generator=gen, device="cuda") < 0.02
+    offsets = torch.zeros(rows + 1, dtype=torch.int32, device="cuda")
+    offsets[1:] = keep.sum(1).cumsum(0)
+    ids = torch.arange(vocab, device="cuda").expand(rows, vocab)[keep].int()
+    sets = (offsets, ids, 2 * torch.randn(ids.numel(), generator=gen, device="cuda"))
+    grad = torch.rand(rows, generator=gen, device="cuda") - 0.2
+    loss = mf.DenseLoss(e, rows, stream=torch.cuda.Stream())
+    runs = []
+    for fill in (0xFF, 0x7F):
+        out = []
+        for call in (lambda: loss.cross_entropy(h, t), lambda: loss.distill(h, *sets, 2.0),
+                     lambda: loss.cross_entropy_backward(h, t, out[0][1], grad),
+                     lambda: loss.distill_backward(h, *sets, 2.0, out[1][1], grad)):
+            loss.workspace.fill_(fill)
+            torch.cuda.synchronize()
+            out.append(call())
+            torch.cuda.synchronize()
+        runs.append(out)
+    for a, b in zip(*runs):
+        for x, y in zip(a, b):
+            assert bool(torch.isfinite(x).all()) and torch.equal(x, y)

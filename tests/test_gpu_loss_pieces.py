@@ -17,6 +17,8 @@ import math
 
 import pytest
 
+from test_gpu_loss import Reference, _near
+
 pytestmark = pytest.mark.gpu
 
 # 7 pieces and 4 sets; 3 and 1; 5 and 4 of 2 splits; 12 and 11 of 2 splits, the last
@@ -121,3 +123,42 @@ def test_same_bits_whatever_the_workspace_held(mf, rows, vocab, width, kind):
     loss.workspace.fill_(0x7F)
     _, _, none, de = _step(loss, h, t, grad, hidden_grad=False)
     assert none is None and torch.equal(de, want[3])
+
+
+@pytest.mark.parametrize("kind", ("f16", "bf16"))
+@pytest.mark.parametrize("distill", (False, True))
+@pytest.mark.parametrize("rows,width", [(16, 648), (40, 72), (64, 136), (65, 72)])
+def test_few_rows_over_several_pieces(mf, rows, width, distill, kind):
+    """More vocabulary than a piece of one row tile holds (262,144 columns): score
+    tiles of two segments, d in two halves and products share a launch."""
+    import torch
+
+    vocab = 300_000
+    h, e, t, grad = _problem(rows, vocab, width, kind)
+    if distill:
+        gen = torch.Generator(device="cuda").manual_seed(width)
+        ids = torch.randint(0, vocab, (rows, 40), generator=gen, device="cuda").sort(1).values
+        keep = torch.ones_like(ids, dtype=torch.bool)
+        keep[:, 1:] = ids[:, 1:] != ids[:, :-1]
+        offsets = torch.zeros(rows + 1, dtype=torch.int32, device="cuda")
+        offsets[1:] = keep.sum(1).cumsum(0)
+        ids = ids[keep].int()
+        kw = dict(sets=(offsets, ids, 2 * torch.randn(ids.numel(), generator=gen, device="cuda")),
+                  temperature=1.5)
+    else:
+        kw = dict(targets=t)
+    ref = Reference(h, e, kind, grad=grad, **kw)
+    loss = mf.DenseLoss(e, rows, stream=torch.cuda.Stream())
+    loss.workspace.fill_(0xFF)
+    torch.cuda.synchronize()
+    losses, lse = loss.distill(h, *kw["sets"], 1.5) if distill else loss.cross_entropy(h, t)
+    torch.cuda.synchronize()
+    loss.workspace.fill_(0xFF)
+    torch.cuda.synchronize()
+    dh, de = (loss.distill_backward(h, *kw["sets"], 1.5, lse, grad) if distill
+              else loss.cross_entropy_backward(h, t, lse, grad))
+    torch.cuda.synchronize()
+    _near(lse, ref.lse, ref.lse_off, "lse")
+    _near(losses, ref.losses, ref.losses_off, "losses")
+    _near(dh, ref.d_hidden, ref.dh_off, "d_hidden")
+    _near(de, ref.d_embedding, ref.de_off, "d_embedding")
