@@ -205,17 +205,25 @@ def _made_on(stream, device, make):
         return make()
 
 
-def _output_on(stream, device, make):
-    """An output for the caller from the memory of ``stream``, which writes it;
-    a caller on another current stream may read it there and drop it."""
-    t = _made_on(stream, device, make)
-    if stream is not None and device.type == "cuda":
-        import torch
+def _outputs_on(stream, device, *makes):
+    """Outputs for the caller from the memory of ``stream``, which writes them; a
+    caller on another current stream may read them there and drop them.  None
+    stands for an output that is given."""
+    import torch
 
-        current = torch.cuda.current_stream(device)
-        if current.cuda_stream != _stream_handle(stream):
+    def made():
+        return [make and make() for make in makes]
+
+    if stream is None or device.type != "cuda":
+        return made()
+    current = torch.cuda.current_stream(device)
+    if current.cuda_stream == _stream_handle(stream):
+        return made()
+    out = _made_on(stream, device, made)
+    for t in out:
+        if t is not None:
             t.record_stream(current)
-    return t
+    return out
 
 
 class _Workspace:
@@ -548,8 +556,10 @@ class RaggedHead:
 
     ``embedding`` stays resident; each ``__call__`` takes a batch of hidden
     rows and its CSR allowed sets (device tensors) and returns
-    ``(token_ids, scores)`` device tensors.  Without a ``stream`` the
-    constructor waits for the work queued on the current stream.
+    ``(token_ids, scores)`` device tensors, which are made (from the stream's
+    memory, 25 us of host time where it is not the current one) unless given.
+    Without a ``stream`` the constructor waits for the work queued on the
+    current stream.
     """
 
     def __init__(self, embedding, max_rows: int, stream=None):
@@ -570,13 +580,16 @@ class RaggedHead:
         rows = int(hidden.shape[0])
         if rows > self.max_rows:
             raise ValueError(f"batch of {rows} rows exceeds max_rows={self.max_rows}")
-        device = hidden.device
-        if out_ids is None:
-            out_ids = _output_on(self.stream, device,
-                                 lambda: torch.empty(rows, dtype=torch.int32, device=device))
-        if out_scores is None:
-            out_scores = _output_on(self.stream, device,
-                                    lambda: torch.empty(rows, dtype=torch.float32, device=device))
+        if out_ids is None or out_scores is None:
+            device = hidden.device
+            ids_made, scores_made = _outputs_on(
+                self.stream, device,
+                None if out_ids is not None else
+                lambda: torch.empty(rows, dtype=torch.int32, device=device),
+                None if out_scores is not None else
+                lambda: torch.empty(rows, dtype=torch.float32, device=device))
+            out_ids = ids_made if out_ids is None else out_ids
+            out_scores = scores_made if out_scores is None else out_scores
         ws = self.workspace[: head_workspace_bytes(rows)]
         stream = self.stream
         if stream is None:
