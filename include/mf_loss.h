@@ -23,8 +23,8 @@
  * that grows steadily, so d_embedding of more rows in one call would lose what
  * its type holds; larger batches go in slices whose gradients the caller adds.
  *
- * Scores come from the tensor cores: relative to a score, an error of about
- * 1e-9 to 3e-9 a product of its width remains.  A target's own score is summed
+ * Scores come from the tensor cores: relative to a score, an error of up to
+ * about 3e-9 a product of its width remains (bfloat16 2e-9).  A target's own score is summed
  * with rounding to nearest.  A call's losses, lse and gradients are made of the
  * same scores, so where p and q are nearly equal, p - q is good to lse's
  * rounding to f32, 2^-24 |lse|, and the loss to a few 2^-24.

@@ -68,22 +68,25 @@ constexpr uint64_t kPieceBytes = 128ull << 20; // one piece of d
 constexpr uint32_t kHalvesRows = 64;           // up to these, d in two halves
 constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = (float)(1.4426950408889634 - (double)kLog2e);
 constexpr float kLn2 = 0.6931471805599453f, kLn2Low = (float)(0.6931471805599453 - (double)kLn2);
-// The tensor core's additions drop the bits that fall below the sum's last
-// place, so a score of K products comes out too small.  Measured, relative to
-// the score and per product, for K from 128 to 2,048: 1.1e-9 where the products
-// nearly cancel (cosine of the two rows 0.1), 1.4e-9 to 1.9e-9 at cosine 0.3,
-// 2.2e-9 to 2.7e-9 at 0.5, 4.2e-9 to 4.8e-9 at 0.9, with a standard deviation
-// of 1.3e-7 to 4.5e-7 of the score.  Scores are scaled by 1 + K 2^-29.
-constexpr float kLostPerProduct = 1.862645149230957e-9f;
 // A maximum below this (units of ln 2) is that of masked columns: -inf, whose
 // exponential relative to itself is NaN, or a score whose rounding is more than
 // an exponential's range.  Their exponentials are taken as they are, that is 0.
 constexpr float kMasked = -2147483648.f;
 
+// kLostPerProduct: the tensor core's additions drop the bits that fall below the
+// sum's last place, so a score of K products comes out too small, the more the
+// products are of one sign and the more bits they have.  Measured over 16,384 rows
+// for K from 192 to 2,048, relative to the score and per product, in 1e-9:
+//   cosine of the two rows    0.1   0.3   0.5   0.7   0.8   0.9   1
+//   fp16                      1.2   1.7   2.4   2.9   3.5   4.4   4.7 to 6.1
+//   bfloat16                  0.9   1.1   1.2   1.2   1.3   1.6   1.7 to 3.0
+// with a standard deviation of 1e-7 to 4e-7 of the score.  Scores are scaled by 1 + K
+// times a number between those of the rows that a softmax is made of (0.5 and above).
 template <typename T>
 struct Type;
 template <>
 struct Type<__half> {
+  static constexpr float kLostPerProduct = 3e-9f;
   // d / (largest weight) is at most 1: times 2^15 it uses fp16's whole range,
   // and keeps full precision down to 2^-29 of the largest weight
   static constexpr float kScale = 32768.f;
@@ -103,6 +106,7 @@ struct Type<__half> {
 };
 template <>
 struct Type<__nv_bfloat16> {
+  static constexpr float kLostPerProduct = 1.25e-9f;
   static constexpr float kScale = 1.f;
   static constexpr uint32_t kFormat = 1;
   static constexpr CUtensorMapDataType kMap = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -2470,6 +2474,7 @@ cudaError_t launch_after(void (*kernel)(P...), uint64_t blocks, unsigned threads
 }
 
 // What both directions' engine launches share.
+template <typename T>
 Params base_params(uint64_t rows, uint64_t width, uint64_t vocab) {
   Params p = {};
   p.rows = (uint32_t)rows;
@@ -2484,7 +2489,7 @@ Params base_params(uint64_t rows, uint64_t width, uint64_t vocab) {
   if (p.s_stages > kMaxStages) p.s_stages = kMaxStages;
   if (p.keep_hidden && p.s_stages > p.w_chunks) p.s_stages = p.w_chunks;
   p.p_stages = 1;
-  p.score_scale = 1.f + (float)width * kLostPerProduct;
+  p.score_scale = 1.f + (float)width * Type<T>::kLostPerProduct;
   return p;
 }
 
@@ -2623,9 +2628,10 @@ struct FewPlan {
 };
 
 // 1 / T and the correction of scores summed in segments, in units of ln 2.
+template <typename T>
 float few_scale(float inv_t, uint32_t segments, uint32_t seg_chunks, uint64_t width) {
   const uint64_t products = segments == 1 ? width : seg_chunks * kBK;
-  return inv_t * (1.f + (float)products * kLostPerProduct) * kLog2e;
+  return inv_t * (1.f + (float)products * Type<T>::kLostPerProduct) * kLog2e;
 }
 
 template <typename T, bool kDistill>
@@ -2645,7 +2651,7 @@ mf_status forward_few(const FewPlan& few, Wanted w, const T* hidden, const T* ta
   p.stages = few.stages;
   p.segments = few.segments;
   p.seg_chunks = few.seg_chunks;
-  p.c2 = few_scale(w.inv_t, few.segments, few.seg_chunks, width);
+  p.c2 = few_scale<T>(w.inv_t, few.segments, few.seg_chunks, width);
   p.entries = (uint32_t)entries;
   p.partial = static_cast<Partial*>(partial);
   p.local = static_cast<float*>(local);
@@ -2704,7 +2710,7 @@ mf_status forward(Span hidden, Span embedding, Span targets, Span ids, Span logi
   }
   const uint64_t total = plan.m_tiles * plan.n_tiles;
   if (pairs > total) pairs = (uint32_t)total;
-  Params p = base_params(rows, width, vocab);
+  Params p = base_params<T>(rows, width, vocab);
   p.cols = (uint32_t)vocab;
   p.n_tiles = (uint32_t)plan.n_tiles;
   p.partial = reinterpret_cast<Partial*>(ws + plan.partial);
@@ -2789,7 +2795,7 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
     f.range = few.range;
     f.segments = few.segments;
     f.seg_chunks = few.seg_chunks;
-    f.c2 = few_scale(w.inv_t, few.segments, few.seg_chunks, width);
+    f.c2 = few_scale<T>(w.inv_t, few.segments, few.seg_chunks, width);
     f.hidden = hidden.p;
     f.table = embedding.p;
     f.grad = static_cast<const float*>(grad.p);
@@ -2816,7 +2822,7 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
                      gmax, (uint32_t)rows, (uint32_t)width, (uint32_t)vocab, plan.halves);
   if (err != cudaSuccess) return launched(err);
 
-  Params p = base_params(rows, width, vocab);
+  Params p = base_params<T>(rows, width, vocab);
   p.lse = static_cast<const float*>(lse.p);
   p.rg = rg;
   p.bn = plan.bn;
@@ -2835,7 +2841,7 @@ mf_status backward(Span hidden, Span embedding, Span targets, Span ids, Span log
     if (forward.stages > 0 && forward.segments > 1 && p.w_chunks > 1) {
       p.score_accs = 2;
       p.seg_chunks = first;
-      p.score_scale = 1.f + (float)(first * kBK) * kLostPerProduct;
+      p.score_scale = 1.f + (float)(first * kBK) * Type<T>::kLostPerProduct;
     }
   }
   p.r_chunks = (uint32_t)((d_rows + kBK - 1) / kBK);
