@@ -7,7 +7,7 @@ at most 2 p (1 - p) s and the loss by s sum |p - q|, as long as loss, lse and gr
 are made of the same ones.  Beyond that only roundings of numbers near 1 remain:
 2^-20 relative of q, log q and exponentials, `steps` additions of 2^-24 in the
 sum, and lse's rounding to FP32, 2^-24 |lse|, which the gradient sees.  d is rounded
-once (u |d|; fp16 below its range by 2^-40 of the weight; up to 32 rows to two
+once (u |d|; fp16 below its range by 2^-40 of the weight; up to 64 rows to two
 16-bit numbers), the products add in FP32, the result is rounded once.
 """
 from __future__ import annotations
